@@ -63,8 +63,35 @@ class FsAdamLayout(_Int64Fields):
     ]
 
 
+TYPE_F32 = 0
+TYPE_F16 = 1
+TYPE_BF16 = 2
+PRODUCTS_HALF = 1
+PRODUCTS_SPLIT = 2
+
+
+class FsMomentumTensor(ctypes.Structure):
+    _fields_ = [("g", ctypes.c_void_p), ("m", ctypes.c_void_p), ("u", ctypes.c_void_p), ("numel", ctypes.c_int64)]
+
+
+class FsOrthOptions(ctypes.Structure):
+    _fields_ = [("a", ctypes.c_float), ("b", ctypes.c_float), ("c", ctypes.c_float), ("eps", ctypes.c_float),
+                ("steps", ctypes.c_int32), ("products", ctypes.c_int32)]
+
+
+class FsMatrix(ctypes.Structure):
+    _fields_ = [("src", ctypes.c_void_p), ("dst", ctypes.c_void_p)] + [
+        (name, ctypes.c_int64) for name in ("batch", "rows", "cols", "src_ld", "src_stride", "dst_ld", "dst_stride")]
+
+
+class FsMuonTensor(ctypes.Structure):
+    _fields_ = [("p", ctypes.c_void_p), ("g", ctypes.c_void_p), ("m", ctypes.c_void_p), ("p_copy", ctypes.c_void_p),
+                ("batch", ctypes.c_int64), ("rows", ctypes.c_int64), ("cols", ctypes.c_int64), ("ratio", ctypes.c_double)]
+
+
 # name -> (restype, argtypes); one entry per function include/fsadam.h declares
 _f32, _i32, _i64, _vp = ctypes.c_float, ctypes.c_int, ctypes.c_int64, ctypes.c_void_p
+_f64 = ctypes.c_double
 _SCALARS = [_f32, _f32, _f32, _f32, _f32, _f32, _f32, _i32, _i32, _i32]
 SIGNATURES = {
     "fsadam_version": (_i32, []),
@@ -87,6 +114,15 @@ SIGNATURES = {
     "fsadam_grad_pass": (_i32, [ctypes.POINTER(FsGradTensor), _i64, _i32, _f32, _vp, _i32, _vp, _vp, _vp, _vp]),
     "fsadam_grad_pass_noalloc": (_i32, [ctypes.POINTER(FsGradTensor), _i64, _i32, _f32, _vp, _i32, _vp, _vp, _vp, _vp]),
     "fsadam_clear_cache": (_i32, []),
+    "fsadam_momentum_workspace": (_i32, [ctypes.POINTER(FsMomentumTensor), _i64, ctypes.POINTER(_i64)]),
+    # tensors, n, grad_type, update_type, momentum, nesterov, scale, scale_dev, norms, found_inf, workspace, bytes, stream
+    "fsadam_momentum_pass": (_i32, [ctypes.POINTER(FsMomentumTensor), _i64, _i32, _i32, _f64, _i32, _f32, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "fsadam_orth_workspace": (_i32, [ctypes.POINTER(FsMatrix), _i64, ctypes.POINTER(FsOrthOptions), ctypes.POINTER(_i64)]),
+    "fsadam_orthogonalize": (_i32, [ctypes.POINTER(FsMatrix), _i64, _i32, ctypes.POINTER(FsOrthOptions), _vp, _i64, _vp]),
+    "fsadam_muon_workspace": (_i32, [ctypes.POINTER(FsMuonTensor), _i64, ctypes.POINTER(FsOrthOptions), ctypes.POINTER(_i64)]),
+    # tensors, n, param_type, grad_type, copy_type, options, lr, momentum, nesterov, weight_decay, scale, scale_dev, workspace, bytes, stream
+    "fsadam_muon_step": (_i32, [ctypes.POINTER(FsMuonTensor), _i64, _i32, _i32, _i32, ctypes.POINTER(FsOrthOptions), _f64, _f64, _i32, _f64, _f32,
+                                _vp, _vp, _i64, _vp]),
 }
 
 _lib: Optional[ctypes.CDLL] = None

@@ -1,4 +1,4 @@
-"""Compiles fsadam.hip (with the kernel headers next to it) into libfsadam.so next to this file (hipcc, gfx950 only), and the host-side
+"""Compiles fsadam.hip and matrix.hip (with the kernel headers next to them) into libfsadam.so next to this file (hipcc, gfx950 only), and the host-side
 helper tensor_rows.cpp into a CPython extension module (g++, against the installed torch).
 
 Usage: ``python -m fairscale_amd.csrc.build`` (``--membench``: the microbenchmark library instead), or ``build_library()`` /
@@ -14,7 +14,7 @@ import sys
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 REPO = os.path.dirname(os.path.dirname(HERE))
-SOURCE = os.path.join(HERE, "fsadam.hip")
+SOURCES = [os.path.join(HERE, "fsadam.hip"), os.path.join(HERE, "matrix.hip")]
 LIBRARY = os.path.join(HERE, "libfsadam.so")
 INCLUDE = os.path.join(REPO, "include")
 
@@ -37,7 +37,7 @@ def hipcc_path() -> str:
 def build_library(verbose: bool = False) -> str:
     """Always recompiles; returns the path of the shared library."""
     target = LIBRARY
-    cmd = [hipcc_path(), *HIPCC_FLAGS, "-I", INCLUDE, "-I", HERE, "-o", target + ".tmp", SOURCE]
+    cmd = [hipcc_path(), *HIPCC_FLAGS, "-I", INCLUDE, "-I", HERE, "-o", target + ".tmp", *SOURCES]
     proc = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
     noise = "is not a recognized feature for this target"  # the host pass does not know the device feature
     log = "\n".join(line for line in proc.stdout.splitlines() if noise not in line)

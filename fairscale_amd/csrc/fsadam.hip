@@ -1020,6 +1020,15 @@ bool same_options(const Options& a, const Options& b) {
 
 }  // namespace
 
+// matrix.hip's errors share the thread's message.
+__attribute__((visibility("hidden"))) int fsadam_fail(int code, const char* msg) noexcept {
+    try {
+        g_last_error = msg;
+    } catch (...) {  // no memory for the message: the code stands alone
+    }
+    return code;
+}
+
 extern "C" {
 
 int fsadam_version(void) { return FSADAM_ABI_VERSION; }

@@ -1,0 +1,619 @@
+// Kernels of the matrix operators: momentum pass, normalisation, the Newton-Schulz products.
+// Included by matrix.hip only.
+//
+// The iteration.  For U (rows x cols) let X be U / max(|U|_F, eps), turned so that its short side s comes first
+// (s x l, s <= l).  One step with coefficients (a, b, c) is
+//     A = X X^T,    B = b A + c A A,    X <- a X + B X,
+// which maps every singular value x of X to a x + b x^3 + c x^5 and leaves the singular vectors.  A and B are
+// symmetric: only the tiles on and under their diagonal are computed, each is stored at its mirror place too.
+//
+// How numbers are held.  Frobenius norm 1 bounds the singular values of X0 by 1; the host follows that bound through
+// the polynomial (step_bounds in matrix.hip), and no entry of a matrix is larger than its largest singular value.  So
+// X, A and B are kept as halves times a power of two that the bound allows: 11 bits each and no overflow, which
+// bfloat16 (8 bits) would pay for a range that is not needed.  A second half holds what the first leaves over (22 bits):
+//   * X always has it, for the term a X: a > 3 there multiplies the rounding of X at every step, and for directions
+//     of small singular values nothing takes it back (rounding X to 11 bits: error 4e-2 after five steps on a matrix
+//     of rank 8 plus 1 % noise; with the second half 4e-4, simulated against 64 bits);
+//   * with PLANES == 2 the products use it as well: hi hi + hi lo + lo hi in one fp32 accumulator, three matrix
+//     instructions in place of one, and errors like those of fp32 products (the dropped lo lo is 2^-22 of the sum).
+// Sums are held in fp32 (matrix instructions), norms in fp64.
+//
+// Storage in the workspace, all sizes padded to 64 with zeros (zero rows and columns stay zero through the iteration,
+// so no product needs a mask): X is s64 x l64, A and B are s64 x s64, row-major, the planes one behind the other.
+#pragma once
+
+#include <cstdint>
+
+namespace {
+
+typedef _Float16 half4_t __attribute__((ext_vector_type(4)));
+typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
+typedef short short4_t __attribute__((ext_vector_type(4)));
+typedef float float4_t __attribute__((ext_vector_type(4)));
+
+#define FM_LDS __attribute__((address_space(3)))
+#define FM_GLOBAL __attribute__((address_space(1)))
+
+enum { kTypeF32 = 0, kTypeF16 = 1, kTypeBF16 = 2 };
+
+// Which of a row's tile counts a launch goes by.
+enum { kTilesSym128, kTilesFull128, kTilesSym256, kTilesFull256, kTilesPrep, kTilesChunk, kTileKinds };
+
+// One row of a call's table: `batch` matrices of one shape, equally spaced.
+struct alignas(16) MatrixRow {
+    const void* src;   // orthogonalize: the matrices.  step: the gradients
+    float* buf;        // step: the momentum
+    void* dst;         // orthogonalize: the results.  step: the parameters (fp32 masters in mixed precision)
+    void* copy;        // step, mixed precision: the 16-bit parameters
+    int64_t src_ld, src_stride, dst_ld, dst_stride;  // elements from row to row, from matrix to matrix
+    int64_t x_off[2];  // workspace: X and its successor (halves from the workspace's start)
+    int64_t a_off, b_off;
+    int32_t batch, rows, cols;
+    int32_t s, l, s64, l64;
+    int32_t tall;      // rows > cols: X is the transpose
+    int32_t first_matrix;           // index of the row's first matrix in the chunk
+    int32_t chunks;                 // partial sums per matrix
+    float step_ratio;               // step: lr * ratio of this shape
+    int32_t first[kTileKinds];      // tiles of the rows before this one
+    int32_t n[kTileKinds];          // tiles of one matrix
+};
+
+__device__ __forceinline__ float load_as_float(const void* p, int64_t i, int type) {
+    if (type == kTypeF32) return static_cast<const float*>(p)[i];
+    if (type == kTypeF16) return (float)static_cast<const _Float16*>(p)[i];
+    return __builtin_bit_cast(float, (uint32_t)static_cast<const uint16_t*>(p)[i] << 16);
+}
+// Round to nearest even; NaN stays NaN.
+__device__ __forceinline__ uint16_t bf16_bits(float v) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, v);
+    if ((u & 0x7fffffffu) > 0x7f800000u) return (uint16_t)((u >> 16) | 0x40u);
+    return (uint16_t)((u + 0x7fffu + ((u >> 16) & 1u)) >> 16);
+}
+__device__ __forceinline__ void store_from_float(void* p, int64_t i, int type, float v) {
+    if (type == kTypeF32) static_cast<float*>(p)[i] = v;
+    else if (type == kTypeF16) static_cast<_Float16*>(p)[i] = (_Float16)v;
+    else static_cast<uint16_t*>(p)[i] = bf16_bits(v);
+}
+// What a stored value of this type reads back as.
+__device__ __forceinline__ float round_to(float v, int type) {
+    if (type == kTypeF32) return v;
+    if (type == kTypeF16) return (float)(_Float16)v;
+    return __builtin_bit_cast(float, (uint32_t)bf16_bits(v) << 16);
+}
+
+__device__ __forceinline__ void split_halves(float v, _Float16& hi, _Float16& lo) {
+    hi = (_Float16)v;
+    lo = (_Float16)(v - (float)hi);
+}
+
+// Workgroups are handed to the 8 XCDs in turn, each with an L2 of its own: give every XCD a contiguous range of tiles.
+__device__ __forceinline__ uint32_t xcd_contiguous(uint32_t block, uint32_t n) {
+    const uint32_t per = n / 8, extra = n % 8, xcd = block % 8, at = block / 8;
+    return xcd * per + (xcd < extra ? xcd : extra) + at;
+}
+
+// The row, the matrix in it and the tile in that of the launch's tile `t`.
+__device__ __forceinline__ const MatrixRow& find_tile(const MatrixRow* table, int n_rows, int kind, uint32_t t, int& matrix, uint32_t& tile) {
+    int low = 0, high = n_rows - 1;
+    while (low < high) {
+        const int mid = (low + high + 1) >> 1;
+        if ((uint32_t)table[mid].first[kind] <= t) low = mid;
+        else high = mid - 1;
+    }
+    const MatrixRow& row = table[low];
+    const uint32_t at = t - (uint32_t)row.first[kind], per = (uint32_t)row.n[kind];
+    matrix = (int)(at / per);
+    tile = at - (uint32_t)matrix * per;
+    return row;
+}
+
+// ---- momentum -----------------------------------------------------------------------------------------------------
+
+struct MomentumArgs {
+    const float* scale_dev;  // when not NULL the gradients are divided by this instead of `scale`
+    float scale;
+    float momentum, one_minus;
+    int nesterov;
+};
+
+//     r = g / scale;   m <- m + (1 - mu) (r - m);   u = nesterov ? r + mu (m - r) : m
+__device__ __forceinline__ float momentum_update(float g, float& m, float scale, const MomentumArgs& k) {
+    const float r = g / scale;
+    m = m + (r - m) * k.one_minus;
+    return k.nesterov ? r + (m - r) * k.momentum : m;
+}
+__device__ __forceinline__ float update_again(float g, float m, float scale, const MomentumArgs& k) {  // from the stored m
+    const float r = g / scale;
+    return k.nesterov ? r + (m - r) * k.momentum : m;
+}
+
+constexpr int kChunkThreads = 256;
+constexpr int kChunkElems = 8192;  // elements of one partial sum
+
+// Sum over a workgroup of 256 in a fixed order; the result is valid in thread 0.
+__device__ __forceinline__ double block_sum(double v) {
+    __shared__ double part[4];
+    for (int d = 32; d > 0; d >>= 1) v += __shfl_down(v, d);
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+    __syncthreads();
+    return part[0] + part[1] + part[2] + part[3];
+}
+
+// One row of the momentum pass's table: a tensor as a line of elements.
+struct alignas(16) MomentumRow {
+    const void* g;
+    float* m;
+    void* u;          // NULL: the update is not stored (the step takes it from g and m again)
+    int64_t numel;
+    int64_t first;    // chunks of the rows before this one
+};
+
+template <int GT, int UT>
+__global__ __launch_bounds__(kChunkThreads) void fsadam_momentum_chunks(const MomentumRow* table, int n_rows, MomentumArgs k, double* partials) {
+    int low = 0, high = n_rows - 1;
+    const int64_t t = blockIdx.x;
+    while (low < high) {
+        const int mid = (low + high + 1) >> 1;
+        if (table[mid].first <= t) low = mid;
+        else high = mid - 1;
+    }
+    const MomentumRow& row = table[low];
+    const int64_t begin = (t - row.first) * kChunkElems;
+    const int64_t end = begin + kChunkElems < row.numel ? begin + kChunkElems : row.numel;
+    const float scale = k.scale_dev ? *k.scale_dev : k.scale;
+    double sum = 0.0;
+    for (int64_t i = begin + threadIdx.x; i < end; i += kChunkThreads) {
+        float m = row.m[i];
+        const float u = momentum_update(load_as_float(row.g, i, GT), m, scale, k);
+        row.m[i] = m;
+        if (row.u) store_from_float(row.u, i, UT, u);
+        const double r = row.u ? (double)round_to(u, UT) : (double)u;
+        sum += r * r;
+    }
+    sum = block_sum(sum);
+    if (threadIdx.x == 0) partials[t] = sum;
+}
+
+// norms[row] = sqrt of the row's sum of squares; found_inf is raised where that is not finite (a double holds the sum of
+// squares of any floats, so it is not finite exactly where an update is not).
+__global__ __launch_bounds__(kChunkThreads) void fsadam_momentum_norms(const MomentumRow* table, const double* partials, float* norms, float* found_inf) {
+    const MomentumRow& row = table[blockIdx.x];
+    const int64_t n = (row.numel + kChunkElems - 1) / kChunkElems;
+    double sum = 0.0;
+    for (int64_t i = threadIdx.x; i < n; i += kChunkThreads) sum += partials[row.first + i];
+    sum = block_sum(sum);
+    if (threadIdx.x == 0) {
+        if (norms) norms[blockIdx.x] = (float)sqrt(sum);
+        if (found_inf && !__builtin_isfinite(sum)) *found_inf = 1.0f;
+    }
+}
+
+// ---- norms and normalisation of the matrices ----------------------------------------------------------------------
+
+// STEP: the source is the gradient, the momentum is updated and what is summed is the update.
+template <int ST, bool STEP>
+__global__ __launch_bounds__(kChunkThreads) void fsadam_matrix_chunks(const MatrixRow* table, int n_rows, MomentumArgs k, double* partials) {
+    int matrix;
+    uint32_t chunk;
+    const MatrixRow& row = find_tile(table, n_rows, kTilesChunk, blockIdx.x, matrix, chunk);
+    const int64_t numel = (int64_t)row.rows * row.cols;
+    const int64_t begin = (int64_t)chunk * kChunkElems;
+    const int64_t end = begin + kChunkElems < numel ? begin + kChunkElems : numel;
+    double sum = 0.0;
+    if constexpr (STEP) {
+        const float scale = k.scale_dev ? *k.scale_dev : k.scale;
+        const int64_t base = (int64_t)matrix * numel;
+        for (int64_t i = begin + threadIdx.x; i < end; i += kChunkThreads) {
+            float m = row.buf[base + i];
+            const double u = (double)momentum_update(load_as_float(row.src, base + i, ST), m, scale, k);
+            row.buf[base + i] = m;
+            sum += u * u;
+        }
+    } else {
+        const int64_t base = (int64_t)matrix * row.src_stride;
+        for (int64_t i = begin + threadIdx.x; i < end; i += kChunkThreads) {
+            const int64_t r = i / row.cols;
+            const double u = (double)load_as_float(row.src, base + r * row.src_ld + (i - r * row.cols), ST);
+            sum += u * u;
+        }
+    }
+    sum = block_sum(sum);
+    if (threadIdx.x == 0) partials[blockIdx.x] = sum;
+}
+
+// One workgroup per matrix: inverse[matrix] = 1 / max(norm, eps), NaN where the norm is not finite (every entry of the
+// result is then NaN, which is what one product of the iteration would make of it).
+__global__ __launch_bounds__(kChunkThreads) void fsadam_matrix_norms(const MatrixRow* table, int n_rows, double eps, const double* partials, double* inverse) {
+    int low = 0, high = n_rows - 1;
+    while (low < high) {
+        const int mid = (low + high + 1) >> 1;
+        if (table[mid].first_matrix <= (int)blockIdx.x) low = mid;
+        else high = mid - 1;
+    }
+    const MatrixRow& row = table[low];
+    const double* p = partials + row.first[kTilesChunk] + (int64_t)((int)blockIdx.x - row.first_matrix) * row.chunks;
+    double sum = 0.0;
+    for (int i = threadIdx.x; i < row.chunks; i += kChunkThreads) sum += p[i];
+    sum = block_sum(sum);
+    if (threadIdx.x == 0) {
+        const double norm = sqrt(sum);
+        inverse[blockIdx.x] = __builtin_isfinite(sum) ? 1.0 / (norm > eps ? norm : eps) : __builtin_nan("");
+    }
+}
+
+// X0 * 2^k as two halves, 64 x 64 elements a workgroup, turned where the matrix is tall; the padding is written as zeros.
+template <int ST, bool STEP>
+__global__ __launch_bounds__(256) void fsadam_matrix_normalise(const MatrixRow* table, int n_rows, MomentumArgs k, const double* inverse, double power, _Float16* work) {
+    __shared__ float tile[64][65];
+    int matrix;
+    uint32_t t;
+    const MatrixRow& row = find_tile(table, n_rows, kTilesPrep, blockIdx.x, matrix, t);
+    const uint32_t across = (uint32_t)row.l64 / 64;
+    const int i0 = (int)(t / across) * 64, j0 = (int)(t % across) * 64;  // in X
+    const int r0 = row.tall ? j0 : i0, c0 = row.tall ? i0 : j0;         // in the source
+    const double factor = inverse[row.first_matrix + matrix] * power;
+    const float scale = STEP ? (k.scale_dev ? *k.scale_dev : k.scale) : 1.0f;
+    for (int e = threadIdx.x; e < 64 * 64; e += 256) {
+        const int r = e >> 6, c = e & 63;
+        float v = 0.0f;
+        if (r0 + r < row.rows && c0 + c < row.cols) {
+            float u;
+            if constexpr (STEP) {
+                const int64_t at = (int64_t)matrix * row.rows * row.cols + (int64_t)(r0 + r) * row.cols + c0 + c;
+                u = update_again(load_as_float(row.src, at, ST), row.buf[at], scale, k);
+            } else {
+                u = load_as_float(row.src, (int64_t)matrix * row.src_stride + (int64_t)(r0 + r) * row.src_ld + c0 + c, ST);
+            }
+            v = (float)((double)u * factor);
+        }
+        tile[r][c] = v;
+    }
+    __syncthreads();
+    const int64_t plane = (int64_t)row.s64 * row.l64;
+    _Float16* x = work + row.x_off[0] + (int64_t)matrix * 2 * plane;
+    for (int e = threadIdx.x; e < 64 * 8; e += 256) {
+        const int i = e >> 3, j = (e & 7) * 8;
+        half8_t hi, lo;
+        for (int q = 0; q < 8; ++q) {
+            const float v = row.tall ? tile[j + q][i] : tile[i][j + q];
+            _Float16 h, o;
+            split_halves(v, h, o);
+            hi[q] = h;
+            lo[q] = o;
+        }
+        const int64_t at = (int64_t)(i0 + i) * row.l64 + j0 + j;
+        *reinterpret_cast<half8_t*>(x + at) = hi;
+        *reinterpret_cast<half8_t*>(x + plane + at) = lo;
+    }
+}
+
+// ---- the products -------------------------------------------------------------------------------------------------
+
+enum { kStageGram, kStagePoly, kStageUpdate, kStageOut, kStageStep };
+
+struct StageArgs {
+    int from, to;       // which of the two X buffers is read and written
+    float linear, product;  // result = linear * (what is added) + product * (accumulator), powers of two included
+    float keep;         // step: 1 - lr * weight_decay
+    int dst_type, copy_type;  // out, step: kType*; copy_type < 0: no copies
+};
+
+// A tile's operand panel in LDS, K contiguous ("NT"): `rows` x BK halves, 16-byte chunks of a row exchanged (xor) so that
+// the 16 rows a fragment reads spread over the banks.
+template <int BK>
+__device__ __forceinline__ int swizzle_nt(int row) {
+    return BK == 64 ? (row & 7) : ((row >> 1) & 3);
+}
+// K x columns ("NN", read with the transposing LDS loads): pairs of chunks (32 bytes, 16 columns) exchanged so that the rows
+// one load touches (8g + 0..3 for the four groups g of 16 lanes) spread over the banks.
+__device__ __forceinline__ int swizzle_nn(int row) { return (row & 3) | (((row >> 3) & 1) << 2); }
+
+// 1 KiB straight from memory into LDS: every lane gives the address of 16 bytes, which land at dst + 16 * lane.
+// From assembly because of the wait: behind the builtin the compiler places a wait for ALL loads before the next read
+// of LDS (it cannot tell the buffer being filled from the one being read), which takes away the overlap the two
+// buffers are there for.  The statement has no output register; what it writes is LDS, and nothing reads that before
+// loads_arrived() and the barrier behind it.  m0 is a reserved register: the compiler writes it right before each use of
+// its own and keeps nothing in it.  The s_nop: a write of m0 needs one wait state before the load that uses it.
+__device__ __forceinline__ void load_to_lds(const _Float16* src, uint32_t dst) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(dst), "v"((const FM_GLOBAL void*)src) : "memory");
+}
+__device__ __forceinline__ void loads_arrived() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ uint32_t lds_address(const void* p) { return (uint32_t)(uintptr_t)(FM_LDS const void*)p; }
+
+// C tile (TM x TN) = P Q^T (NT) or P Q (NN) over K, by WM x WN waves; the caller's epilogue takes acc.
+template <int TM, int TN, int WM, int WN, int BK, int PLANES, bool NN>
+struct Product {
+    static constexpr int kThreads = 64 * WM * WN, kWaves = WM * WN;
+    static constexpr int MI = TM / WM / 16, NJ = TN / WN / 16;
+    static constexpr int kPanelP = TM * BK, kPanelQ = TN * BK;             // halves of one plane
+    static constexpr int kStageHalves = PLANES * (kPanelP + kPanelQ);
+    static constexpr int kLdsHalves = 2 * kStageHalves;
+    static constexpr int kLoadsP = kPanelP / 512 / kWaves, kLoadsQ = kPanelQ / 512 / kWaves;  // 1 KiB loads of a wave, one plane
+    static_assert(kLoadsP * 512 * kWaves == kPanelP && kLoadsQ * 512 * kWaves == kPanelQ, "panels divide among the waves");
+
+    float4_t acc[MI][NJ];
+
+    // p: first row of the panel, rows_p: how many rows there are from it on (further ones are read as the last);
+    // q: NT as p; NN the panel's first column, cols_q columns from it on.
+    __device__ __forceinline__ void run(const _Float16* p, int64_t ld_p, int64_t plane_p, int rows_p, const _Float16* q, int64_t ld_q, int64_t plane_q,
+                                        int rows_q, int k_total, _Float16* lds) {
+        const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        const int wm = wave / WN, wn = wave % WN;
+        uint32_t off_p[kLoadsP], off_q[kLoadsQ];
+#pragma unroll
+        for (int n = 0; n < kLoadsP; ++n) {
+            int r = (wave * kLoadsP + n) * (512 / BK) + lane / (BK / 8);
+            const int chunk = (lane % (BK / 8)) ^ swizzle_nt<BK>(r);
+            r = r < rows_p ? r : rows_p - 1;
+            off_p[n] = (uint32_t)(r * ld_p + chunk * 8);
+        }
+#pragma unroll
+        for (int n = 0; n < kLoadsQ; ++n) {
+            if constexpr (NN) {
+                constexpr int kChunks = TN / 8;  // of a row
+                const int r = (wave * kLoadsQ + n) * (64 / kChunks) + lane / kChunks;
+                const int slot = lane % kChunks;
+                int chunk = (((slot >> 1) ^ swizzle_nn(r)) << 1) | (slot & 1);
+                const int last = rows_q / 8 - 1;
+                chunk = chunk < last ? chunk : last;
+                off_q[n] = (uint32_t)(r * ld_q + chunk * 8);
+            } else {
+                int r = (wave * kLoadsQ + n) * (512 / BK) + lane / (BK / 8);
+                const int chunk = (lane % (BK / 8)) ^ swizzle_nt<BK>(r);
+                r = r < rows_q ? r : rows_q - 1;
+                off_q[n] = (uint32_t)(r * ld_q + chunk * 8);
+            }
+        }
+        const int64_t advance_q = NN ? (int64_t)BK * ld_q : BK;
+        const uint32_t lds_at = __builtin_amdgcn_readfirstlane((int)lds_address(lds));
+        auto fetch = [&](uint32_t stage) {
+#pragma unroll
+            for (int plane = 0; plane < PLANES; ++plane) {
+                const _Float16* gp = p + plane * plane_p;
+                const _Float16* gq = q + plane * plane_q;
+                const uint32_t lp = stage + 2 * (plane * kPanelP + wave * kLoadsP * 512);
+                const uint32_t lq = stage + 2 * (PLANES * kPanelP + plane * kPanelQ + wave * kLoadsQ * 512);
+#pragma unroll
+                for (int n = 0; n < kLoadsP; ++n) load_to_lds(gp + off_p[n], lp + n * 1024);
+#pragma unroll
+                for (int n = 0; n < kLoadsQ; ++n) load_to_lds(gq + off_q[n], lq + n * 1024);
+            }
+            p += BK;
+            q += advance_q;
+        };
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) acc[i][j] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+
+        const int g = lane >> 4, c = lane & 15;
+        const int row_p = wm * (TM / WM) + c, row_q = wn * (TN / WN) + c;
+        const int turn_p = swizzle_nt<BK>(row_p), turn_q = swizzle_nt<BK>(row_q);
+        int nn_at[NJ];
+        if constexpr (NN) {
+            const int r = 8 * g + (c >> 2);
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) nn_at[j] = r * TN + (((wn * (TN / WN) / 16 + j) ^ swizzle_nn(r)) * 16) + (c & 3) * 4;
+        }
+
+        fetch(lds_at);
+        loads_arrived();
+        __syncthreads();
+        const int n_k = k_total / BK;
+        for (int step = 0; step < n_k; ++step) {
+            _Float16* now = lds + (step & 1) * kStageHalves;
+            if (step + 1 < n_k) fetch(lds_at + ((step + 1) & 1) * kStageHalves * 2);
+#pragma unroll
+            for (int kk = 0; kk < BK / 32; ++kk) {
+                half8_t fp[PLANES][MI], fq[PLANES][NJ];
+#pragma unroll
+                for (int plane = 0; plane < PLANES; ++plane) {
+                    const _Float16* lp = now + plane * kPanelP + row_p * BK + ((kk * 4 + g) ^ turn_p) * 8;
+                    const _Float16* lq = now + PLANES * kPanelP + plane * kPanelQ;
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j) {
+                        if constexpr (NN) {
+                            const short4_t low = __builtin_amdgcn_ds_read_tr16_b64_v4i16((FM_LDS short4_t*)(lq + nn_at[j] + kk * 32 * TN));
+                            const short4_t high = __builtin_amdgcn_ds_read_tr16_b64_v4i16((FM_LDS short4_t*)(lq + nn_at[j] + (kk * 32 + 4) * TN));
+                            const half4_t l4 = __builtin_bit_cast(half4_t, low), h4 = __builtin_bit_cast(half4_t, high);
+                            fq[plane][j] = __builtin_shufflevector(l4, h4, 0, 1, 2, 3, 4, 5, 6, 7);
+                        } else {
+                            fq[plane][j] = *reinterpret_cast<const half8_t*>(lq + row_q * BK + ((kk * 4 + g) ^ turn_q) * 8 + j * 16 * BK);
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < MI; ++i) fp[plane][i] = *reinterpret_cast<const half8_t*>(lp + i * 16 * BK);
+                }
+#pragma unroll
+                for (int i = 0; i < MI; ++i)
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j) {
+                        if constexpr (PLANES == 2) {
+                            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fp[1][i], fq[0][j], acc[i][j], 0, 0, 0);
+                            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fp[0][i], fq[1][j], acc[i][j], 0, 0, 0);
+                        }
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fp[0][i], fq[0][j], acc[i][j], 0, 0, 0);
+                    }
+            }
+            loads_arrived();
+            __syncthreads();
+        }
+    }
+};
+
+// Eight values as one or two planes of halves.
+template <int PLANES>
+__device__ __forceinline__ void store_planes(_Float16* at, int64_t plane, const float (&v)[8]) {
+    half8_t hi, lo;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+        _Float16 h, o;
+        split_halves(v[q], h, o);
+        hi[q] = h;
+        lo[q] = o;
+    }
+    *reinterpret_cast<half8_t*>(at) = hi;
+    if constexpr (PLANES == 2) *reinterpret_cast<half8_t*>(at + plane) = lo;
+}
+template <int PLANES>
+__device__ __forceinline__ void load_planes(const _Float16* at, int64_t plane, float (&v)[8]) {
+    const half8_t hi = *reinterpret_cast<const half8_t*>(at);
+#pragma unroll
+    for (int q = 0; q < 8; ++q) v[q] = (float)hi[q];
+    if constexpr (PLANES == 2) {
+        const half8_t lo = *reinterpret_cast<const half8_t*>(at + plane);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) v[q] += (float)lo[q];
+    }
+}
+
+// One stage of the iteration over every matrix of the chunk.
+template <int STAGE, int TM, int TN, int WM, int WN, int BK, int PLANES>
+__global__ __launch_bounds__(64 * WM * WN) void fsadam_matrix_stage(const MatrixRow* table, int n_rows, StageArgs k, _Float16* work) {
+    constexpr bool kSym = STAGE == kStageGram || STAGE == kStagePoly;
+    constexpr bool kNN = !kSym;
+    using Prod = Product<TM, TN, WM, WN, BK, PLANES, kNN>;
+    constexpr int kSlab = 64, kStride = TN + 4;  // the accumulators pass through LDS 64 rows at a time
+    constexpr int kLdsBytes = Prod::kLdsHalves * 2 > kSlab * kStride * 4 ? Prod::kLdsHalves * 2 : kSlab * kStride * 4;
+    __shared__ __attribute__((aligned(1024))) unsigned char lds[kLdsBytes];
+
+    constexpr int kind = kSym ? (TM == 128 ? kTilesSym128 : kTilesSym256) : (TM == 128 ? kTilesFull128 : kTilesFull256);
+    int matrix;
+    uint32_t tile;
+    const MatrixRow& row = find_tile(table, n_rows, kind, xcd_contiguous(blockIdx.x, gridDim.x), matrix, tile);
+    const int s64 = row.s64, l64 = row.l64;
+    int ti, tj;
+    if constexpr (kSym) {  // row by row under the diagonal
+        ti = (int)((__builtin_sqrtf(8.0f * (float)tile + 1.0f) - 1.0f) * 0.5f);
+        while ((uint32_t)((ti + 1) * (ti + 2) / 2) <= tile) ++ti;
+        while ((uint32_t)(ti * (ti + 1) / 2) > tile) --ti;
+        tj = (int)tile - ti * (ti + 1) / 2;
+    } else {
+        const int down = (s64 + TM - 1) / TM;
+        ti = (int)(tile % (uint32_t)down);
+        tj = (int)(tile / (uint32_t)down);
+    }
+    const int64_t plane_x = (int64_t)s64 * l64, plane_a = (int64_t)s64 * s64;
+    const _Float16* x = work + row.x_off[k.from] + (int64_t)matrix * 2 * plane_x;
+    _Float16* a = work + row.a_off + (int64_t)matrix * PLANES * plane_a;
+    _Float16* b = work + row.b_off + (int64_t)matrix * PLANES * plane_a;
+    const int i0 = ti * TM, j0 = tj * TN;
+
+    Prod prod;
+    if constexpr (STAGE == kStageGram)
+        prod.run(x + (int64_t)i0 * l64, l64, plane_x, s64 - i0, x + (int64_t)j0 * l64, l64, plane_x, s64 - j0, l64, reinterpret_cast<_Float16*>(lds));
+    else if constexpr (STAGE == kStagePoly)
+        prod.run(a + (int64_t)i0 * s64, s64, plane_a, s64 - i0, a + (int64_t)j0 * s64, s64, plane_a, s64 - j0, s64, reinterpret_cast<_Float16*>(lds));
+    else
+        prod.run(b + (int64_t)i0 * s64, s64, plane_a, s64 - i0, x + j0, l64, plane_x, l64 - j0, s64, reinterpret_cast<_Float16*>(lds));
+
+    float* slab = reinterpret_cast<float*>(lds);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / WN, wn = wave % WN;
+    constexpr int kWaveRows = TM / WM;
+#pragma unroll
+    for (int part = 0; part < TM / kSlab; ++part) {
+        if (wm == part * kSlab / kWaveRows) {
+            constexpr int kPer = kSlab / 16;
+            const int first = (part * kSlab % kWaveRows) / 16;
+#pragma unroll
+            for (int i = 0; i < kPer; ++i)
+#pragma unroll
+                for (int j = 0; j < Prod::NJ; ++j)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        slab[(i * 16 + (lane >> 4) * 4 + r) * kStride + wn * (TN / WN) + j * 16 + (lane & 15)] = prod.acc[first + i][j][r];
+        }
+        __syncthreads();
+        const int r0 = i0 + part * kSlab;  // the slab's first row in the result
+        if (r0 < s64) {  // sizes are multiples of 64: all rows of the slab are there, or none
+            if constexpr (STAGE <= kStageUpdate) {
+                const int width = kSym ? s64 : l64;
+                for (int e = threadIdx.x; e < kSlab * TN / 8; e += Prod::kThreads) {
+                    const int i = e / (TN / 8), j = (e % (TN / 8)) * 8;
+                    if (j0 + j >= width) continue;
+                    const int64_t at = (int64_t)(r0 + i) * width + j0 + j;
+                    float v[8];
+                    if constexpr (STAGE == kStageGram) {
+#pragma unroll
+                        for (int q = 0; q < 8; ++q) v[q] = k.product * slab[i * kStride + j + q];
+                        store_planes<PLANES>(a + at, plane_a, v);
+                    } else if constexpr (STAGE == kStagePoly) {
+                        load_planes<PLANES>(a + at, plane_a, v);
+#pragma unroll
+                        for (int q = 0; q < 8; ++q) v[q] = k.linear * v[q] + k.product * slab[i * kStride + j + q];
+                        store_planes<PLANES>(b + at, plane_a, v);
+                    } else {
+                        load_planes<2>(x + at, plane_x, v);
+#pragma unroll
+                        for (int q = 0; q < 8; ++q) v[q] = k.linear * v[q] + k.product * slab[i * kStride + j + q];
+                        store_planes<2>(work + row.x_off[k.to] + (int64_t)matrix * 2 * plane_x + at, plane_x, v);
+                    }
+                }
+                if constexpr (kSym) {
+                    if (ti != tj) {  // the mirror image: lanes along j, eight values along i
+                        for (int e = threadIdx.x; e < TN * kSlab / 8; e += Prod::kThreads) {
+                            const int j = e % TN, i = (e / TN) * 8;
+                            if (j0 + j >= s64) continue;
+                            const int64_t at = (int64_t)(j0 + j) * s64 + r0 + i;
+                            float v[8];
+                            if constexpr (STAGE == kStageGram) {
+#pragma unroll
+                                for (int q = 0; q < 8; ++q) v[q] = k.product * slab[(i + q) * kStride + j];
+                                store_planes<PLANES>(a + at, plane_a, v);
+                            } else {
+                                load_planes<PLANES>(a + at, plane_a, v);
+#pragma unroll
+                                for (int q = 0; q < 8; ++q) v[q] = k.linear * v[q] + k.product * slab[(i + q) * kStride + j];
+                                store_planes<PLANES>(b + at, plane_a, v);
+                            }
+                        }
+                    }
+                }
+            } else {
+                // the last product: into the results or the parameters, in their own orientation, lanes along their rows
+                const int64_t numel = (int64_t)row.rows * row.cols;
+                const float ratio = row.step_ratio;
+                for (int e = threadIdx.x; e < kSlab * TN; e += Prod::kThreads) {
+                    int i, j;
+                    if (row.tall) { i = e % kSlab; j = e / kSlab; }
+                    else { i = e / TN; j = e % TN; }
+                    if (r0 + i >= row.s || j0 + j >= row.l) continue;
+                    const int64_t at = (int64_t)(r0 + i) * l64 + j0 + j;
+                    const float o = k.linear * ((float)x[at] + (float)x[plane_x + at]) + k.product * slab[i * kStride + j];
+                    const int64_t r = row.tall ? j0 + j : r0 + i, c = row.tall ? r0 + i : j0 + j;
+                    if constexpr (STAGE == kStageOut) {
+                        store_from_float(row.dst, (int64_t)matrix * row.dst_stride + r * row.dst_ld + c, k.dst_type, o);
+                    } else {
+                        const int64_t to = (int64_t)matrix * numel + r * row.cols + c;
+                        const float p = load_as_float(row.dst, to, k.dst_type) * k.keep - ratio * o;
+                        store_from_float(row.dst, to, k.dst_type, p);
+                        if (k.copy_type >= 0) store_from_float(row.copy, to, k.copy_type, p);
+                    }
+                }
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// Rows of a call's table, in the arguments of the launch: nothing is allocated or copied, and a captured graph holds them.
+constexpr int kRowsPerPut = 20;
+struct MatrixRows {
+    MatrixRow row[kRowsPerPut];
+};
+__global__ void fsadam_put_matrix_rows(MatrixRow* table, int n, MatrixRows rows) {
+    constexpr int kWords = sizeof(MatrixRow) / 16;
+    typedef uint32_t word_t __attribute__((ext_vector_type(4)));
+    for (int e = threadIdx.x; e < n * kWords; e += blockDim.x) reinterpret_cast<word_t*>(table)[e] = reinterpret_cast<const word_t*>(rows.row)[e];
+}
+constexpr int kMomentumRowsPerPut = 64;
+struct MomentumRows {
+    MomentumRow row[kMomentumRowsPerPut];
+};
+__global__ void fsadam_put_momentum_rows(MomentumRow* table, int n, MomentumRows rows) {
+    constexpr int kWords = sizeof(MomentumRow) / 16;
+    typedef uint32_t word_t __attribute__((ext_vector_type(4)));
+    for (int e = threadIdx.x; e < n * kWords; e += blockDim.x) reinterpret_cast<word_t*>(table)[e] = reinterpret_cast<const word_t*>(rows.row)[e];
+}
+
+}  // namespace

@@ -1,0 +1,235 @@
+"""``Muon``: momentum whose update is orthogonalised before it is applied, on the gfx950 matrix kernels.
+
+For weights that are matrices.  Everything else in a model (embeddings and heads as one prefers, biases, norms) belongs to
+``fairscale_amd.optim.Adam``; both take the same gradients, loss scales and scalers.  The constructor follows
+``torch.optim.Muon``, the precision modes, ``step(scale=...)`` and ``fp32_param_groups`` follow ``Adam`` of this package.  The
+reference has no counterpart.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import Any, Callable, Dict, List, Optional, Sequence, Tuple, Union
+
+import torch
+
+from .. import _cabi
+from ..matrix_ops import NS_COEFFICIENTS, TYPE_CODE, orth_options, refuse_shared, scale_arguments, workspace_for
+from .adam import Precision
+
+__all__ = ["Muon"]
+
+
+class Muon(torch.optim.Optimizer):
+    """Momentum orthogonalised by Newton-Schulz products. GPU-only.
+
+    Per matrix, with ``r = grad / scale``: ``m <- m + (r - m) * (1 - momentum)``; ``u = r + (m - r) * momentum`` (``nesterov``) or
+    ``m``; ``O = orthogonalize(u)``; ``p <- p * (1 - lr * weight_decay) - lr * ratio * O``.  One call covers a group; the
+    update of the parameters happens inside the last product.
+
+    Arguments:
+        params: parameters of one dtype with at least two dimensions, or groups of them.  The last two dimensions
+            are the matrix, leading ones count matrices (experts); a convolution's weight is passed as a view
+            of two dimensions.
+        lr, weight_decay, momentum, nesterov, ns_coefficients, eps, ns_steps: as in the formulas above and in
+            ``fairscale_amd.optim.orthogonalize``.
+        adjust_lr_fn: ``ratio`` by the matrix's shape: None or ``"original"`` sqrt(max(1, rows / cols)),
+            ``"match_rms_adamw"`` 0.2 * sqrt(max(rows, cols)).
+        row_blocks: every matrix of the group is split into this many blocks of rows, each orthogonalised on its own (the
+            query, key and value parts of one projection; heads).  ``ratio`` goes by the block.
+        precision: FULL_PRECISION (fp32 parameters and gradients), MIXED_PRECISION (fp16 or bf16 parameters and gradients,
+            fp32 master copies in ``fp32_param_groups``) or MEMORY_EFFICIENT_MIXED_PRECISION (fp16 or bf16, no master copies).
+            The momentum is fp32 in all of them; PURE_FP16 is refused, since an average that takes in 5 % of a
+            gradient a step loses most of it in 11 bits.  Inferred from the first parameter when None, as ``Adam`` does.
+        products: ``"half"`` or ``"split"`` (see ``orthogonalize``).  None: ``"split"`` where the parameters are updated in
+            fp32, ``"half"`` where they are stored in 16 bits and round its error away.
+    """
+
+    def __init__(
+        self,
+        params: Any,
+        lr: float = 1e-3,
+        weight_decay: float = 0.1,
+        momentum: float = 0.95,
+        nesterov: bool = True,
+        ns_coefficients: Sequence[float] = NS_COEFFICIENTS,
+        eps: float = 1e-7,
+        ns_steps: int = 5,
+        adjust_lr_fn: Optional[str] = None,
+        row_blocks: int = 1,
+        *,
+        precision: Optional[Precision] = None,
+        products: Optional[str] = None,
+    ):
+        if products not in (None, "half", "split"):
+            raise ValueError(f"products must be None, 'half' or 'split', got {products!r}")
+        super().__init__(params, dict(lr=lr, weight_decay=weight_decay, momentum=momentum, nesterov=nesterov,
+                                      ns_coefficients=tuple(ns_coefficients), eps=eps, ns_steps=ns_steps,
+                                      adjust_lr_fn=adjust_lr_fn, row_blocks=row_blocks))
+        first_dtype = self.param_groups[0]["params"][0].dtype
+        if precision is None:
+            precision = Precision.FULL_PRECISION if first_dtype == torch.float32 else Precision.MIXED_PRECISION
+        if precision is Precision.PURE_FP16:
+            raise ValueError("Muon keeps its momentum in fp32: PURE_FP16 is not supported (MEMORY_EFFICIENT_MIXED_PRECISION is)")
+        allowed = (torch.float32,) if precision is Precision.FULL_PRECISION else (torch.float16, torch.bfloat16)
+        if first_dtype not in allowed:
+            raise ValueError(f"{precision.name} needs parameters of {' or '.join(str(d) for d in allowed)}, got {first_dtype}")
+        self.precision = precision
+        self.products = products or ("half" if precision is Precision.MEMORY_EFFICIENT_MIXED_PRECISION else "split")
+        self._dtype = first_dtype
+        for group in self.param_groups:
+            self._check_group(group)
+        self.fp32_param_groups: List[Dict[str, Any]] = []
+        if self.mixed_precision:
+            for group in self.param_groups:
+                self._add_masters(group)
+
+    @property
+    def mixed_precision(self) -> bool:
+        return self.precision is Precision.MIXED_PRECISION
+
+    @property
+    def supports_memory_efficient_fp16(self) -> bool:
+        return True
+
+    # ------------------------------------------------------------------ groups and state
+
+    def _check_group(self, group: Dict[str, Any]) -> None:
+        if not 0.0 <= group["lr"] < math.inf:
+            raise ValueError(f"Invalid learning rate: {group['lr']}")
+        if not 0.0 <= group["weight_decay"] < math.inf:
+            raise ValueError(f"Invalid weight_decay value: {group['weight_decay']}")
+        if not 0.0 <= group["momentum"] < 1.0:
+            raise ValueError(f"Invalid momentum value: {group['momentum']}")
+        if group["adjust_lr_fn"] not in (None, "original", "match_rms_adamw"):
+            raise ValueError(f"adjust_lr_fn must be None, 'original' or 'match_rms_adamw', got {group['adjust_lr_fn']!r}")
+        if not 0.0 < group["eps"] < math.inf:
+            raise ValueError(f"Invalid epsilon value: {group['eps']}")
+        options = orth_options(group["ns_steps"], group["ns_coefficients"], group["eps"], self.products)
+        size = ctypes.c_int64(0)
+        if _cabi.lib().fsadam_muon_workspace(None, 0, ctypes.byref(options), ctypes.byref(size)) != 0:
+            raise ValueError(_cabi.lib().fsadam_last_error().decode("utf-8", "replace"))
+        blocks = group["row_blocks"]
+        if int(blocks) != blocks or blocks < 1:
+            raise ValueError(f"row_blocks must be a positive whole number, got {blocks}")
+        for p in group["params"]:
+            if p.dtype != self._dtype:
+                raise ValueError(f"all parameters must share one dtype, got {self._dtype} and {p.dtype}")
+            if p.dim() < 2:
+                raise ValueError(f"Muon optimizes matrices, got a parameter of shape {tuple(p.shape)} (Adam takes it)")
+            if p.shape[-2] % blocks:
+                raise ValueError(f"{p.shape[-2]} rows cannot be split into {blocks} blocks")
+
+    def _add_masters(self, group: Dict[str, Any]) -> None:
+        masters = []
+        for p in group["params"]:
+            self.state[p]["master"] = p.detach().to(torch.float32, memory_format=torch.contiguous_format, copy=True)
+            masters.append(self.state[p]["master"])
+        self.fp32_param_groups.append({**{k: v for k, v in group.items() if k != "params"}, "params": masters})
+
+    def add_param_group(self, param_group: Dict[str, Any]) -> None:
+        super().add_param_group(param_group)
+        if "precision" in self.__dict__:  # not during construction, which checks all groups at its end
+            group = self.param_groups[-1]
+            try:
+                self._check_group(group)
+            except ValueError:
+                self.param_groups.pop()
+                raise
+            if self.mixed_precision:
+                self._add_masters(group)
+
+    def load_state_dict(self, state_dict: Dict[str, Any]) -> None:
+        """Restores momentum and master copies bit for bit (torch alone casts them to the parameters' dtype)."""
+        super().load_state_dict(state_dict)
+        saved = state_dict["state"]
+        self.fp32_param_groups = []
+        for group, saved_group in zip(self.param_groups, state_dict["param_groups"]):
+            self._check_group(group)
+            for p, pid in zip(group["params"], saved_group["params"]):
+                for key in ("momentum_buffer", "master"):
+                    if key in saved.get(pid, {}):
+                        self.state[p][key] = saved[pid][key].detach().to(device=p.device, dtype=torch.float32, copy=True).contiguous()
+            if self.mixed_precision:
+                masters = []
+                for p in group["params"]:
+                    if "master" not in self.state[p]:
+                        self.state[p]["master"] = p.detach().to(torch.float32, memory_format=torch.contiguous_format, copy=True)
+                    masters.append(self.state[p]["master"])
+                self.fp32_param_groups.append({**{k: v for k, v in group.items() if k != "params"}, "params": masters})
+
+    # ------------------------------------------------------------------ the step
+
+    def _gather(self, gi: int, group: Dict[str, Any]) -> Dict[torch.device, List[Tuple]]:
+        """(parameter or master, gradient, momentum, copy, ratio) of what takes part, by device.  Raises before anything is changed
+        but for momenta that are made."""
+        batches: Dict[torch.device, List[Tuple]] = {}
+        masters = self.fp32_param_groups[gi]["params"] if self.mixed_precision else None
+        for k, p in enumerate(group["params"]):
+            grad = p.grad
+            if grad is None:
+                continue
+            if grad.layout != torch.strided:
+                raise RuntimeError("Muon does not support sparse gradients")
+            if not p.is_cuda or not p.is_contiguous() or not grad.is_contiguous() or grad.device != p.device:
+                raise RuntimeError("parameters and gradients must be dense, contiguous tensors on one device each")
+            if grad.dtype != p.dtype or grad.shape != p.shape:
+                raise RuntimeError("gradients must have their parameter's dtype and shape")
+            if p.dtype != self._dtype:
+                raise RuntimeError(f"a parameter has changed its dtype from {self._dtype} to {p.dtype}")
+            state = self.state[p]
+            if state.get("momentum_buffer") is None:
+                if torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError("a graph that makes the momentum would clear it at every replay: step once before the capture")
+                state["momentum_buffer"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
+            buf = state["momentum_buffer"]
+            master = masters[k] if masters is not None else None
+            for t in (buf, master):
+                if t is not None and (t.dtype != torch.float32 or t.device != p.device or t.shape != p.shape or not t.is_contiguous()):
+                    raise RuntimeError("momentum and master copies must be contiguous float32 tensors with their parameter's shape and device")
+            batches.setdefault(p.device, []).append((p if master is None else master, grad, buf, p if master is not None else None))
+        return batches
+
+    def step(self, closure: Optional[Callable[[], float]] = None, *, scale: Union[float, torch.Tensor] = 1.0) -> Optional[float]:
+        """One optimization step.
+
+        Arguments:
+            closure: re-evaluates the model and returns the loss.
+            scale: gradients are divided by this inside the kernels, as in ``Adam.step``: a float, or a one-element float32
+                tensor on the parameters' device (``clip_grad_norm_(..., fold="device")``).
+
+        May be captured into a graph after one eager step; a replay then repeats the recorded lr, weight decay and (float) scale.
+        """
+        loss = closure() if closure is not None else None
+        calls = []
+        for gi, group in enumerate(self.param_groups):
+            self._check_group(group)
+            for device, batch in self._gather(gi, group).items():
+                refuse_shared([row[0] for row in batch], "parameters")
+                refuse_shared([row[2] for row in batch], "momenta")
+                calls.append((group, device, batch, *scale_arguments(scale, device)))
+        with torch.autograd.profiler.record_function("fairscale_amd::muon::fused_step"):
+            for call in calls:
+                self._launch(*call)
+        return loss
+
+    def _launch(self, group: Dict[str, Any], device: torch.device, batch: List[Tuple], scale: float, scale_pointer: Optional[int]) -> None:
+        blocks = int(group["row_blocks"])
+        rows = (_cabi.FsMuonTensor * len(batch))()
+        for row, (p, g, m, copy) in zip(rows, batch):
+            height, cols = p.shape[-2] // blocks, p.shape[-1]
+            row.p, row.g, row.m, row.p_copy = p.data_ptr(), g.data_ptr(), m.data_ptr(), None if copy is None else copy.data_ptr()
+            row.batch, row.rows, row.cols = (p.numel() // (height * cols) if p.numel() else 0), height, cols
+            if group["adjust_lr_fn"] == "match_rms_adamw":
+                row.ratio = 0.2 * math.sqrt(max(height, cols))
+            else:
+                row.ratio = math.sqrt(max(1.0, height / cols)) if cols else 1.0
+        options = orth_options(group["ns_steps"], group["ns_coefficients"], group["eps"], self.products)
+        code = TYPE_CODE[self._dtype]
+        lib = _cabi.lib()
+        with torch.cuda.device(device), torch.no_grad():
+            workspace, size = workspace_for(lib.fsadam_muon_workspace, device, rows, len(batch), ctypes.byref(options))
+            _cabi.check(lib.fsadam_muon_step(
+                rows, len(batch), _cabi.TYPE_F32 if self.mixed_precision else code, code, code if self.mixed_precision else -1, ctypes.byref(options),
+                float(group["lr"]), float(group["momentum"]), 1 if group["nesterov"] else 0, float(group["weight_decay"]), scale, scale_pointer,
+                workspace.data_ptr(), size, int(torch.cuda.current_stream(device).cuda_stream)))

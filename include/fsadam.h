@@ -280,6 +280,85 @@ int fsadam_grad_pass(const FsGradTensor* grads, int64_t n_tensors, int grad_dtyp
 int fsadam_grad_pass_noalloc(const FsGradTensor* grads, int64_t n_tensors, int grad_dtype, float inv_scale, const float* inv_scale_dev,
                              int write_back, float* found_inf_dev, double* sum_squares_dev, float* abs_max_dev, void* hip_stream);
 
+/* ---- matrix operators: the momentum pass, the orthogonalisation of matrices, and the optimizer step made of both.
+ * No counterpart in the reference, whose optimizers are elementwise.  Unlike the plans above these calls keep nothing:
+ * the caller gives them scratch memory (the *_workspace functions say how much, on the host, for the same list and
+ * arguments), their tables travel in kernel arguments, and they allocate nothing, create no stream or event and
+ * copy nothing with the copy engines.  They may be recorded into a HIP graph; scalars that travel by value (lr, scale ...)
+ * are then those of the recording.  1 - momentum, 1 - lr * weight_decay and lr * ratio are taken in fp64 and rounded
+ * to fp32 once.  The workspace may be reused as soon as the stream has passed the call; two calls
+ * that may overlap in time need one each (two captured graphs included). */
+
+#define FSADAM_TYPE_F32 0
+#define FSADAM_TYPE_F16 1
+#define FSADAM_TYPE_BF16 2
+
+/* Momentum pass, for every element of every tensor, in fp32 as written:
+ *     r = g / scale;   m <- m + (r - m) * (1 - momentum);   u = nesterov ? r + (m - r) * momentum : m
+ * m is updated in place; u is stored in update_type (u may be g itself where the types are the same: updates over the
+ * gradients).  norms_dev[t] (may be NULL) is the L2 norm of tensor t's update as stored, summed in fp64 in a fixed order;
+ * found_inf_dev[0] (may be NULL) is set to 1.0f, never cleared, where a stored update is not finite.
+ * scale_dev, when not NULL, is a device float[1] read in place of scale. */
+typedef struct FsMomentumTensor {
+    const void* g;
+    float* m;
+    void* u;
+    int64_t numel;
+} FsMomentumTensor;
+int fsadam_momentum_workspace(const FsMomentumTensor* tensors, int64_t n_tensors, int64_t* bytes);
+int fsadam_momentum_pass(const FsMomentumTensor* tensors, int64_t n_tensors, int grad_type, int update_type, double momentum, int nesterov,
+                         float scale, const float* scale_dev, float* norms_dev, float* found_inf_dev, void* workspace,
+                         int64_t workspace_bytes, void* hip_stream);
+
+/* Orthogonalisation by Newton-Schulz products.  For every matrix U (rows x cols), with X = U / max(|U|_F, eps), `steps` times
+ *     X <- a X + (b X X^T + c (X X^T)^2) X         (X^T X on the other side where rows > cols: the same values)
+ * which sends each singular value x to a x + b x^3 + c x^5 and leaves the singular vectors.  A matrix of zeros gives
+ * zeros (X is held to 2^-40: what is smaller than that beside max(|U|, eps) counts as 0), one with an entry that is not finite gives NaN in every entry; other matrices of the list are not touched by it.
+ * products: how many bits of the operands the matrix products take (fp32 sums either way): FSADAM_PRODUCTS_HALF 11 (error of
+ * the result about 2e-3 of its norm), FSADAM_PRODUCTS_SPLIT 22 (like fp32 products, about three times the work; always
+ * taken for matrices of a short side up to 128).
+ * Refused with FSADAM_EINVAL: coefficients that let singular values in [0, 1] grow past 1024 within the steps, steps
+ * outside 1..32, eps that is not positive, sides over 2^20. */
+#define FSADAM_PRODUCTS_HALF 1
+#define FSADAM_PRODUCTS_SPLIT 2
+typedef struct FsOrthOptions {
+    float a, b, c;
+    float eps;
+    int32_t steps;
+    int32_t products;
+} FsOrthOptions;
+
+/* `batch` matrices of one shape.  Elements of a row of a matrix are neighbours; ld: elements from one row to the next
+ * (>= cols), stride: from one matrix to the next.  dst may be src (same ld and stride), no other overlap is allowed. */
+typedef struct FsMatrix {
+    const void* src;
+    void* dst;
+    int64_t batch, rows, cols;
+    int64_t src_ld, src_stride;
+    int64_t dst_ld, dst_stride;
+} FsMatrix;
+int fsadam_orth_workspace(const FsMatrix* matrices, int64_t n, const FsOrthOptions* options, int64_t* bytes);
+int fsadam_orthogonalize(const FsMatrix* matrices, int64_t n, int type, const FsOrthOptions* options, void* workspace, int64_t workspace_bytes,
+                         void* hip_stream);
+
+/* The step: momentum pass on the gradients, orthogonalisation O of the update, and
+ *     p <- p * (1 - lr * weight_decay) - lr * ratio * O
+ * fused into the last product.  All tensors are contiguous, `batch` matrices of rows x cols each; momentum is fp32.
+ * param_type / grad_type / copy_type: (F32, F32, -1), (F32, F16, F16), (F32, BF16, BF16), (F16, F16, -1), (BF16, BF16, -1);
+ * copy_type names the type of p_copy, overwritten with the rounded parameters (-1: none). */
+typedef struct FsMuonTensor {
+    void* p;
+    const void* g;
+    float* m;
+    void* p_copy;
+    int64_t batch, rows, cols;
+    double ratio;
+} FsMuonTensor;
+int fsadam_muon_workspace(const FsMuonTensor* tensors, int64_t n, const FsOrthOptions* options, int64_t* bytes);
+int fsadam_muon_step(const FsMuonTensor* tensors, int64_t n, int param_type, int grad_type, int copy_type, const FsOrthOptions* options,
+                     double lr, double momentum, int nesterov, double weight_decay, float scale, const float* scale_dev, void* workspace,
+                     int64_t workspace_bytes, void* hip_stream);
+
 /* Drops the tables cached by fsadam_step and fsadam_grad_pass (synchronises the devices that own them). */
 int fsadam_clear_cache(void);
 

@@ -1,0 +1,280 @@
+"""What the matrix operators say without a GPU: their C entries refuse bad arguments before they touch a device, the workspace
+sizes are those of the documented storage, and the Python layer names what it will not take."""
+from __future__ import annotations
+
+import ctypes
+import math
+
+import pytest
+import torch
+
+from fairscale_amd import _cabi, matrix_ops
+from fairscale_amd.optim import Muon, Precision, momentum_pass, orthogonalize
+import _matrix_oracle as M
+
+L = _cabi.lib()
+FAKE = 1 << 20  # an address nothing is read from
+
+
+def options(steps=5, coefficients=M.COEFFICIENTS, eps=1e-7, products=_cabi.PRODUCTS_HALF):
+    return _cabi.FsOrthOptions(*coefficients, eps, steps, products)
+
+
+def matrices(*shapes, ld=None, src=FAKE, dst=FAKE * 2):
+    rows = (_cabi.FsMatrix * len(shapes))()
+    for row, (b, m, n) in zip(rows, shapes):
+        row.src, row.dst, row.batch, row.rows, row.cols = src, dst, b, m, n
+        row.src_ld = row.dst_ld = ld or n
+        row.src_stride = row.dst_stride = m * (ld or n)
+    return rows
+
+
+def workspace(rows, opt):
+    size = ctypes.c_int64(-1)
+    rc = L.fsadam_orth_workspace(rows, len(rows), ctypes.byref(opt), ctypes.byref(size))
+    return rc, size.value
+
+
+def up(v, m):
+    return (v + m - 1) // m * m
+
+
+@pytest.mark.parametrize("products", [1, 2])
+def test_workspace_holds_two_x_and_two_square_matrices_per_matrix(products):
+    rc, got = workspace(matrices((3, 300, 170), (1, 135, 200)), options(products=products))
+    assert rc == 0
+    x = lambda s, l: 2 * 2 * up(s, 64) * up(l, 64) * 2  # two buffers of two planes of halves
+    a = lambda s: 2 * products * up(s, 64) ** 2 * 2
+    body = 3 * (x(170, 300) + a(170)) + x(135, 200) + a(135)
+    assert body < got < body + 4096  # and the tables
+
+
+def test_workspace_of_a_long_list_stays_within_the_budget():
+    one = workspace(matrices((1, 4096, 4096)), options())[1]
+    rc, many = workspace(matrices(*[(1, 4096, 4096)] * 100), options())
+    assert rc == 0 and one < many <= 4 << 30
+    assert workspace(matrices((100, 4096, 4096)), options())[1] <= 4 << 30
+    rc, big = workspace(matrices((1, 32768, 32768)), options())  # a matrix over the budget gets what it needs
+    assert rc == 0 and big > 4 << 30
+
+
+def test_empty_lists_and_matrices_need_nothing():
+    assert workspace(matrices(), options()) == (0, 0)
+    assert workspace(matrices((0, 4, 4), (1, 0, 4), (1, 4, 0)), options()) == (0, 0)
+    opt = options()
+    assert L.fsadam_orthogonalize(matrices((1, 0, 4)), 1, 0, ctypes.byref(opt), None, 0, None) == 0
+    assert L.fsadam_orthogonalize(None, 0, 0, ctypes.byref(opt), None, 0, None) == 0
+    assert L.fsadam_muon_step(None, 0, 0, 0, -1, ctypes.byref(opt), 0.1, 0.9, 1, 0.0, 1.0, None, None, 0, None) == 0
+
+
+@pytest.mark.parametrize("bad", [
+    dict(steps=0), dict(steps=33), dict(eps=0.0), dict(eps=-1.0), dict(eps=math.inf), dict(eps=math.nan), dict(products=0), dict(products=3),
+    dict(coefficients=(math.nan, 0, 0)), dict(coefficients=(math.inf, 0, 0)),
+    dict(coefficients=(30.0, 0.0, 0.0)),       # 30^5
+    dict(coefficients=(1.0, 0.0, 5.0), steps=8),
+])
+def test_bad_options_are_refused(bad):
+    rc, _ = workspace(matrices((1, 4, 4)), options(**bad))
+    assert rc == -1 and L.fsadam_last_error()
+
+
+@pytest.mark.parametrize("good", [
+    dict(coefficients=(1.5, -0.5, 0.0)), dict(coefficients=(1.875, -1.25, 0.375)), dict(coefficients=(0.0, 0.0, 0.0)), dict(coefficients=(-3.4445, 4.7750, -2.0315)),
+    dict(coefficients=(1.0, 0.0, 0.0), steps=32), dict(eps=1e-30), dict(coefficients=(2.0, -1.5, 0.5), steps=32),
+])
+def test_other_iterations_are_taken(good):
+    assert workspace(matrices((1, 4, 4)), options(**good))[0] == 0
+
+
+@pytest.mark.parametrize("rows, message", [
+    (matrices((-1, 4, 4)), "negative"), (matrices((1, -4, 4)), "negative"), (matrices((1, 4, -4)), "negative"),
+    (matrices((1, (1 << 20) + 1, 4)), "2^20"), (matrices((1, 1 << 20, 1 << 20)), "2^34"),
+    (matrices((1, 4, 4), src=0), "NULL"), (matrices((1, 4, 4), dst=0), "NULL"), (matrices((1, 4, 4), ld=3), "overlap"),
+])
+def test_bad_matrices_are_refused(rows, message):
+    rc, _ = workspace(rows, options())
+    assert rc == -1 and message in L.fsadam_last_error().decode()
+
+
+def test_bad_strides_alignment_and_workspaces_are_refused():
+    opt = options()
+    rows = matrices((2, 4, 4))
+    rows[0].dst_stride = 15
+    assert L.fsadam_orthogonalize(rows, 1, 0, ctypes.byref(opt), FAKE, 1 << 20, None) == -1
+    rows = matrices((1, 4, 4), src=FAKE + 2)
+    assert L.fsadam_orthogonalize(rows, 1, 0, ctypes.byref(opt), FAKE, 1 << 20, None) == -1 and b"aligned" in L.fsadam_last_error()
+    rows = matrices((1, 4, 4), src=FAKE, dst=FAKE)
+    rows[0].dst_ld = 8
+    assert L.fsadam_orthogonalize(rows, 1, 0, ctypes.byref(opt), FAKE, 1 << 20, None) == -1 and b"same strides" in L.fsadam_last_error()
+    rows = matrices((1, 4, 4))
+    size = workspace(rows, opt)[1]
+    assert L.fsadam_orthogonalize(rows, 1, 0, ctypes.byref(opt), None, size, None) == -1 and b"workspace" in L.fsadam_last_error()
+    assert L.fsadam_orthogonalize(rows, 1, 0, ctypes.byref(opt), FAKE, size - 1, None) == -1 and b"workspace" in L.fsadam_last_error()
+    assert L.fsadam_orthogonalize(rows, 1, 0, ctypes.byref(opt), FAKE + 16, size, None) == -1
+    assert L.fsadam_orthogonalize(rows, 1, 3, ctypes.byref(opt), FAKE, size, None) == -1
+    assert L.fsadam_orthogonalize(rows, 1, 0, None, FAKE, size, None) == -1
+    assert L.fsadam_orth_workspace(rows, 1, ctypes.byref(opt), None) == -1
+    assert L.fsadam_orth_workspace(None, 1, ctypes.byref(opt), ctypes.byref(ctypes.c_int64())) == -1
+
+
+def muon_rows(**change):
+    rows = (_cabi.FsMuonTensor * 1)()
+    r = rows[0]
+    r.p, r.g, r.m, r.p_copy, r.batch, r.rows, r.cols, r.ratio = FAKE, FAKE * 2, FAKE * 3, FAKE * 4, 1, 4, 4, 1.0
+    for k, v in change.items():
+        setattr(r, k, v)
+    return rows
+
+
+@pytest.mark.parametrize("call", [
+    dict(types=(1, 0, -1)), dict(types=(0, 1, -1)), dict(types=(0, 1, 2)), dict(types=(0, 0, 0)), dict(types=(3, 3, -1)), dict(types=(1, 2, -1)),
+    dict(lr=math.nan), dict(lr=math.inf), dict(weight_decay=math.inf), dict(momentum=1.0), dict(momentum=-0.1), dict(momentum=math.nan),
+    dict(scale=0.0), dict(scale=math.inf), dict(scale=math.nan),
+    dict(rows=muon_rows(p=0)), dict(rows=muon_rows(g=0)), dict(rows=muon_rows(m=0)), dict(rows=muon_rows(p_copy=0), types=(0, 1, 1)),
+    dict(rows=muon_rows(m=FAKE + 2)), dict(rows=muon_rows(p=FAKE + 2)), dict(rows=muon_rows(ratio=math.nan)), dict(rows=muon_rows(rows=-1)),
+    dict(bytes=100),
+])
+def test_bad_steps_are_refused(call):
+    opt = options()
+    p, g, c = call.get("types", (0, 0, -1))
+    rc = L.fsadam_muon_step(call.get("rows", muon_rows()), 1, p, g, c, ctypes.byref(opt), call.get("lr", 0.1), call.get("momentum", 0.9), 1,
+                            call.get("weight_decay", 0.0), call.get("scale", 1.0), None, FAKE, call.get("bytes", 0), None)
+    assert rc == -1 and L.fsadam_last_error()
+
+
+def momentum_rows(**change):
+    rows = (_cabi.FsMomentumTensor * 1)()
+    r = rows[0]
+    r.g, r.m, r.u, r.numel = FAKE, FAKE * 2, FAKE * 3, 10
+    for k, v in change.items():
+        setattr(r, k, v)
+    return rows
+
+
+@pytest.mark.parametrize("call", [
+    dict(rows=momentum_rows(g=0)), dict(rows=momentum_rows(m=0)), dict(rows=momentum_rows(u=0)), dict(rows=momentum_rows(numel=-1)),
+    dict(rows=momentum_rows(numel=1 << 43)), dict(rows=momentum_rows(g=FAKE + 2)), dict(types=(0, 3)), dict(types=(-1, 0)), dict(momentum=1.5),
+    dict(scale=0.0), dict(bytes=100), dict(rows=momentum_rows(u=FAKE), types=(0, 1)),
+])
+def test_bad_momentum_passes_are_refused(call):
+    g, u = call.get("types", (0, 0))
+    rc = L.fsadam_momentum_pass(call.get("rows", momentum_rows()), 1, g, u, call.get("momentum", 0.9), 1, call.get("scale", 1.0), None, None, None, FAKE,
+                                call.get("bytes", 100), None)
+    assert rc == -1 and L.fsadam_last_error()
+
+
+def test_python_layer_refuses_what_is_not_on_a_gpu():
+    with pytest.raises(RuntimeError, match="device"):
+        orthogonalize([torch.zeros(4, 4)])
+    with pytest.raises(RuntimeError, match="device"):
+        momentum_pass([torch.zeros(4)], [torch.zeros(4)])
+    with pytest.raises(RuntimeError, match="float32, float16 or bfloat16"):
+        orthogonalize([torch.zeros(4, 4, dtype=torch.float64)])
+    with pytest.raises(RuntimeError, match="same length"):
+        momentum_pass([torch.zeros(4)], [])
+    with pytest.raises(RuntimeError, match="at least one"):
+        momentum_pass([], [])
+    with pytest.raises(RuntimeError, match="as long"):
+        orthogonalize([], out=[torch.zeros(1, 1)])
+    assert orthogonalize([]) == []
+
+
+def brute_layout(t):
+    """What _layout promises, checked element by element against storage offsets."""
+    got = matrix_ops._layout(t)
+    if got is None:
+        return None
+    turned, ld, stride = got
+    m = t.transpose(-2, -1) if turned else t
+    offsets = torch.arange(t.untyped_storage().size() // t.element_size()).as_strided(m.shape, m.stride(), t.storage_offset())
+    flat = offsets.reshape(-1, *m.shape[-2:])
+    b, r, c = torch.meshgrid(*[torch.arange(n) for n in flat.shape], indexing="ij")
+    assert torch.equal(flat, t.storage_offset() + b * stride + r * ld + c), (t.shape, t.stride(), got)
+    assert ld >= m.shape[-1]
+    return got
+
+
+def test_layouts_describe_the_memory_they_are_read_from():
+    base = torch.zeros(4, 6, 10)
+    for t in (base, base.transpose(1, 2), base[:, :3], base[:, :, 2:7], base[:, 1:2], base[:, :, 4:5], base[1], base[1].t(), base[1:2], base[::2],
+              base.view(2, 2, 6, 10), base.transpose(1, 2)[:, 3:4], base[:, 2:3, 3:4], base.view(2, 2, 6, 10)[:, :1], torch.zeros(1, 1), torch.zeros(1, 7), torch.zeros(7, 1),
+              torch.zeros(7, 1).t(), torch.zeros(3, 1).expand(3, 1), torch.zeros(1, 4, 4).expand(5, 4, 4)):
+        assert brute_layout(t) is not None, (t.shape, t.stride())
+    for t in (base[:, :, ::2], base[:, ::2, ::2], torch.zeros(1, 4).expand(4, 4), base.view(2, 2, 6, 10).transpose(0, 1), base.view(2, 2, 6, 10)[:, :, :, ::3]):
+        assert brute_layout(t) is None, (t.shape, t.stride())
+
+
+def test_a_single_row_or_column_can_be_read_either_way():
+    for t in (torch.zeros(5, 1), torch.zeros(1, 5), torch.zeros(5, 1).t(), torch.zeros(9, 9)[:, 2:3], torch.zeros(9, 9)[3:4]):
+        turned = matrix_ops._layout(t)[0]
+        other = matrix_ops._layout_as(t, not turned)
+        if other is not None:
+            m = t.transpose(-2, -1) if not turned else t
+            assert other[0] is (not turned)
+            assert m.shape[-1] == 1 or m.stride(-1) == 1
+    assert matrix_ops._layout_as(torch.zeros(4, 5), True) is None
+
+
+def test_optimizer_checks_its_arguments():
+    w = lambda *s, dtype=torch.float32: [torch.nn.Parameter(torch.zeros(*s, dtype=dtype))]
+    for bad in (dict(lr=-1.0), dict(lr=math.inf), dict(weight_decay=-1.0), dict(momentum=1.0), dict(momentum=-0.5), dict(eps=0.0), dict(ns_steps=0), dict(ns_steps=2.5),
+                dict(ns_coefficients=(1.0, 2.0)), dict(ns_coefficients=(50.0, 0.0, 0.0)), dict(adjust_lr_fn="other"), dict(row_blocks=0), dict(row_blocks=3),
+                dict(products="bf16"), dict(precision=Precision.PURE_FP16), dict(precision=Precision.MIXED_PRECISION)):
+        with pytest.raises(ValueError):
+            Muon(w(4, 4), **bad)
+    with pytest.raises(ValueError, match="matrices"):
+        Muon(w(4))
+    with pytest.raises(ValueError, match="dtype"):
+        Muon(w(4, 4) + w(4, 4, dtype=torch.float16))
+    with pytest.raises(ValueError, match="FULL_PRECISION"):
+        Muon(w(4, 4, dtype=torch.bfloat16), precision=Precision.FULL_PRECISION)
+    opt = Muon(w(4, 4))
+    assert opt.precision is Precision.FULL_PRECISION and opt.products == "split"
+    opt = Muon(w(4, 4, dtype=torch.bfloat16))
+    assert opt.precision is Precision.MIXED_PRECISION and opt.products == "split"
+    assert opt.fp32_param_groups[0]["params"][0].dtype == torch.float32
+    opt = Muon(w(4, 4, dtype=torch.bfloat16), precision=Precision.MEMORY_EFFICIENT_MIXED_PRECISION)
+    assert opt.products == "half" and opt.fp32_param_groups == []
+    with pytest.raises(ValueError):
+        opt.add_param_group({"params": w(5, dtype=torch.bfloat16)})
+    assert len(opt.param_groups) == 1
+
+
+def test_optimizer_refuses_parameters_on_the_cpu_and_sparse_gradients():
+    p = torch.nn.Parameter(torch.zeros(4, 4))
+    opt = Muon([p])
+    assert opt.step() is None  # no gradient: nothing to do
+    p.grad = torch.zeros(4, 4)
+    with pytest.raises(RuntimeError, match="device tensors|one device"):
+        opt.step()
+    p.grad = torch.zeros(4, 4).to_sparse()
+    with pytest.raises(RuntimeError, match="sparse"):
+        opt.step()
+    assert torch.equal(p.detach(), torch.zeros(4, 4))
+
+
+def test_state_of_16_bit_parameters_is_restored_bit_for_bit():
+    p = torch.nn.Parameter(torch.randn(4, 4).to(torch.bfloat16))
+    opt = Muon([p], lr=0.5)
+    opt.state[p]["momentum_buffer"] = torch.randn(4, 4)
+    opt.state[p]["master"] += 1e-5
+    saved = opt.state_dict()
+    other = Muon([torch.nn.Parameter(p.detach().clone())])
+    other.load_state_dict(saved)
+    q = other.param_groups[0]["params"][0]
+    for key in ("momentum_buffer", "master"):
+        assert torch.equal(other.state[q][key], opt.state[p][key]) and other.state[q][key].dtype == torch.float32
+        assert other.state[q][key].data_ptr() != opt.state[p][key].data_ptr()
+    assert other.fp32_param_groups[0]["params"][0] is other.state[q]["master"] and other.param_groups[0]["lr"] == 0.5
+
+
+def test_oracle_agrees_with_singular_values():
+    """The oracle's products against the polynomial on the singular values."""
+    torch.manual_seed(0)
+    u = torch.randn(2, 9, 5, dtype=torch.float64)
+    a, b, c = M.COEFFICIENTS
+    x, s, y = torch.linalg.svd(u, full_matrices=False)
+    s = s / s.norm(dim=-1, keepdim=True)
+    for _ in range(5):
+        s = a * s + b * s**3 + c * s**5
+    assert M.relative(M.orthogonal(u), x @ torch.diag_embed(s) @ y) < 1e-12
