@@ -237,7 +237,7 @@ int launch_stage(int stage, const Chunk& c, const MatrixRow* table, const StageA
     const bool sym = stage == kStageGram || stage == kStagePoly;
     const dim3 grid((uint32_t)c.tiles[sym ? kTilesSym128 : kTilesFull128]), block(256);
 #define FM_STAGE(S) \
-    case S: hipLaunchKernelGGL((fsadam_matrix_stage<S, 128, 128, 2, 2, BK, PLANES>), grid, block, 0, stream, table, n, k, work); break
+    case S: hipLaunchKernelGGL((fsadam_matrix_stage<S, 128, 128, 2, 2, BK, 2, PLANES>), grid, block, 0, stream, table, n, k, work); break
     switch (stage) {
         FM_STAGE(kStageGram);
         FM_STAGE(kStagePoly);

@@ -81,6 +81,52 @@ __device__ __forceinline__ float round_to(float v, int type) {
     return __builtin_bit_cast(float, (uint32_t)bf16_bits(v) << 16);
 }
 
+// Eight neighbours p[i .. i + 7], of which the first `left` are there: 16-byte accesses where all are and the address allows it.
+typedef uint32_t words4_t __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ void load_eight(const void* p, int64_t i, int type, int left, float (&v)[8]) {
+    const char* at = static_cast<const char*>(p) + i * (type == kTypeF32 ? 4 : 2);
+    if (left >= 8 && ((uintptr_t)at & 15) == 0) {
+        if (type == kTypeF32) {
+#pragma unroll
+            for (int q = 0; q < 8; ++q) v[q] = reinterpret_cast<const float4_t*>(at)[q >> 2][q & 3];
+        } else if (type == kTypeF16) {
+            const half8_t h = *reinterpret_cast<const half8_t*>(at);
+#pragma unroll
+            for (int q = 0; q < 8; ++q) v[q] = (float)h[q];
+        } else {
+            const words4_t w = *reinterpret_cast<const words4_t*>(at);
+#pragma unroll
+            for (int q = 0; q < 8; ++q) v[q] = __builtin_bit_cast(float, q & 1 ? w[q >> 1] & 0xffff0000u : w[q >> 1] << 16);
+        }
+    } else {
+#pragma unroll
+        for (int q = 0; q < 8; ++q) v[q] = q < left ? load_as_float(p, i + q, type) : 0.0f;
+    }
+}
+__device__ __forceinline__ void store_eight(void* p, int64_t i, int type, int left, const float (&v)[8]) {
+    char* at = static_cast<char*>(p) + i * (type == kTypeF32 ? 4 : 2);
+    if (left >= 8 && ((uintptr_t)at & 15) == 0) {
+        if (type == kTypeF32) {
+            reinterpret_cast<float4_t*>(at)[0] = float4_t{v[0], v[1], v[2], v[3]};
+            reinterpret_cast<float4_t*>(at)[1] = float4_t{v[4], v[5], v[6], v[7]};
+        } else if (type == kTypeF16) {
+            half8_t h;
+#pragma unroll
+            for (int q = 0; q < 8; ++q) h[q] = (_Float16)v[q];
+            *reinterpret_cast<half8_t*>(at) = h;
+        } else {
+            words4_t w;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) w[q] = (uint32_t)bf16_bits(v[2 * q]) | (uint32_t)bf16_bits(v[2 * q + 1]) << 16;
+            *reinterpret_cast<words4_t*>(at) = w;
+        }
+    } else {
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+            if (q < left) store_from_float(p, i + q, type, v[q]);
+    }
+}
+
 __device__ __forceinline__ void split_halves(float v, _Float16& hi, _Float16& lo) {
     hi = (_Float16)v;
     lo = (_Float16)(v - (float)hi);
@@ -317,17 +363,22 @@ __device__ __forceinline__ int swizzle_nn(int row) { return (row & 3) | (((row >
 __device__ __forceinline__ void load_to_lds(const _Float16* src, uint32_t dst) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(dst), "v"((const FM_GLOBAL void*)src) : "memory");
 }
-__device__ __forceinline__ void loads_arrived() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+template <int LEFT>
+__device__ __forceinline__ void loads_arrived() {  // all but the last LEFT loads of this wave
+    static_assert(LEFT < 64, "the counter has six bits");
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LEFT) : "memory");
+}
 __device__ __forceinline__ uint32_t lds_address(const void* p) { return (uint32_t)(uintptr_t)(FM_LDS const void*)p; }
 
-// C tile (TM x TN) = P Q^T (NT) or P Q (NN) over K, by WM x WN waves; the caller's epilogue takes acc.
-template <int TM, int TN, int WM, int WN, int BK, int PLANES, bool NN>
+// C tile (TM x TN) = P Q^T (NT) or P Q (NN) over K, by WM x WN waves; the caller's epilogue takes acc.  DEPTH panels are in LDS:
+// one is multiplied while the others are on their way.
+template <int TM, int TN, int WM, int WN, int BK, int DEPTH, int PLANES, bool NN>
 struct Product {
     static constexpr int kThreads = 64 * WM * WN, kWaves = WM * WN;
     static constexpr int MI = TM / WM / 16, NJ = TN / WN / 16;
     static constexpr int kPanelP = TM * BK, kPanelQ = TN * BK;             // halves of one plane
     static constexpr int kStageHalves = PLANES * (kPanelP + kPanelQ);
-    static constexpr int kLdsHalves = 2 * kStageHalves;
+    static constexpr int kLdsHalves = DEPTH * kStageHalves;
     static constexpr int kLoadsP = kPanelP / 512 / kWaves, kLoadsQ = kPanelQ / 512 / kWaves;  // 1 KiB loads of a wave, one plane
     static_assert(kLoadsP * 512 * kWaves == kPanelP && kLoadsQ * 512 * kWaves == kPanelQ, "panels divide among the waves");
 
@@ -396,13 +447,22 @@ struct Product {
             for (int j = 0; j < NJ; ++j) nn_at[j] = r * TN + (((wn * (TN / WN) / 16 + j) ^ swizzle_nn(r)) * 16) + (c & 3) * 4;
         }
 
-        fetch(lds_at);
-        loads_arrived();
-        __syncthreads();
+        constexpr int kLoads = PLANES * (kLoadsP + kLoadsQ);  // of a wave for one panel pair
         const int n_k = k_total / BK;
+        int fetched = 0, into = 0;
+        for (; fetched < DEPTH - 1 && fetched < n_k; ++fetched) fetch(lds_at + fetched * kStageHalves * 2);
+        into = fetched % DEPTH;
+        const _Float16* now = lds;
         for (int step = 0; step < n_k; ++step) {
-            _Float16* now = lds + (step & 1) * kStageHalves;
-            if (step + 1 < n_k) fetch(lds_at + ((step + 1) & 1) * kStageHalves * 2);
+            // panel `step` is there for this wave, behind the barrier for all, and behind it all are done with panel step - 1
+            if (fetched - step == DEPTH - 1) loads_arrived<kLoads*(DEPTH - 2)>();
+            else loads_arrived<0>();
+            __syncthreads();
+            if (fetched < n_k) {
+                fetch(lds_at + into * kStageHalves * 2);
+                ++fetched;
+                into = into + 1 == DEPTH ? 0 : into + 1;
+            }
 #pragma unroll
             for (int kk = 0; kk < BK / 32; ++kk) {
                 half8_t fp[PLANES][MI], fq[PLANES][NJ];
@@ -435,9 +495,9 @@ struct Product {
                         acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fp[0][i], fq[0][j], acc[i][j], 0, 0, 0);
                     }
             }
-            loads_arrived();
-            __syncthreads();
+            now = step % DEPTH == DEPTH - 1 ? lds : now + kStageHalves;
         }
+        __syncthreads();  // the epilogue writes over the panels
     }
 };
 
@@ -468,11 +528,11 @@ __device__ __forceinline__ void load_planes(const _Float16* at, int64_t plane, f
 }
 
 // One stage of the iteration over every matrix of the chunk.
-template <int STAGE, int TM, int TN, int WM, int WN, int BK, int PLANES>
+template <int STAGE, int TM, int TN, int WM, int WN, int BK, int DEPTH, int PLANES>
 __global__ __launch_bounds__(64 * WM * WN) void fsadam_matrix_stage(const MatrixRow* table, int n_rows, StageArgs k, _Float16* work) {
     constexpr bool kSym = STAGE == kStageGram || STAGE == kStagePoly;
     constexpr bool kNN = !kSym;
-    using Prod = Product<TM, TN, WM, WN, BK, PLANES, kNN>;
+    using Prod = Product<TM, TN, WM, WN, BK, DEPTH, PLANES, kNN>;
     constexpr int kSlab = 64, kStride = TN + 4;  // the accumulators pass through LDS 64 rows at a time
     constexpr int kLdsBytes = Prod::kLdsHalves * 2 > kSlab * kStride * 4 ? Prod::kLdsHalves * 2 : kSlab * kStride * 4;
     __shared__ __attribute__((aligned(1024))) unsigned char lds[kLdsBytes];
@@ -508,8 +568,20 @@ __global__ __launch_bounds__(64 * WM * WN) void fsadam_matrix_stage(const Matrix
         prod.run(b + (int64_t)i0 * s64, s64, plane_a, s64 - i0, x + j0, l64, plane_x, l64 - j0, s64, reinterpret_cast<_Float16*>(lds));
 
     float* slab = reinterpret_cast<float*>(lds);
+    // element (i, j) of the slab; columns are exchanged in blocks of 8 by the rows' block of 8, so that reading eight
+    // rows of a column at a time (mirror images, tall matrices) spreads over the banks as well
+    auto at_slab = [&](int i, int j) { return slab + i * kStride + (j ^ (((i >> 3) & 7) << 3)); };
+    auto along_row = [&](int i, int j, float (&v)[8]) {  // (i, j .. j + 7)
+        const float4_t* from = reinterpret_cast<const float4_t*>(at_slab(i, j));
+#pragma unroll
+        for (int q = 0; q < 8; ++q) v[q] = from[q >> 2][q & 3];
+    };
+    auto along_column = [&](int i, int j, float (&v)[8]) {  // (i .. i + 7, j)
+#pragma unroll
+        for (int q = 0; q < 8; ++q) v[q] = at_slab(i, j)[q * kStride];
+    };
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / WN, wn = wave % WN;
-    constexpr int kWaveRows = TM / WM;
+    constexpr int kWaveRows = TM / WM, kPieces = kSlab * TN / 8;  // pieces of eight elements
 #pragma unroll
     for (int part = 0; part < TM / kSlab; ++part) {
         if (wm == part * kSlab / kWaveRows) {
@@ -521,73 +593,92 @@ __global__ __launch_bounds__(64 * WM * WN) void fsadam_matrix_stage(const Matrix
                 for (int j = 0; j < Prod::NJ; ++j)
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
-                        slab[(i * 16 + (lane >> 4) * 4 + r) * kStride + wn * (TN / WN) + j * 16 + (lane & 15)] = prod.acc[first + i][j][r];
+                        *at_slab(i * 16 + (lane >> 4) * 4 + r, wn * (TN / WN) + j * 16 + (lane & 15)) = prod.acc[first + i][j][r];
         }
         __syncthreads();
         const int r0 = i0 + part * kSlab;  // the slab's first row in the result
         if (r0 < s64) {  // sizes are multiples of 64: all rows of the slab are there, or none
             if constexpr (STAGE <= kStageUpdate) {
                 const int width = kSym ? s64 : l64;
-                for (int e = threadIdx.x; e < kSlab * TN / 8; e += Prod::kThreads) {
+                for (int e = threadIdx.x; e < kPieces; e += Prod::kThreads) {
                     const int i = e / (TN / 8), j = (e % (TN / 8)) * 8;
                     if (j0 + j >= width) continue;
                     const int64_t at = (int64_t)(r0 + i) * width + j0 + j;
-                    float v[8];
+                    float v[8], w[8];
+                    along_row(i, j, v);
                     if constexpr (STAGE == kStageGram) {
 #pragma unroll
-                        for (int q = 0; q < 8; ++q) v[q] = k.product * slab[i * kStride + j + q];
+                        for (int q = 0; q < 8; ++q) v[q] *= k.product;
                         store_planes<PLANES>(a + at, plane_a, v);
                     } else if constexpr (STAGE == kStagePoly) {
-                        load_planes<PLANES>(a + at, plane_a, v);
+                        load_planes<PLANES>(a + at, plane_a, w);
 #pragma unroll
-                        for (int q = 0; q < 8; ++q) v[q] = k.linear * v[q] + k.product * slab[i * kStride + j + q];
+                        for (int q = 0; q < 8; ++q) v[q] = k.linear * w[q] + k.product * v[q];
                         store_planes<PLANES>(b + at, plane_a, v);
                     } else {
-                        load_planes<2>(x + at, plane_x, v);
+                        load_planes<2>(x + at, plane_x, w);
 #pragma unroll
-                        for (int q = 0; q < 8; ++q) v[q] = k.linear * v[q] + k.product * slab[i * kStride + j + q];
+                        for (int q = 0; q < 8; ++q) v[q] = k.linear * w[q] + k.product * v[q];
                         store_planes<2>(work + row.x_off[k.to] + (int64_t)matrix * 2 * plane_x + at, plane_x, v);
                     }
                 }
                 if constexpr (kSym) {
-                    if (ti != tj) {  // the mirror image: lanes along j, eight values along i
-                        for (int e = threadIdx.x; e < TN * kSlab / 8; e += Prod::kThreads) {
-                            const int j = e % TN, i = (e / TN) * 8;
+                    if (ti != tj) {  // the mirror image
+                        for (int e = threadIdx.x; e < kPieces; e += Prod::kThreads) {
+                            const int j = e / (kSlab / 8), i = (e % (kSlab / 8)) * 8;
                             if (j0 + j >= s64) continue;
                             const int64_t at = (int64_t)(j0 + j) * s64 + r0 + i;
-                            float v[8];
+                            float v[8], w[8];
+                            along_column(i, j, v);
                             if constexpr (STAGE == kStageGram) {
 #pragma unroll
-                                for (int q = 0; q < 8; ++q) v[q] = k.product * slab[(i + q) * kStride + j];
+                                for (int q = 0; q < 8; ++q) v[q] *= k.product;
                                 store_planes<PLANES>(a + at, plane_a, v);
                             } else {
-                                load_planes<PLANES>(a + at, plane_a, v);
+                                load_planes<PLANES>(a + at, plane_a, w);
 #pragma unroll
-                                for (int q = 0; q < 8; ++q) v[q] = k.linear * v[q] + k.product * slab[(i + q) * kStride + j];
+                                for (int q = 0; q < 8; ++q) v[q] = k.linear * w[q] + k.product * v[q];
                                 store_planes<PLANES>(b + at, plane_a, v);
                             }
                         }
                     }
                 }
             } else {
-                // the last product: into the results or the parameters, in their own orientation, lanes along their rows
+                // the last product: into the results or the parameters, in their own orientation, eight elements along
+                // their rows at a time
                 const int64_t numel = (int64_t)row.rows * row.cols;
                 const float ratio = row.step_ratio;
-                for (int e = threadIdx.x; e < kSlab * TN; e += Prod::kThreads) {
+                for (int e = threadIdx.x; e < kPieces; e += Prod::kThreads) {
                     int i, j;
-                    if (row.tall) { i = e % kSlab; j = e / kSlab; }
-                    else { i = e / TN; j = e % TN; }
-                    if (r0 + i >= row.s || j0 + j >= row.l) continue;
-                    const int64_t at = (int64_t)(r0 + i) * l64 + j0 + j;
-                    const float o = k.linear * ((float)x[at] + (float)x[plane_x + at]) + k.product * slab[i * kStride + j];
+                    float o[8], w[8];
+                    if (row.tall) {
+                        j = e / (kSlab / 8);
+                        i = (e % (kSlab / 8)) * 8;
+                        if (r0 + i >= row.s || j0 + j >= row.l) continue;
+                        along_column(i, j, o);
+                        const _Float16* from = x + (int64_t)(r0 + i) * l64 + j0 + j;
+#pragma unroll
+                        for (int q = 0; q < 8; ++q) w[q] = (float)from[(int64_t)q * l64] + (float)from[plane_x + (int64_t)q * l64];
+                    } else {
+                        i = e / (TN / 8);
+                        j = (e % (TN / 8)) * 8;
+                        if (r0 + i >= row.s || j0 + j >= row.l) continue;
+                        along_row(i, j, o);
+                        load_planes<2>(x + (int64_t)(r0 + i) * l64 + j0 + j, plane_x, w);
+                    }
+#pragma unroll
+                    for (int q = 0; q < 8; ++q) o[q] = k.linear * w[q] + k.product * o[q];
                     const int64_t r = row.tall ? j0 + j : r0 + i, c = row.tall ? r0 + i : j0 + j;
+                    const int left = row.cols - (int)c;  // elements of the row from here on
                     if constexpr (STAGE == kStageOut) {
-                        store_from_float(row.dst, (int64_t)matrix * row.dst_stride + r * row.dst_ld + c, k.dst_type, o);
+                        store_eight(row.dst, (int64_t)matrix * row.dst_stride + r * row.dst_ld + c, k.dst_type, left, o);
                     } else {
                         const int64_t to = (int64_t)matrix * numel + r * row.cols + c;
-                        const float p = load_as_float(row.dst, to, k.dst_type) * k.keep - ratio * o;
-                        store_from_float(row.dst, to, k.dst_type, p);
-                        if (k.copy_type >= 0) store_from_float(row.copy, to, k.copy_type, p);
+                        load_eight(row.dst, to, k.dst_type, left, w);
+#pragma unroll
+                        for (int q = 0; q < 8; ++q) o[q] = w[q] * k.keep - ratio * o[q];
+                        store_eight(row.dst, to, k.dst_type, left, o);
+                        if (k.copy_type >= 0) store_eight(row.copy, to, k.copy_type, left, o);
                     }
                 }
             }
