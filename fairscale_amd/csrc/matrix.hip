@@ -59,49 +59,61 @@ constexpr int64_t kChunkBytes = int64_t(4) << 30;
 
 // ---- numbers of the iteration -------------------------------------------------------------------------------------
 
-// Exponents of the powers of two that X, A and B are held with at every step.
-struct StepNumbers {
-    int x[kMaxSteps + 1], a[kMaxSteps], b[kMaxSteps];
-};
+// Largest magnitude of c[0] + c[1] t + ... + c[n] t^n on [0, top]: at the ends, or where the derivative vanishes (found by
+// bisection between samples where it changes sign; the polynomials are of low degree and far from the bounds).
+double largest(const double* c, int n, double top) {
+    auto value = [&](double t) { double v = 0.0; for (int i = n; i >= 0; --i) v = v * t + c[i]; return v; };
+    auto slope = [&](double t) { double v = 0.0; for (int i = n; i >= 1; --i) v = v * t + i * c[i]; return v; };
+    constexpr int kSamples = 256;
+    double most = std::max(std::fabs(value(0.0)), std::fabs(value(top)));
+    for (int i = 0; i < kSamples; ++i) {
+        double low = top * i / kSamples, high = top * (i + 1) / kSamples;
+        most = std::max(most, std::fabs(value(low)));
+        if ((slope(low) < 0.0) == (slope(high) < 0.0)) continue;
+        const bool down = slope(low) < 0.0;
+        for (int k = 0; k < 50; ++k) {
+            const double mid = 0.5 * (low + high);
+            if ((slope(mid) < 0.0) == down) low = mid;
+            else high = mid;
+        }
+        most = std::max(most, std::fabs(value(low)));
+    }
+    return most;
+}
 
+// The powers of two that a step's matrices are held with.  With t the square of a singular value (a: step's polynomial
+// q(t) = a + b t + c t^2, so that X <- q(A) X):  A: t,  B: b t + c t^2,  R: q(t),  T: t q(t).
+struct StepNumbers {
+    int x, a, b, r, t;
+    double q_bound;  // of |q|
+};
 int exponent_for(double bound) {  // the largest k with bound * 2^k <= 60000 (halves end at 65504), at most 15
     if (!(bound > 0x1p-15)) return 15;
     return std::min(15, (int)std::floor(std::log2(60000.0 / bound)));
 }
 
-// How large singular values of X, A and B can be at every step, when those of X0 are in [0, 1].  The polynomial's extremes on
-// [0, m] are at the ends and where its derivative (quadratic in x^2) vanishes.  2 % a step stands for what rounding adds.
-int step_bounds(const FsOrthOptions& o, StepNumbers& n) {
-    const double a = o.a, b = o.b, c = o.c;
+// How large the eigenvalues of those matrices can be at every step, when the singular values of X0 are in [0, 1].  2 % a step stands
+// for what rounding adds.
+int step_bounds(const FsOrthOptions& o, std::vector<StepNumbers>& numbers) {
+    const double q[] = {o.a, o.b, o.c}, b[] = {0.0, o.b, o.c}, t[] = {0.0, o.a, o.b, o.c};
+    const double p2[] = {0.0, q[0] * q[0], 2 * q[0] * q[1], q[1] * q[1] + 2 * q[0] * q[2], 2 * q[1] * q[2], q[2] * q[2]};  // t q(t)^2: the next t
+    numbers.clear();
     double m = 1.0;
     for (int k = 0; k < o.steps; ++k) {
         m *= 1.02;
-        n.x[k] = exponent_for(m);
-        n.a[k] = exponent_for(m * m);
-        const double top = m * m;
-        double most_b = std::fabs(b * top + c * top * top);
-        if (c != 0.0) {
-            const double at = -b / (2.0 * c);
-            if (at > 0.0 && at < top) most_b = std::max(most_b, std::fabs(b * at + c * at * at));
-        }
-        n.b[k] = exponent_for(most_b);
-        auto p = [&](double t) { return std::fabs(std::sqrt(t) * (a + b * t + c * t * t)); };  // t = x^2
-        double next = p(top);
-        const double d = 9.0 * b * b - 20.0 * a * c;
-        if (c != 0.0 && d >= 0.0) {
-            for (double sign : {-1.0, 1.0}) {
-                const double t = (-3.0 * b + sign * std::sqrt(d)) / (10.0 * c);
-                if (t > 0.0 && t < top) next = std::max(next, p(t));
-            }
-        } else if (c == 0.0 && b != 0.0) {
-            const double t = -a / (3.0 * b);
-            if (t > 0.0 && t < top) next = std::max(next, p(t));
-        }
-        m = next;
-        if (!(m <= 1024.0) || !(most_b <= 1024.0))
+        StepNumbers n;
+        const double top = m * m, most_q = largest(q, 2, top), most_b = largest(b, 2, top), most_t = largest(t, 3, top);
+        m = std::sqrt(largest(p2, 5, top));
+        if (!(m <= 1024.0))
             return fail(FSADAM_EINVAL, "the coefficients let singular values in [0, 1] grow past 1024 by step " + std::to_string(k + 1));
+        n.x = exponent_for(std::sqrt(top));
+        n.a = exponent_for(top);
+        n.b = exponent_for(most_b);
+        n.r = exponent_for(most_q);
+        n.t = exponent_for(most_t);
+        n.q_bound = most_q;
+        numbers.push_back(n);
     }
-    n.x[o.steps] = 0;
     return FSADAM_OK;
 }
 
@@ -111,7 +123,7 @@ int check_options(const FsOrthOptions* o) {
     if (!std::isfinite(o->a) || !std::isfinite(o->b) || !std::isfinite(o->c)) return fail(FSADAM_EINVAL, "the coefficients must be finite");
     if (!(o->eps > 0.0f) || !std::isfinite(o->eps)) return fail(FSADAM_EINVAL, "eps must be positive and finite");
     if (o->products != FSADAM_PRODUCTS_HALF && o->products != FSADAM_PRODUCTS_SPLIT) return fail(FSADAM_EINVAL, "unknown products " + std::to_string(o->products));
-    StepNumbers numbers;
+    std::vector<StepNumbers> numbers;
     return step_bounds(*o, numbers);
 }
 
@@ -123,6 +135,7 @@ struct Chunk {
     int64_t tiles[kTileKinds] = {};
     int64_t halves = 0;  // of the intermediate matrices
     int products = 0;    // FSADAM_PRODUCTS_* of its launches
+    bool pairs() const { return products == FSADAM_PRODUCTS_SPLIT; }  // steps are taken two at a time (run_chunk)
     int64_t head_bytes() const { return up((int64_t)rows.size() * sizeof(MatrixRow), 256) + up(matrices * 8, 256) + up(tiles[kTilesChunk] * 8, 256); }
     int64_t bytes() const { return head_bytes() + halves * 2; }
 };
@@ -134,7 +147,8 @@ int64_t full_tiles(int64_t s, int64_t l, int64_t t) { return ((s + t - 1) / t) *
 int64_t add_to_chunk(Chunk& chunk, const MatrixRow& proto, int64_t batch) {
     const int64_t products = chunk.products;
     const int64_t x = 2 * (int64_t)proto.s64 * proto.l64, a = products * (int64_t)proto.s64 * proto.s64;  // halves of one matrix, one buffer
-    const int64_t per = 2 * (x + a), room = kChunkBytes / 2 - chunk.halves;
+    const int squares = chunk.pairs() ? 3 : 2;
+    const int64_t per = 2 * x + squares * a, room = kChunkBytes / 2 - chunk.halves;
     int64_t n = std::min(batch, room / per);
     int64_t most = kMaxTiles;
     for (int k = 0; k < kTileKinds; ++k) most = std::min(most, (kMaxTiles - chunk.tiles[k]) / proto.n[k]);
@@ -152,9 +166,11 @@ int64_t add_to_chunk(Chunk& chunk, const MatrixRow& proto, int64_t batch) {
     }
     row.x_off[0] = chunk.halves;
     row.x_off[1] = row.x_off[0] + n * x;
-    row.a_off = row.x_off[1] + n * x;
-    row.b_off = row.a_off + n * a;
-    chunk.halves = row.b_off + n * a;
+    chunk.halves = row.x_off[1] + n * x;
+    for (int k = 0; k < squares; ++k) {
+        row.sq_off[k] = chunk.halves;
+        chunk.halves += n * a;
+    }
     chunk.matrices += n;
     chunk.rows.push_back(row);
     return n;
@@ -190,6 +206,8 @@ void make_chunks(const std::vector<Source>& all, int asked, std::vector<Chunk>& 
         row.dst_ld = in.dst_ld; row.dst_stride = in.dst_stride;
         row.step_ratio = in.step_ratio;
         row.chunks = (int32_t)(up(in.rows * in.cols, kChunkElems) / kChunkElems);
+        row.n[kTilesSym64] = (int32_t)symmetric_tiles(row.s64, 64);
+        row.n[kTilesFull64] = (int32_t)full_tiles(row.s64, row.l64, 64);
         row.n[kTilesSym128] = (int32_t)symmetric_tiles(row.s64, 128);
         row.n[kTilesFull128] = (int32_t)full_tiles(row.s64, row.l64, 128);
         row.n[kTilesSym256] = (int32_t)symmetric_tiles(row.s64, 256);
@@ -230,22 +248,34 @@ int check_shape(int64_t t, int64_t batch, int64_t rows, int64_t cols) {
 
 // ---- launches -----------------------------------------------------------------------------------------------------
 
+template <int STAGE, int PLANES>
+void launch_tiles(const Chunk& c, const MatrixRow* table, const StageArgs& k, _Float16* work, hipStream_t stream) {
+    constexpr bool kSym = STAGE == kStageGram || STAGE == kStageSquare;
+    const int64_t t64 = c.tiles[kSym ? kTilesSym64 : kTilesFull64], t128 = c.tiles[kSym ? kTilesSym128 : kTilesFull128], t256 = c.tiles[kSym ? kTilesSym256 : kTilesFull256];
+    const int n = (int)c.rows.size();
+    static const int force = getenv("FM_TILE") ? atoi(getenv("FM_TILE")) : 0;
+#define FM_LAUNCH(TILE, WM, WN, BK, DEPTH, COUNT)     hipLaunchKernelGGL((fsadam_matrix_stage<STAGE, TILE, TILE, WM, WN, BK, DEPTH, PLANES>), dim3((uint32_t)COUNT), dim3(64 * WM * WN), 0, stream, table, n, k, work)
+    if (force == 256) FM_LAUNCH(256, 2, 4, (PLANES == 2 ? 32 : 64), 2, t256);
+    else if (force == 1288) FM_LAUNCH(128, 2, 4, (PLANES == 2 ? 32 : 64), 2, t128);
+    else if (force == 642) FM_LAUNCH(64, 2, 2, 64, 2, t64);
+    else {
+        const auto cost = [](int64_t tiles, int64_t unit) { return (tiles + 255) / 256 * unit; };
+        const int64_t c64 = cost(t64, 13), c128 = cost(t128, 30), c256 = cost(t256, 92);
+        if (c256 < c128 && c256 < c64) FM_LAUNCH(256, 2, 4, (PLANES == 2 ? 32 : 64), 2, t256);
+        else if (c128 < c64) FM_LAUNCH(128, 2, 4, (PLANES == 2 ? 32 : 64), 2, t128);
+        else FM_LAUNCH(64, 2, 2, 64, 2, t64);
+    }
+#undef FM_LAUNCH
+}
 template <int PLANES>
 int launch_stage(int stage, const Chunk& c, const MatrixRow* table, const StageArgs& k, _Float16* work, hipStream_t stream) {
-    const int n = (int)c.rows.size();
-    constexpr int BK = PLANES == 2 ? 32 : 64;
-    const bool sym = stage == kStageGram || stage == kStagePoly;
-    const dim3 grid((uint32_t)c.tiles[sym ? kTilesSym128 : kTilesFull128]), block(256);
-#define FM_STAGE(S) \
-    case S: hipLaunchKernelGGL((fsadam_matrix_stage<S, 128, 128, 2, 2, BK, 2, PLANES>), grid, block, 0, stream, table, n, k, work); break
     switch (stage) {
-        FM_STAGE(kStageGram);
-        FM_STAGE(kStagePoly);
-        FM_STAGE(kStageUpdate);
-        FM_STAGE(kStageOut);
-        FM_STAGE(kStageStep);
+        case kStageGram: launch_tiles<kStageGram, PLANES>(c, table, k, work, stream); break;
+        case kStageSquare: launch_tiles<kStageSquare, PLANES>(c, table, k, work, stream); break;
+        case kStageUpdate: launch_tiles<kStageUpdate, PLANES>(c, table, k, work, stream); break;
+        case kStageOut: launch_tiles<kStageOut, PLANES>(c, table, k, work, stream); break;
+        case kStageStep: launch_tiles<kStageStep, PLANES>(c, table, k, work, stream); break;
     }
-#undef FM_STAGE
     return launched();
 }
 
@@ -253,7 +283,7 @@ struct Call {
     bool step;
     int src_type, dst_type, copy_type;
     FsOrthOptions options;
-    StepNumbers numbers;
+    std::vector<StepNumbers> numbers;
     MomentumArgs momentum;
     float keep;
 };
@@ -262,7 +292,7 @@ template <bool STEP>
 void launch_prepare(const Chunk& c, const Call& call, const MatrixRow* table, double* inverse, double* partials, _Float16* work, hipStream_t stream) {
     const int n = (int)c.rows.size();
     const dim3 chunks((uint32_t)c.tiles[kTilesChunk]), matrices((uint32_t)c.matrices), tiles((uint32_t)c.tiles[kTilesPrep]), block(256);
-    const double power = std::ldexp(1.0, call.numbers.x[0]);
+    const double power = std::ldexp(1.0, call.numbers[0].x);
 #define FM_TYPE(T, EACH) \
     if (call.src_type == T) { EACH(T); }
 #define FM_CHUNKS(T) hipLaunchKernelGGL((fsadam_matrix_chunks<T, STEP>), chunks, block, 0, stream, table, n, call.momentum, partials)
@@ -297,23 +327,52 @@ int run_chunk(const Chunk& c, const Call& call, void* workspace, hipStream_t str
     if (rc) return rc;
 
     const FsOrthOptions& o = call.options;
-    const StepNumbers& n = call.numbers;
-    for (int s = 0; s < o.steps; ++s) {
-        StageArgs k{};
-        k.from = s & 1;
-        k.to = k.from ^ 1;
-        k.dst_type = call.dst_type;
-        k.copy_type = call.copy_type;
-        k.keep = call.keep;
-        auto stage = [&](int which, double linear, int linear_exp, double product, int product_exp) {
-            k.linear = (float)std::ldexp(linear, linear_exp);
-            k.product = (float)std::ldexp(product, product_exp);
-            return c.products == FSADAM_PRODUCTS_SPLIT ? launch_stage<2>(which, c, table, k, work, stream) : launch_stage<1>(which, c, table, k, work, stream);
-        };
-        if ((rc = stage(kStageGram, 0.0, 0, 1.0, n.a[s] - 2 * n.x[s]))) return rc;
-        if ((rc = stage(kStagePoly, o.b, n.b[s] - n.a[s], o.c, n.b[s] - 2 * n.a[s]))) return rc;
-        const int which = s + 1 < o.steps ? kStageUpdate : call.step ? kStageStep : kStageOut;
-        if ((rc = stage(which, o.a, n.x[s + 1] - n.x[s], 1.0, n.x[s + 1] - n.b[s] - n.x[s]))) return rc;
+    const std::vector<StepNumbers>& n = call.numbers;
+    StageArgs k{};
+    k.dst_type = call.dst_type;
+    k.copy_type = call.copy_type;
+    k.keep = call.keep;
+    auto stage = [&](int which) {
+        return c.products == FSADAM_PRODUCTS_SPLIT ? launch_stage<2>(which, c, table, k, work, stream) : launch_stage<1>(which, c, table, k, work, stream);
+    };
+    auto square = [&](int p, int q, int add, double linear, int linear_exp, double product, int product_exp, double diagonal, int into) {
+        k.p = p; k.q = q; k.add = add; k.into = into;
+        k.linear = (float)std::ldexp(linear, linear_exp);
+        k.product = (float)std::ldexp(product, product_exp);
+        k.diagonal = (float)diagonal;
+        return stage(kStageSquare);
+    };
+    int s = 0, from = 0;
+    while (s < o.steps) {
+        const bool pair = c.pairs() && s + 2 <= o.steps;
+        const StepNumbers& n0 = n[s];
+        const int after = s + (pair ? 2 : 1), next_x = after < o.steps ? n[after].x : 0;
+        const int last = after < o.steps ? kStageUpdate : call.step ? kStageStep : kStageOut;
+        k.from = from;
+        k.to = from ^ 1;
+        k.into = 0;
+        k.product = (float)std::ldexp(1.0, n0.a - 2 * n0.x);
+        if ((rc = stage(kStageGram))) return rc;  // 0: A
+        if (pair) {
+            const StepNumbers& n1 = n[s + 1];
+            const int q = exponent_for(n0.q_bound * n1.q_bound);
+            if ((rc = square(0, 0, 0, o.b, n0.r - n0.a, o.c, n0.r - 2 * n0.a, std::ldexp((double)o.a, n0.r), 1))) return rc;  // 1: R
+            if ((rc = square(1, 0, -1, 0.0, 0, 1.0, n0.t - n0.r - n0.a, 0.0, 2))) return rc;                                  // 2: R A
+            if ((rc = square(2, 1, -1, 0.0, 0, 1.0, n1.a - n0.t - n0.r, 0.0, 0))) return rc;                                  // 0: R A R, the next A
+            if ((rc = square(0, 0, 0, o.b, n1.r - n1.a, o.c, n1.r - 2 * n1.a, std::ldexp((double)o.a, n1.r), 2))) return rc;  // 2: the next R
+            if ((rc = square(2, 1, -1, 0.0, 0, 1.0, q - n1.r - n0.r, 0.0, 0))) return rc;                                     // 0: their product
+            k.p = 0;
+            k.linear = 0.0f;
+            k.product = (float)std::ldexp(1.0, next_x - q - n0.x);
+        } else {
+            if ((rc = square(0, 0, 0, o.b, n0.b - n0.a, o.c, n0.b - 2 * n0.a, 0.0, 1))) return rc;  // 1: B
+            k.p = 1;
+            k.linear = (float)std::ldexp((double)o.a, next_x - n0.x);
+            k.product = (float)std::ldexp(1.0, next_x - n0.b - n0.x);
+        }
+        if ((rc = stage(last))) return rc;
+        from ^= 1;
+        s = after;
     }
     return FSADAM_OK;
 }

@@ -37,7 +37,7 @@ typedef float float4_t __attribute__((ext_vector_type(4)));
 enum { kTypeF32 = 0, kTypeF16 = 1, kTypeBF16 = 2 };
 
 // Which of a row's tile counts a launch goes by.
-enum { kTilesSym128, kTilesFull128, kTilesSym256, kTilesFull256, kTilesPrep, kTilesChunk, kTileKinds };
+enum { kTilesSym64, kTilesFull64, kTilesSym128, kTilesFull128, kTilesSym256, kTilesFull256, kTilesPrep, kTilesChunk, kTileKinds };
 
 // One row of a call's table: `batch` matrices of one shape, equally spaced.
 struct alignas(16) MatrixRow {
@@ -47,7 +47,8 @@ struct alignas(16) MatrixRow {
     void* copy;        // step, mixed precision: the 16-bit parameters
     int64_t src_ld, src_stride, dst_ld, dst_stride;  // elements from row to row, from matrix to matrix
     int64_t x_off[2];  // workspace: X and its successor (halves from the workspace's start)
-    int64_t a_off, b_off;
+    int64_t sq_off[3]; // workspace: square matrices (A and B; a pair of steps uses all three)
+    int64_t unused;
     int32_t batch, rows, cols;
     int32_t s, l, s64, l64;
     int32_t tall;      // rows > cols: X is the transpose
@@ -335,11 +336,13 @@ __global__ __launch_bounds__(256) void fsadam_matrix_normalise(const MatrixRow* 
 
 // ---- the products -------------------------------------------------------------------------------------------------
 
-enum { kStageGram, kStagePoly, kStageUpdate, kStageOut, kStageStep };
+enum { kStageGram, kStageSquare, kStageUpdate, kStageOut, kStageStep };
 
 struct StageArgs {
     int from, to;       // which of the two X buffers is read and written
+    int p, q, add, into;  // square matrices: operands, what is added (< 0: nothing), result.  Update: p is the left operand
     float linear, product;  // result = linear * (what is added) + product * (accumulator), powers of two included
+    float diagonal;     // square matrices: added on the diagonal
     float keep;         // step: 1 - lr * weight_decay
     int dst_type, copy_type;  // out, step: kType*; copy_type < 0: no copies
 };
@@ -351,8 +354,11 @@ __device__ __forceinline__ int swizzle_nt(int row) {
     return BK == 64 ? (row & 7) : ((row >> 1) & 3);
 }
 // K x columns ("NN", read with the transposing LDS loads): pairs of chunks (32 bytes, 16 columns) exchanged so that the rows
-// one load touches (8g + 0..3 for the four groups g of 16 lanes) spread over the banks.
-__device__ __forceinline__ int swizzle_nn(int row) { return (row & 3) | (((row >> 3) & 1) << 2); }
+// one load touches (8g + 0..3 for the four groups g of 16 lanes) spread over the banks.  A row of 64 columns has four pairs only.
+template <int COLS>
+__device__ __forceinline__ int swizzle_nn(int row) {
+    return (row & 3) | (COLS > 64 ? ((row >> 3) & 1) << 2 : 0);
+}
 
 // 1 KiB straight from memory into LDS: every lane gives the address of 16 bytes, which land at dst + 16 * lane.
 // From assembly because of the wait: behind the builtin the compiler places a wait for ALL loads before the next read
@@ -380,6 +386,9 @@ struct Product {
     static constexpr int kStageHalves = PLANES * (kPanelP + kPanelQ);
     static constexpr int kLdsHalves = DEPTH * kStageHalves;
     static constexpr int kLoadsP = kPanelP / 512 / kWaves, kLoadsQ = kPanelQ / 512 / kWaves;  // 1 KiB loads of a wave, one plane
+    // registers for a second slice of operands beside the accumulators and the first: 256 per lane with two waves to a SIMD
+    static constexpr bool kAhead = MI * NJ * 4 + 2 * PLANES * (MI + NJ) * 4 <= 228;
+    static_assert(BK == 32 || BK == 64, "one or two slices of 32");
     static_assert(kLoadsP * 512 * kWaves == kPanelP && kLoadsQ * 512 * kWaves == kPanelQ, "panels divide among the waves");
 
     float4_t acc[MI][NJ];
@@ -404,7 +413,7 @@ struct Product {
                 constexpr int kChunks = TN / 8;  // of a row
                 const int r = (wave * kLoadsQ + n) * (64 / kChunks) + lane / kChunks;
                 const int slot = lane % kChunks;
-                int chunk = (((slot >> 1) ^ swizzle_nn(r)) << 1) | (slot & 1);
+                int chunk = (((slot >> 1) ^ swizzle_nn<TN>(r)) << 1) | (slot & 1);
                 const int last = rows_q / 8 - 1;
                 chunk = chunk < last ? chunk : last;
                 off_q[n] = (uint32_t)(r * ld_q + chunk * 8);
@@ -444,58 +453,96 @@ struct Product {
         if constexpr (NN) {
             const int r = 8 * g + (c >> 2);
 #pragma unroll
-            for (int j = 0; j < NJ; ++j) nn_at[j] = r * TN + (((wn * (TN / WN) / 16 + j) ^ swizzle_nn(r)) * 16) + (c & 3) * 4;
+            for (int j = 0; j < NJ; ++j) nn_at[j] = r * TN + (((wn * (TN / WN) / 16 + j) ^ swizzle_nn<TN>(r)) * 16) + (c & 3) * 4;
         }
 
         constexpr int kLoads = PLANES * (kLoadsP + kLoadsQ);  // of a wave for one panel pair
+        constexpr int kSlices = BK / 32;                      // of a panel, 32 deep: what one matrix instruction takes
         const int n_k = k_total / BK;
         int fetched = 0, into = 0;
         for (; fetched < DEPTH - 1 && fetched < n_k; ++fetched) fetch(lds_at + fetched * kStageHalves * 2);
         into = fetched % DEPTH;
-        const _Float16* now = lds;
-        for (int step = 0; step < n_k; ++step) {
-            // panel `step` is there for this wave, behind the barrier for all, and behind it all are done with panel step - 1
-            if (fetched - step == DEPTH - 1) loads_arrived<kLoads*(DEPTH - 2)>();
+        int waited = 0;  // panels that are there
+        // Panel `waited` is there for this wave, behind the barrier for all; and behind it every wave has read all of the
+        // panel before, whose place the next fetch takes.
+        auto next_panel = [&] {
+            if (fetched - waited == DEPTH - 1) loads_arrived<kLoads*(DEPTH - 2)>();
             else loads_arrived<0>();
             __syncthreads();
+            ++waited;
             if (fetched < n_k) {
                 fetch(lds_at + into * kStageHalves * 2);
                 ++fetched;
                 into = into + 1 == DEPTH ? 0 : into + 1;
             }
+        };
+        struct Slice {
+            half8_t p[PLANES][MI], q[PLANES][NJ];
+        };
+        auto read = [&](Slice& f, const _Float16* now, int kk) {
 #pragma unroll
-            for (int kk = 0; kk < BK / 32; ++kk) {
-                half8_t fp[PLANES][MI], fq[PLANES][NJ];
+            for (int plane = 0; plane < PLANES; ++plane) {
+                const _Float16* lp = now + plane * kPanelP + row_p * BK + ((kk * 4 + g) ^ turn_p) * 8;
+                const _Float16* lq = now + PLANES * kPanelP + plane * kPanelQ;
 #pragma unroll
-                for (int plane = 0; plane < PLANES; ++plane) {
-                    const _Float16* lp = now + plane * kPanelP + row_p * BK + ((kk * 4 + g) ^ turn_p) * 8;
-                    const _Float16* lq = now + PLANES * kPanelP + plane * kPanelQ;
-#pragma unroll
-                    for (int j = 0; j < NJ; ++j) {
-                        if constexpr (NN) {
-                            const short4_t low = __builtin_amdgcn_ds_read_tr16_b64_v4i16((FM_LDS short4_t*)(lq + nn_at[j] + kk * 32 * TN));
-                            const short4_t high = __builtin_amdgcn_ds_read_tr16_b64_v4i16((FM_LDS short4_t*)(lq + nn_at[j] + (kk * 32 + 4) * TN));
-                            const half4_t l4 = __builtin_bit_cast(half4_t, low), h4 = __builtin_bit_cast(half4_t, high);
-                            fq[plane][j] = __builtin_shufflevector(l4, h4, 0, 1, 2, 3, 4, 5, 6, 7);
-                        } else {
-                            fq[plane][j] = *reinterpret_cast<const half8_t*>(lq + row_q * BK + ((kk * 4 + g) ^ turn_q) * 8 + j * 16 * BK);
-                        }
+                for (int j = 0; j < NJ; ++j) {
+                    if constexpr (NN) {
+                        const short4_t low = __builtin_amdgcn_ds_read_tr16_b64_v4i16((FM_LDS short4_t*)(lq + nn_at[j] + kk * 32 * TN));
+                        const short4_t high = __builtin_amdgcn_ds_read_tr16_b64_v4i16((FM_LDS short4_t*)(lq + nn_at[j] + (kk * 32 + 4) * TN));
+                        const half4_t l4 = __builtin_bit_cast(half4_t, low), h4 = __builtin_bit_cast(half4_t, high);
+                        f.q[plane][j] = __builtin_shufflevector(l4, h4, 0, 1, 2, 3, 4, 5, 6, 7);
+                    } else {
+                        f.q[plane][j] = *reinterpret_cast<const half8_t*>(lq + row_q * BK + ((kk * 4 + g) ^ turn_q) * 8 + j * 16 * BK);
                     }
-#pragma unroll
-                    for (int i = 0; i < MI; ++i) fp[plane][i] = *reinterpret_cast<const half8_t*>(lp + i * 16 * BK);
                 }
 #pragma unroll
-                for (int i = 0; i < MI; ++i)
-#pragma unroll
-                    for (int j = 0; j < NJ; ++j) {
-                        if constexpr (PLANES == 2) {
-                            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fp[1][i], fq[0][j], acc[i][j], 0, 0, 0);
-                            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fp[0][i], fq[1][j], acc[i][j], 0, 0, 0);
-                        }
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fp[0][i], fq[0][j], acc[i][j], 0, 0, 0);
-                    }
+                for (int i = 0; i < MI; ++i) f.p[plane][i] = *reinterpret_cast<const half8_t*>(lp + i * 16 * BK);
             }
-            now = step % DEPTH == DEPTH - 1 ? lds : now + kStageHalves;
+        };
+        auto multiply = [&](const Slice& f) {
+#pragma unroll
+            for (int i = 0; i < MI; ++i)
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) {
+                    if constexpr (PLANES == 2) {
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.p[1][i], f.q[0][j], acc[i][j], 0, 0, 0);
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.p[0][i], f.q[1][j], acc[i][j], 0, 0, 0);
+                    }
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.p[0][i], f.q[0][j], acc[i][j], 0, 0, 0);
+                }
+        };
+        const _Float16* now = lds;
+        if constexpr (kAhead) {
+            // the next slice is read while this one is multiplied, across the barrier between panels too
+            Slice f[2];
+            next_panel();
+            read(f[0], now, 0);
+            for (int step = 0; step < n_k; step += 2 / kSlices) {
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {  // two slices: f[0], f[1]
+                    const int panel = step + n / kSlices, kk = n % kSlices;
+                    if (kSlices == 1 && panel >= n_k) break;
+                    if (kk + 1 < kSlices) {
+                        read(f[1 - n], now, kk + 1);
+                    } else if (panel + 1 < n_k) {
+                        next_panel();
+                        now = (panel + 1) % DEPTH == 0 ? lds : now + kStageHalves;
+                        read(f[1 - n], now, 0);
+                    }
+                    multiply(f[n]);
+                }
+            }
+        } else {
+            for (int step = 0; step < n_k; ++step) {
+                next_panel();
+#pragma unroll
+                for (int kk = 0; kk < kSlices; ++kk) {
+                    Slice f;
+                    read(f, now, kk);
+                    multiply(f);
+                }
+                now = step % DEPTH == DEPTH - 1 ? lds : now + kStageHalves;
+            }
         }
         __syncthreads();  // the epilogue writes over the panels
     }
@@ -530,14 +577,14 @@ __device__ __forceinline__ void load_planes(const _Float16* at, int64_t plane, f
 // One stage of the iteration over every matrix of the chunk.
 template <int STAGE, int TM, int TN, int WM, int WN, int BK, int DEPTH, int PLANES>
 __global__ __launch_bounds__(64 * WM * WN) void fsadam_matrix_stage(const MatrixRow* table, int n_rows, StageArgs k, _Float16* work) {
-    constexpr bool kSym = STAGE == kStageGram || STAGE == kStagePoly;
+    constexpr bool kSym = STAGE == kStageGram || STAGE == kStageSquare;
     constexpr bool kNN = !kSym;
     using Prod = Product<TM, TN, WM, WN, BK, DEPTH, PLANES, kNN>;
     constexpr int kSlab = 64, kStride = TN + 4;  // the accumulators pass through LDS 64 rows at a time
     constexpr int kLdsBytes = Prod::kLdsHalves * 2 > kSlab * kStride * 4 ? Prod::kLdsHalves * 2 : kSlab * kStride * 4;
     __shared__ __attribute__((aligned(1024))) unsigned char lds[kLdsBytes];
 
-    constexpr int kind = kSym ? (TM == 128 ? kTilesSym128 : kTilesSym256) : (TM == 128 ? kTilesFull128 : kTilesFull256);
+    constexpr int kind = TM == 64 ? (kSym ? kTilesSym64 : kTilesFull64) : TM == 128 ? (kSym ? kTilesSym128 : kTilesFull128) : (kSym ? kTilesSym256 : kTilesFull256);
     int matrix;
     uint32_t tile;
     const MatrixRow& row = find_tile(table, n_rows, kind, xcd_contiguous(blockIdx.x, gridDim.x), matrix, tile);
@@ -555,17 +602,17 @@ __global__ __launch_bounds__(64 * WM * WN) void fsadam_matrix_stage(const Matrix
     }
     const int64_t plane_x = (int64_t)s64 * l64, plane_a = (int64_t)s64 * s64;
     const _Float16* x = work + row.x_off[k.from] + (int64_t)matrix * 2 * plane_x;
-    _Float16* a = work + row.a_off + (int64_t)matrix * PLANES * plane_a;
-    _Float16* b = work + row.b_off + (int64_t)matrix * PLANES * plane_a;
+    auto square = [&](int which) { return work + row.sq_off[which] + (int64_t)matrix * PLANES * plane_a; };
     const int i0 = ti * TM, j0 = tj * TN;
 
     Prod prod;
     if constexpr (STAGE == kStageGram)
         prod.run(x + (int64_t)i0 * l64, l64, plane_x, s64 - i0, x + (int64_t)j0 * l64, l64, plane_x, s64 - j0, l64, reinterpret_cast<_Float16*>(lds));
-    else if constexpr (STAGE == kStagePoly)
-        prod.run(a + (int64_t)i0 * s64, s64, plane_a, s64 - i0, a + (int64_t)j0 * s64, s64, plane_a, s64 - j0, s64, reinterpret_cast<_Float16*>(lds));
+    else if constexpr (STAGE == kStageSquare)
+        prod.run(square(k.p) + (int64_t)i0 * s64, s64, plane_a, s64 - i0, square(k.q) + (int64_t)j0 * s64, s64, plane_a, s64 - j0, s64,
+                 reinterpret_cast<_Float16*>(lds));
     else
-        prod.run(b + (int64_t)i0 * s64, s64, plane_a, s64 - i0, x + j0, l64, plane_x, l64 - j0, s64, reinterpret_cast<_Float16*>(lds));
+        prod.run(square(k.p) + (int64_t)i0 * s64, s64, plane_a, s64 - i0, x + j0, l64, plane_x, l64 - j0, s64, reinterpret_cast<_Float16*>(lds));
 
     float* slab = reinterpret_cast<float*>(lds);
     // element (i, j) of the slab; columns are exchanged in blocks of 8 by the rows' block of 8, so that reading eight
@@ -580,20 +627,38 @@ __global__ __launch_bounds__(64 * WM * WN) void fsadam_matrix_stage(const Matrix
 #pragma unroll
         for (int q = 0; q < 8; ++q) v[q] = at_slab(i, j)[q * kStride];
     };
+    // eight neighbours of a square result, at `at` of its storage; element `on_diagonal` of them is on the diagonal
+    auto finish = [&](float (&v)[8], int64_t at, int on_diagonal) {
+        float w[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) v[q] *= k.product;
+        if constexpr (STAGE == kStageSquare) {
+            if (k.add >= 0) {
+                load_planes<PLANES>(square(k.add) + at, plane_a, w);
+#pragma unroll
+                for (int q = 0; q < 8; ++q) v[q] += k.linear * w[q];
+            }
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+                if (q == on_diagonal) v[q] += k.diagonal;
+        }
+        store_planes<PLANES>(square(k.into) + at, plane_a, v);
+    };
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / WN, wn = wave % WN;
     constexpr int kWaveRows = TM / WM, kPieces = kSlab * TN / 8;  // pieces of eight elements
+    constexpr int kPer = (kSlab < kWaveRows ? kSlab : kWaveRows) / 16;  // blocks of 16 rows a wave has in a slab
 #pragma unroll
     for (int part = 0; part < TM / kSlab; ++part) {
-        if (wm == part * kSlab / kWaveRows) {
-            constexpr int kPer = kSlab / 16;
-            const int first = (part * kSlab % kWaveRows) / 16;
+        if (kWaveRows > kSlab ? wm == part * kSlab / kWaveRows : wm * kWaveRows / kSlab == part) {
+            const int first = (part * kSlab % kWaveRows) / 16;  // of the wave's blocks
+            const int down = kWaveRows < kSlab ? wm * kWaveRows % kSlab : 0;  // its rows in the slab
 #pragma unroll
             for (int i = 0; i < kPer; ++i)
 #pragma unroll
                 for (int j = 0; j < Prod::NJ; ++j)
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
-                        *at_slab(i * 16 + (lane >> 4) * 4 + r, wn * (TN / WN) + j * 16 + (lane & 15)) = prod.acc[first + i][j][r];
+                        *at_slab(down + i * 16 + (lane >> 4) * 4 + r, wn * (TN / WN) + j * 16 + (lane & 15)) = prod.acc[first + i][j][r];
         }
         __syncthreads();
         const int r0 = i0 + part * kSlab;  // the slab's first row in the result
@@ -606,15 +671,8 @@ __global__ __launch_bounds__(64 * WM * WN) void fsadam_matrix_stage(const Matrix
                     const int64_t at = (int64_t)(r0 + i) * width + j0 + j;
                     float v[8], w[8];
                     along_row(i, j, v);
-                    if constexpr (STAGE == kStageGram) {
-#pragma unroll
-                        for (int q = 0; q < 8; ++q) v[q] *= k.product;
-                        store_planes<PLANES>(a + at, plane_a, v);
-                    } else if constexpr (STAGE == kStagePoly) {
-                        load_planes<PLANES>(a + at, plane_a, w);
-#pragma unroll
-                        for (int q = 0; q < 8; ++q) v[q] = k.linear * w[q] + k.product * v[q];
-                        store_planes<PLANES>(b + at, plane_a, v);
+                    if constexpr (kSym) {
+                        finish(v, at, r0 + i - (j0 + j));
                     } else {
                         load_planes<2>(x + at, plane_x, w);
 #pragma unroll
@@ -628,18 +686,9 @@ __global__ __launch_bounds__(64 * WM * WN) void fsadam_matrix_stage(const Matrix
                             const int j = e / (kSlab / 8), i = (e % (kSlab / 8)) * 8;
                             if (j0 + j >= s64) continue;
                             const int64_t at = (int64_t)(j0 + j) * s64 + r0 + i;
-                            float v[8], w[8];
+                            float v[8];
                             along_column(i, j, v);
-                            if constexpr (STAGE == kStageGram) {
-#pragma unroll
-                                for (int q = 0; q < 8; ++q) v[q] *= k.product;
-                                store_planes<PLANES>(a + at, plane_a, v);
-                            } else {
-                                load_planes<PLANES>(a + at, plane_a, w);
-#pragma unroll
-                                for (int q = 0; q < 8; ++q) v[q] = k.linear * w[q] + k.product * v[q];
-                                store_planes<PLANES>(b + at, plane_a, v);
-                            }
+                            finish(v, at, -8);
                         }
                     }
                 }
@@ -688,7 +737,7 @@ __global__ __launch_bounds__(64 * WM * WN) void fsadam_matrix_stage(const Matrix
 }
 
 // Rows of a call's table, in the arguments of the launch: nothing is allocated or copied, and a captured graph holds them.
-constexpr int kRowsPerPut = 20;
+constexpr int kRowsPerPut = 16;
 struct MatrixRows {
     MatrixRow row[kRowsPerPut];
 };
