@@ -514,6 +514,7 @@ struct Product {
         const _Float16* now = lds;
         if constexpr (kAhead) {
             // the next slice is read while this one is multiplied, across the barrier between panels too
+            constexpr int kReads = PLANES * (MI + NJ * (NN ? 2 : 1)), kProducts = MI * NJ * (PLANES == 2 ? 3 : 1);
             Slice f[2];
             next_panel();
             read(f[0], now, 0);
@@ -530,6 +531,13 @@ struct Product {
                         read(f[1 - n], now, 0);
                     }
                     multiply(f[n]);
+                    // a few matrix instructions behind every read: in the order of the text the matrix cores would wait
+                    // until a wave has got all its reads into the queue
+#pragma unroll
+                    for (int r = 0; r < kReads; ++r) {
+                        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                        __builtin_amdgcn_sched_group_barrier(0x008, kProducts / kReads, 0);
+                    }
                 }
             }
         } else {
