@@ -133,6 +133,32 @@ __device__ __forceinline__ void split_halves(float v, _Float16& hi, _Float16& lo
     lo = (_Float16)(v - (float)hi);
 }
 
+// Eight values as one or two planes of halves.
+template <int PLANES>
+__device__ __forceinline__ void store_planes(_Float16* at, int64_t plane, const float (&v)[8]) {
+    half8_t hi, lo;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+        _Float16 h, o;
+        split_halves(v[q], h, o);
+        hi[q] = h;
+        lo[q] = o;
+    }
+    *reinterpret_cast<half8_t*>(at) = hi;
+    if constexpr (PLANES == 2) *reinterpret_cast<half8_t*>(at + plane) = lo;
+}
+template <int PLANES>
+__device__ __forceinline__ void load_planes(const _Float16* at, int64_t plane, float (&v)[8]) {
+    const half8_t hi = *reinterpret_cast<const half8_t*>(at);
+#pragma unroll
+    for (int q = 0; q < 8; ++q) v[q] = (float)hi[q];
+    if constexpr (PLANES == 2) {
+        const half8_t lo = *reinterpret_cast<const half8_t*>(at + plane);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) v[q] += (float)lo[q];
+    }
+}
+
 // Workgroups are handed to the 8 XCDs in turn, each with an L2 of its own: give every XCD a contiguous range of tiles.
 __device__ __forceinline__ uint32_t xcd_contiguous(uint32_t block, uint32_t n) {
     const uint32_t per = n / 8, extra = n % 8, xcd = block % 8, at = block / 8;
@@ -186,15 +212,41 @@ __device__ __forceinline__ double block_sum(double v) {
     return part[0] + part[1] + part[2] + part[3];
 }
 
+// A thread's share of the sum of p[0 .. n - 1], eight loads at a time in flight.
+__device__ __forceinline__ double sum_of(const double* p, int64_t n) {
+    double sum = 0.0;
+    for (int64_t i = threadIdx.x; i < n; i += 8 * kChunkThreads) {
+        double v[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) v[q] = i + q * kChunkThreads < n ? p[i + q * kChunkThreads] : 0.0;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) sum += v[q];
+    }
+    return sum;
+}
+
 // One row of the momentum pass's table: a tensor as a line of elements.
 struct alignas(16) MomentumRow {
     const void* g;
     float* m;
-    void* u;          // NULL: the update is not stored (the step takes it from g and m again)
+    void* u;
     int64_t numel;
     int64_t first;    // chunks of the rows before this one
 };
 
+// Elements `begin` to `end` of a line, eight to a thread: calls each(first element, how many) for every piece.  With whole eights
+// all pieces of a thread are independent, so that their loads are all in flight before the first is used.
+template <typename Each>
+__device__ __forceinline__ void for_eights(int64_t begin, int64_t end, Each&& each) {
+    if (end - begin == kChunkElems) {
+#pragma unroll
+        for (int n = 0; n < kChunkElems / 8 / kChunkThreads; ++n) each(begin + (n * kChunkThreads + threadIdx.x) * 8, 8);
+    } else {
+        for (int64_t i = begin + threadIdx.x * 8; i < end; i += kChunkThreads * 8) each(i, end - i < 8 ? (int)(end - i) : 8);
+    }
+}
+
+// Bound by HBM: 2 + 4 bytes read and 2 + 4 written per element with 16-bit gradients and updates.
 template <int GT, int UT>
 __global__ __launch_bounds__(kChunkThreads) void fsadam_momentum_chunks(const MomentumRow* table, int n_rows, MomentumArgs k, double* partials) {
     int low = 0, high = n_rows - 1;
@@ -209,14 +261,20 @@ __global__ __launch_bounds__(kChunkThreads) void fsadam_momentum_chunks(const Mo
     const int64_t end = begin + kChunkElems < row.numel ? begin + kChunkElems : row.numel;
     const float scale = k.scale_dev ? *k.scale_dev : k.scale;
     double sum = 0.0;
-    for (int64_t i = begin + threadIdx.x; i < end; i += kChunkThreads) {
-        float m = row.m[i];
-        const float u = momentum_update(load_as_float(row.g, i, GT), m, scale, k);
-        row.m[i] = m;
-        if (row.u) store_from_float(row.u, i, UT, u);
-        const double r = row.u ? (double)round_to(u, UT) : (double)u;
-        sum += r * r;
-    }
+    for_eights(begin, end, [&](int64_t i, int n) {
+        float g[8], m[8], u[8];
+        load_eight(row.g, i, GT, n, g);
+        load_eight(row.m, i, kTypeF32, n, m);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) u[q] = momentum_update(g[q], m[q], scale, k);
+        store_eight(row.m, i, kTypeF32, n, m);
+        store_eight(row.u, i, UT, n, u);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+            const double r = q < n ? (double)round_to(u[q], UT) : 0.0;
+            sum += r * r;
+        }
+    });
     sum = block_sum(sum);
     if (threadIdx.x == 0) partials[t] = sum;
 }
@@ -226,9 +284,7 @@ __global__ __launch_bounds__(kChunkThreads) void fsadam_momentum_chunks(const Mo
 __global__ __launch_bounds__(kChunkThreads) void fsadam_momentum_norms(const MomentumRow* table, const double* partials, float* norms, float* found_inf) {
     const MomentumRow& row = table[blockIdx.x];
     const int64_t n = (row.numel + kChunkElems - 1) / kChunkElems;
-    double sum = 0.0;
-    for (int64_t i = threadIdx.x; i < n; i += kChunkThreads) sum += partials[row.first + i];
-    sum = block_sum(sum);
+    const double sum = block_sum(sum_of(partials + row.first, n));
     if (threadIdx.x == 0) {
         if (norms) norms[blockIdx.x] = (float)sqrt(sum);
         if (found_inf && !__builtin_isfinite(sum)) *found_inf = 1.0f;
@@ -250,12 +306,25 @@ __global__ __launch_bounds__(kChunkThreads) void fsadam_matrix_chunks(const Matr
     if constexpr (STEP) {
         const float scale = k.scale_dev ? *k.scale_dev : k.scale;
         const int64_t base = (int64_t)matrix * numel;
-        for (int64_t i = begin + threadIdx.x; i < end; i += kChunkThreads) {
-            float m = row.buf[base + i];
-            const double u = (double)momentum_update(load_as_float(row.src, base + i, ST), m, scale, k);
-            row.buf[base + i] = m;
-            sum += u * u;
-        }
+        for_eights(begin, end, [&](int64_t i, int n) {
+            float g[8], m[8];
+            load_eight(row.src, base + i, ST, n, g);
+            load_eight(row.buf, base + i, kTypeF32, n, m);
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+                const double u = q < n ? (double)momentum_update(g[q], m[q], scale, k) : 0.0;
+                sum += u * u;
+            }
+            store_eight(row.buf, base + i, kTypeF32, n, m);
+        });
+    } else if (row.src_ld == row.cols) {
+        const int64_t base = (int64_t)matrix * row.src_stride;
+        for_eights(begin, end, [&](int64_t i, int n) {
+            float v[8];
+            load_eight(row.src, base + i, ST, n, v);
+#pragma unroll
+            for (int q = 0; q < 8; ++q) sum += q < n ? (double)v[q] * (double)v[q] : 0.0;
+        });
     } else {
         const int64_t base = (int64_t)matrix * row.src_stride;
         for (int64_t i = begin + threadIdx.x; i < end; i += kChunkThreads) {
@@ -279,9 +348,7 @@ __global__ __launch_bounds__(kChunkThreads) void fsadam_matrix_norms(const Matri
     }
     const MatrixRow& row = table[low];
     const double* p = partials + row.first[kTilesChunk] + (int64_t)((int)blockIdx.x - row.first_matrix) * row.chunks;
-    double sum = 0.0;
-    for (int i = threadIdx.x; i < row.chunks; i += kChunkThreads) sum += p[i];
-    sum = block_sum(sum);
+    const double sum = block_sum(sum_of(p, row.chunks));
     if (threadIdx.x == 0) {
         const double norm = sqrt(sum);
         inverse[blockIdx.x] = __builtin_isfinite(sum) ? 1.0 / (norm > eps ? norm : eps) : __builtin_nan("");
@@ -300,37 +367,46 @@ __global__ __launch_bounds__(256) void fsadam_matrix_normalise(const MatrixRow* 
     const int r0 = row.tall ? j0 : i0, c0 = row.tall ? i0 : j0;         // in the source
     const double factor = inverse[row.first_matrix + matrix] * power;
     const float scale = STEP ? (k.scale_dev ? *k.scale_dev : k.scale) : 1.0f;
-    for (int e = threadIdx.x; e < 64 * 64; e += 256) {
-        const int r = e >> 6, c = e & 63;
-        float v = 0.0f;
-        if (r0 + r < row.rows && c0 + c < row.cols) {
-            float u;
-            if constexpr (STEP) {
-                const int64_t at = (int64_t)matrix * row.rows * row.cols + (int64_t)(r0 + r) * row.cols + c0 + c;
-                u = update_again(load_as_float(row.src, at, ST), row.buf[at], scale, k);
-            } else {
-                u = load_as_float(row.src, (int64_t)matrix * row.src_stride + (int64_t)(r0 + r) * row.src_ld + c0 + c, ST);
-            }
-            v = (float)((double)u * factor);
-        }
-        tile[r][c] = v;
-    }
-    __syncthreads();
     const int64_t plane = (int64_t)row.s64 * row.l64;
     _Float16* x = work + row.x_off[0] + (int64_t)matrix * 2 * plane;
-    for (int e = threadIdx.x; e < 64 * 8; e += 256) {
-        const int i = e >> 3, j = (e & 7) * 8;
-        half8_t hi, lo;
-        for (int q = 0; q < 8; ++q) {
-            const float v = row.tall ? tile[j + q][i] : tile[i][j + q];
-            _Float16 h, o;
-            split_halves(v, h, o);
-            hi[q] = h;
-            lo[q] = o;
+    auto put = [&](int i, int j, const float (&v)[8]) { store_planes<2>(x + (int64_t)(i0 + i) * row.l64 + j0 + j, plane, v); };
+#pragma unroll
+    for (int part = 0; part < 2; ++part) {
+        const int e = threadIdx.x + part * 256, r = e >> 3, c = (e & 7) * 8;  // eight neighbours in the source
+        float v[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) v[q] = 0.0f;
+        const int left = r0 + r < row.rows ? row.cols - (c0 + c) : 0;
+        if (left > 0) {
+            if constexpr (STEP) {
+                const int64_t at = (int64_t)matrix * row.rows * row.cols + (int64_t)(r0 + r) * row.cols + c0 + c;
+                float m[8];
+                load_eight(row.src, at, ST, left, v);
+                load_eight(row.buf, at, kTypeF32, left, m);
+#pragma unroll
+                for (int q = 0; q < 8; ++q) v[q] = q < left ? update_again(v[q], m[q], scale, k) : 0.0f;
+            } else {
+                load_eight(row.src, (int64_t)matrix * row.src_stride + (int64_t)(r0 + r) * row.src_ld + c0 + c, ST, left, v);
+            }
+#pragma unroll
+            for (int q = 0; q < 8; ++q) v[q] = (float)((double)v[q] * factor);
         }
-        const int64_t at = (int64_t)(i0 + i) * row.l64 + j0 + j;
-        *reinterpret_cast<half8_t*>(x + at) = hi;
-        *reinterpret_cast<half8_t*>(x + plane + at) = lo;
+        if (!row.tall) {
+            put(r, c, v);
+        } else {
+#pragma unroll
+            for (int q = 0; q < 8; ++q) tile[r][c + q] = v[q];
+        }
+    }
+    if (!row.tall) return;
+    __syncthreads();
+#pragma unroll
+    for (int part = 0; part < 2; ++part) {
+        const int e = threadIdx.x + part * 256, i = e >> 3, j = (e & 7) * 8;
+        float v[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) v[q] = tile[j + q][i];
+        put(i, j, v);
     }
 }
 
@@ -556,32 +632,6 @@ struct Product {
     }
 };
 
-// Eight values as one or two planes of halves.
-template <int PLANES>
-__device__ __forceinline__ void store_planes(_Float16* at, int64_t plane, const float (&v)[8]) {
-    half8_t hi, lo;
-#pragma unroll
-    for (int q = 0; q < 8; ++q) {
-        _Float16 h, o;
-        split_halves(v[q], h, o);
-        hi[q] = h;
-        lo[q] = o;
-    }
-    *reinterpret_cast<half8_t*>(at) = hi;
-    if constexpr (PLANES == 2) *reinterpret_cast<half8_t*>(at + plane) = lo;
-}
-template <int PLANES>
-__device__ __forceinline__ void load_planes(const _Float16* at, int64_t plane, float (&v)[8]) {
-    const half8_t hi = *reinterpret_cast<const half8_t*>(at);
-#pragma unroll
-    for (int q = 0; q < 8; ++q) v[q] = (float)hi[q];
-    if constexpr (PLANES == 2) {
-        const half8_t lo = *reinterpret_cast<const half8_t*>(at + plane);
-#pragma unroll
-        for (int q = 0; q < 8; ++q) v[q] += (float)lo[q];
-    }
-}
-
 // One stage of the iteration over every matrix of the chunk.
 template <int STAGE, int TM, int TN, int WM, int WN, int BK, int DEPTH, int PLANES>
 __global__ __launch_bounds__(64 * WM * WN) void fsadam_matrix_stage(const MatrixRow* table, int n_rows, StageArgs k, _Float16* work) {
@@ -676,10 +726,19 @@ __global__ __launch_bounds__(64 * WM * WN) void fsadam_matrix_stage(const Matrix
                 for (int e = threadIdx.x; e < kPieces; e += Prod::kThreads) {
                     const int i = e / (TN / 8), j = (e % (TN / 8)) * 8;
                     if (j0 + j >= width) continue;
+                    // Every element of a symmetric result is its lower triangle's, also in a tile on the diagonal: what a matrix
+                    // gives does not depend on the tiles, and so not on the rest of the list.
+                    if (kSym && j0 + j > r0 + i) continue;
                     const int64_t at = (int64_t)(r0 + i) * width + j0 + j;
                     float v[8], w[8];
                     along_row(i, j, v);
                     if constexpr (kSym) {
+                        if (j0 + j + 7 > r0 + i) {  // the diagonal runs through these eight
+                            const int down = j0 + j - r0;  // the first one's column as a row of the slab
+#pragma unroll
+                            for (int q = 0; q < 8; ++q)
+                                if (j0 + j + q > r0 + i) v[q] = *at_slab(down + q, r0 + i - j0);
+                        }
                         finish(v, at, r0 + i - (j0 + j));
                     } else {
                         load_planes<2>(x + at, plane_x, w);
@@ -689,10 +748,10 @@ __global__ __launch_bounds__(64 * WM * WN) void fsadam_matrix_stage(const Matrix
                     }
                 }
                 if constexpr (kSym) {
-                    if (ti != tj) {  // the mirror image
+                    {  // the mirror image
                         for (int e = threadIdx.x; e < kPieces; e += Prod::kThreads) {
                             const int j = e / (kSlab / 8), i = (e % (kSlab / 8)) * 8;
-                            if (j0 + j >= s64) continue;
+                            if (j0 + j >= s64 || (j0 + j) / 8 >= (r0 + i) / 8) continue;
                             const int64_t at = (int64_t)(j0 + j) * s64 + r0 + i;
                             float v[8];
                             along_column(i, j, v);
