@@ -15,6 +15,7 @@
 #include <cstring>
 #include <exception>
 #include <string>
+#include <type_traits>
 #include <vector>
 
 #include "fsadam.h"
@@ -51,7 +52,6 @@ bool aligned(const void* p, uintptr_t bytes) { return reinterpret_cast<uintptr_t
 int64_t up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
 
 constexpr int64_t kMaxSide = 1 << 20;
-constexpr int kMaxSteps = 32;
 constexpr int64_t kMaxTiles = INT32_MAX / 2;  // of one launch
 // Intermediate matrices of one chunk.  Enough for eight 4096 x 11008 matrices, whose products then have thousands of
 // tiles for the 256 compute units; a matrix that needs more gets what it needs.
@@ -64,14 +64,14 @@ constexpr int64_t kChunkBytes = int64_t(4) << 30;
 double largest(const double* c, int n, double top) {
     auto value = [&](double t) { double v = 0.0; for (int i = n; i >= 0; --i) v = v * t + c[i]; return v; };
     auto slope = [&](double t) { double v = 0.0; for (int i = n; i >= 1; --i) v = v * t + i * c[i]; return v; };
-    constexpr int kSamples = 256;
+    constexpr int kSamples = 32;
     double most = std::max(std::fabs(value(0.0)), std::fabs(value(top)));
     for (int i = 0; i < kSamples; ++i) {
         double low = top * i / kSamples, high = top * (i + 1) / kSamples;
         most = std::max(most, std::fabs(value(low)));
         if ((slope(low) < 0.0) == (slope(high) < 0.0)) continue;
         const bool down = slope(low) < 0.0;
-        for (int k = 0; k < 50; ++k) {
+        for (int k = 0; k < 30; ++k) {
             const double mid = 0.5 * (low + high);
             if ((slope(mid) < 0.0) == down) low = mid;
             else high = mid;
@@ -189,11 +189,13 @@ struct Source {  // what a list entry's row starts from
 // call waits for.
 constexpr int64_t kAlwaysSplit = 128;
 
+bool resident(const Source& in) { return resident_fits(std::min(in.rows, in.cols), std::max(in.rows, in.cols)); }
+
 void make_chunks(const std::vector<Source>& all, int asked, std::vector<Chunk>& chunks) {
   for (int products : {FSADAM_PRODUCTS_HALF, FSADAM_PRODUCTS_SPLIT}) {
     bool fresh = true;  // a chunk is of one kind
     for (const Source& in : all) {
-        if ((std::min(in.rows, in.cols) <= kAlwaysSplit ? FSADAM_PRODUCTS_SPLIT : asked) != products) continue;
+        if (resident(in) || (std::min(in.rows, in.cols) <= kAlwaysSplit ? FSADAM_PRODUCTS_SPLIT : asked) != products) continue;
         MatrixRow row{};
         row.rows = (int32_t)in.rows;
         row.cols = (int32_t)in.cols;
@@ -232,11 +234,39 @@ void make_chunks(const std::vector<Source>& all, int asked, std::vector<Chunk>& 
   }
 }
 
-int64_t workspace_of(const std::vector<Chunk>& chunks) {
-    int64_t bytes = 0;
-    for (const Chunk& c : chunks) bytes = std::max(bytes, c.bytes());
-    return bytes;
-}
+// The rows of the list that fit LDS.
+struct Residents {
+    std::vector<ResidentRow> rows;
+    int64_t matrices = 0;
+    int lds_bytes = 0;  // of the largest
+    int64_t bytes() const { return rows.size() > kResidentRowsPerLaunch ? up((int64_t)(rows.size() * sizeof(ResidentRow)), 256) : 0; }
+};
+
+struct Plan {
+    Residents residents;
+    std::vector<Chunk> chunks;
+    Plan(const std::vector<Source>& list, int products) {
+        for (const Source& in : list) {
+            if (!resident(in)) continue;
+            ResidentRow row{};
+            row.src = in.src; row.buf = in.buf; row.dst = in.dst; row.copy = in.copy;
+            row.src_ld = in.src_ld; row.src_stride = in.src_stride; row.dst_ld = in.dst_ld; row.dst_stride = in.dst_stride;
+            row.rows = (int32_t)in.rows; row.cols = (int32_t)in.cols;
+            row.first_matrix = (int32_t)residents.matrices;
+            row.step_ratio = in.step_ratio;
+            residents.rows.push_back(row);
+            residents.matrices += in.batch;
+            const int s = std::min(row.rows, row.cols), l = std::max(row.rows, row.cols);
+            residents.lds_bytes = std::max(residents.lds_bytes, (int)up(s, 32) * (resident_pitch(s) + resident_pitch(l)) * 4);
+        }
+        make_chunks(list, products, chunks);
+    }
+    int64_t workspace() const {
+        int64_t bytes = residents.bytes();  // the residents' table comes first and is done with when the chunks begin
+        for (const Chunk& c : chunks) bytes = std::max(bytes, c.bytes());
+        return bytes;
+    }
+};
 
 int check_shape(int64_t t, int64_t batch, int64_t rows, int64_t cols) {
     if (batch < 0 || rows < 0 || cols < 0) return fail(FSADAM_EINVAL, "matrix " + std::to_string(t) + ": negative size");
@@ -377,12 +407,56 @@ int run_chunk(const Chunk& c, const Call& call, void* workspace, hipStream_t str
     return FSADAM_OK;
 }
 
-int run_call(const std::vector<Chunk>& chunks, Call& call, void* workspace, int64_t workspace_bytes, void* hip_stream) {
+int run_residents(const Residents& r, const Call& call, void* workspace, hipStream_t stream) {
+    if (r.matrices > kMaxTiles) return fail(FSADAM_EINVAL, "the list has too many matrices for one call");
+    const FsOrthOptions& o = call.options;
+    ResidentArgs k{};
+    k.steps = o.steps;
+    k.src_type = call.src_type; k.dst_type = call.dst_type; k.copy_type = call.copy_type;
+    k.keep = call.keep;
+    k.eps = o.eps;
+    k.power = std::ldexp(1.0, call.numbers[0].x);
+    for (int s = 0; s < o.steps; ++s) {
+        const StepNumbers& n = call.numbers[s];
+        const int next_x = s + 1 < o.steps ? call.numbers[s + 1].x : 0;
+        k.gram[s] = (float)std::ldexp(1.0, n.a - 2 * n.x);
+        k.linear_b[s] = (float)std::ldexp((double)o.b, n.b - n.a);
+        k.product_b[s] = (float)std::ldexp((double)o.c, n.b - 2 * n.a);
+        k.linear_x[s] = (float)std::ldexp((double)o.a, next_x - n.x);
+        k.product_x[s] = (float)std::ldexp(1.0, next_x - n.b - n.x);
+    }
+    auto launch = [&](const auto& table) {
+        using Table = std::decay_t<decltype(table)>;
+        const dim3 grid((uint32_t)r.matrices), block(kResidentThreads);
+        if (call.step) hipLaunchKernelGGL((fsadam_matrix_resident<true, Table>), grid, block, r.lds_bytes, stream, table, k, call.momentum);
+        else hipLaunchKernelGGL((fsadam_matrix_resident<false, Table>), grid, block, r.lds_bytes, stream, table, k, call.momentum);
+        return launched();
+    };
+    if (r.rows.size() <= kResidentRowsPerLaunch) {
+        ResidentInArguments table{};
+        table.n = (int)r.rows.size();
+        std::memcpy(table.rows.row, r.rows.data(), r.rows.size() * sizeof(ResidentRow));
+        return launch(table);
+    }
+    ResidentRow* memory = static_cast<ResidentRow*>(workspace);
+    for (size_t first = 0; first < r.rows.size(); first += kResidentRowsPerLaunch) {
+        ResidentRows rows;
+        const size_t n = std::min<size_t>(kResidentRowsPerLaunch, r.rows.size() - first);
+        std::memcpy(rows.row, r.rows.data() + first, n * sizeof(ResidentRow));
+        hipLaunchKernelGGL(fsadam_put_resident_rows, dim3(1), dim3(256), 0, stream, memory + first, (int)n, rows);
+    }
+    return launch(ResidentInMemory{memory, (int)r.rows.size()});
+}
+
+int run_call(const Plan& plan, Call& call, void* workspace, int64_t workspace_bytes, void* hip_stream) {
     int rc = step_bounds(call.options, call.numbers);
-    if (rc || chunks.empty()) return rc;
-    if (!workspace || !aligned(workspace, 256)) return fail(FSADAM_EINVAL, "the workspace must be a device pointer aligned to 256 bytes");
-    if (workspace_bytes < workspace_of(chunks))
-        return fail(FSADAM_EINVAL, "the workspace holds " + std::to_string(workspace_bytes) + " bytes, this list needs " + std::to_string(workspace_of(chunks)));
+    if (rc) return rc;
+    const std::vector<Chunk>& chunks = plan.chunks;
+    const int64_t need = plan.workspace();
+    if (need && (!workspace || !aligned(workspace, 256))) return fail(FSADAM_EINVAL, "the workspace must be a device pointer aligned to 256 bytes");
+    if (workspace_bytes < need)
+        return fail(FSADAM_EINVAL, "the workspace holds " + std::to_string(workspace_bytes) + " bytes, this list needs " + std::to_string(need));
+    if (!plan.residents.rows.empty() && (rc = run_residents(plan.residents, call, workspace, static_cast<hipStream_t>(hip_stream)))) return rc;
     for (const Chunk& c : chunks) {
         rc = run_chunk(c, call, workspace, static_cast<hipStream_t>(hip_stream));
         if (rc) return rc;
@@ -448,12 +522,15 @@ int momentum_rows(const FsMomentumTensor* t, int64_t n, std::vector<MomentumRow>
     for (int64_t k = 0; k < n; ++k) {
         if (t[k].numel < 0 || t[k].numel > (int64_t(1) << 42)) return fail(FSADAM_EINVAL, "tensor " + std::to_string(k) + ": numel out of range");
         rows.push_back({t[k].g, t[k].m, t[k].u, t[k].numel, chunks});
-        chunks += up(t[k].numel, kChunkElems) / kChunkElems;
+        chunks += up(t[k].numel, kMomentumElems) / kMomentumElems;
     }
     if (chunks > kMaxTiles || n > kMaxTiles) return fail(FSADAM_EINVAL, "the list has too many elements for one call");
     return FSADAM_OK;
 }
-int64_t momentum_bytes(int64_t rows, int64_t chunks) { return up(rows * (int64_t)sizeof(MomentumRow), 256) + up(chunks * 8, 256); }
+// The arguments of a launch are slow to read (they are not in the GPU's memory): worth it for a few workgroups only.
+bool table_in_arguments(int64_t rows, int64_t chunks) { return rows <= kMomentumRowsPerLaunch && chunks <= 2048; }
+int64_t momentum_table_bytes(int64_t rows) { return up(rows * (int64_t)sizeof(MomentumRow), 256); }
+int64_t momentum_bytes(int64_t rows, int64_t chunks) { return momentum_table_bytes(rows) + up(chunks * 8, 256); }
 
 }  // namespace
 
@@ -494,27 +571,37 @@ int fsadam_momentum_pass(const FsMomentumTensor* tensors, int64_t n_tensors, int
         if (workspace_bytes < momentum_bytes(n_tensors, chunks))
             return fail(FSADAM_EINVAL, "the workspace holds " + std::to_string(workspace_bytes) + " bytes, this list needs " + std::to_string(momentum_bytes(n_tensors, chunks)));
         hipStream_t stream = static_cast<hipStream_t>(hip_stream);
-        MomentumRow* table = static_cast<MomentumRow*>(workspace);
-        double* partials = reinterpret_cast<double*>(static_cast<char*>(workspace) + up(n_tensors * (int64_t)sizeof(MomentumRow), 256));
-        for (int64_t first = 0; first < n_tensors; first += kMomentumRowsPerPut) {
-            MomentumRows put;
-            const int64_t n = std::min<int64_t>(kMomentumRowsPerPut, n_tensors - first);
-            std::memcpy(put.row, rows.data() + first, (size_t)n * sizeof(MomentumRow));
-            hipLaunchKernelGGL(fsadam_put_momentum_rows, dim3(1), dim3(256), 0, stream, table + first, (int)n, put);
-        }
+        double* partials = reinterpret_cast<double*>(static_cast<char*>(workspace) + momentum_table_bytes(n_tensors));
         const MomentumArgs k = momentum_args(momentum, nesterov, scale, scale_dev);
-        if (chunks) {
+        auto launch = [&](const auto& table) {
+            using Table = std::decay_t<decltype(table)>;
             const dim3 grid((uint32_t)chunks), block(kChunkThreads);
 #define FM_PASS(G, U) \
-    if (grad_type == G && update_type == U) hipLaunchKernelGGL((fsadam_momentum_chunks<G, U>), grid, block, 0, stream, table, (int)n_tensors, k, partials)
-            FM_PASS(kTypeF32, kTypeF32); FM_PASS(kTypeF32, kTypeF16); FM_PASS(kTypeF32, kTypeBF16);
-            FM_PASS(kTypeF16, kTypeF32); FM_PASS(kTypeF16, kTypeF16); FM_PASS(kTypeF16, kTypeBF16);
-            FM_PASS(kTypeBF16, kTypeF32); FM_PASS(kTypeBF16, kTypeF16); FM_PASS(kTypeBF16, kTypeBF16);
+    if (grad_type == G && update_type == U) hipLaunchKernelGGL((fsadam_momentum_chunks<G, U, Table>), grid, block, 0, stream, table, k, partials)
+            if (chunks) {
+                FM_PASS(kTypeF32, kTypeF32); FM_PASS(kTypeF32, kTypeF16); FM_PASS(kTypeF32, kTypeBF16);
+                FM_PASS(kTypeF16, kTypeF32); FM_PASS(kTypeF16, kTypeF16); FM_PASS(kTypeF16, kTypeBF16);
+                FM_PASS(kTypeBF16, kTypeF32); FM_PASS(kTypeBF16, kTypeF16); FM_PASS(kTypeBF16, kTypeBF16);
+            }
 #undef FM_PASS
+            if (norms_dev || found_inf_dev)
+                hipLaunchKernelGGL((fsadam_momentum_norms<Table>), dim3((uint32_t)n_tensors), block, 0, stream, table, (const double*)partials, norms_dev, found_inf_dev);
+            return launched();
+        };
+        if (table_in_arguments(n_tensors, chunks)) {
+            InArguments table{};
+            table.n = (int)n_tensors;
+            std::memcpy(table.rows.row, rows.data(), (size_t)n_tensors * sizeof(MomentumRow));
+            return launch(table);
         }
-        if (norms_dev || found_inf_dev)
-            hipLaunchKernelGGL(fsadam_momentum_norms, dim3((uint32_t)n_tensors), dim3(kChunkThreads), 0, stream, table, (const double*)partials, norms_dev, found_inf_dev);
-        return launched();
+        MomentumRow* memory = static_cast<MomentumRow*>(workspace);
+        for (int64_t first = 0; first < n_tensors; first += kMomentumRowsPerLaunch) {
+            MomentumRows put;
+            const int64_t n = std::min<int64_t>(kMomentumRowsPerLaunch, n_tensors - first);
+            std::memcpy(put.row, rows.data() + first, (size_t)n * sizeof(MomentumRow));
+            hipLaunchKernelGGL(fsadam_put_momentum_rows, dim3(1), dim3(256), 0, stream, memory + first, (int)n, put);
+        }
+        return launch(InMemory{memory, (int)n_tensors});
     });
 }
 
@@ -525,9 +612,7 @@ int fsadam_orth_workspace(const FsMatrix* matrices, int64_t n, const FsOrthOptio
         if (rc) return rc;
         std::vector<Source> list;
         if ((rc = sources_of(matrices, n, 1, list))) return rc;
-        std::vector<Chunk> chunks;
-        make_chunks(list, options->products, chunks);
-        *bytes = workspace_of(chunks);
+        *bytes = Plan(list, options->products).workspace();
         return FSADAM_OK;
     });
 }
@@ -540,13 +625,12 @@ int fsadam_orthogonalize(const FsMatrix* matrices, int64_t n, int type, const Fs
         if (rc) return rc;
         std::vector<Source> list;
         if ((rc = sources_of(matrices, n, size_of(type), list))) return rc;
-        std::vector<Chunk> chunks;
-        make_chunks(list, options->products, chunks);
+        const Plan plan(list, options->products);
         Call call{};
         call.src_type = call.dst_type = type;
         call.copy_type = -1;
         call.options = *options;
-        return run_call(chunks, call, workspace, workspace_bytes, hip_stream);
+        return run_call(plan, call, workspace, workspace_bytes, hip_stream);
     });
 }
 
@@ -557,9 +641,7 @@ int fsadam_muon_workspace(const FsMuonTensor* tensors, int64_t n, const FsOrthOp
         if (rc) return rc;
         std::vector<Source> list;
         if ((rc = sources_of(tensors, n, 1, 1, 0, 0.0, list))) return rc;
-        std::vector<Chunk> chunks;
-        make_chunks(list, options->products, chunks);
-        *bytes = workspace_of(chunks);
+        *bytes = Plan(list, options->products).workspace();
         return FSADAM_OK;
     });
 }
@@ -577,8 +659,7 @@ int fsadam_muon_step(const FsMuonTensor* tensors, int64_t n, int param_type, int
         if ((rc = check_momentum(momentum, scale, scale_dev))) return rc;
         std::vector<Source> list;
         if ((rc = sources_of(tensors, n, size_of(param_type), size_of(grad_type), mixed ? 2 : 0, lr, list))) return rc;
-        std::vector<Chunk> chunks;
-        make_chunks(list, options->products, chunks);
+        const Plan plan(list, options->products);
         Call call{};
         call.step = true;
         call.src_type = grad_type;
@@ -587,7 +668,7 @@ int fsadam_muon_step(const FsMuonTensor* tensors, int64_t n, int param_type, int
         call.options = *options;
         call.momentum = momentum_args(momentum, nesterov, scale, scale_dev);
         call.keep = (float)(1.0 - lr * weight_decay);
-        return run_call(chunks, call, workspace, workspace_bytes, hip_stream);
+        return run_call(plan, call, workspace, workspace_bytes, hip_stream);
     });
 }
 

@@ -23,6 +23,9 @@
 #pragma once
 
 #include <cstdint>
+#include <type_traits>
+
+#include "fsadam_common.h"  // store_through
 
 namespace {
 
@@ -64,12 +67,11 @@ __device__ __forceinline__ float load_as_float(const void* p, int64_t i, int typ
     if (type == kTypeF16) return (float)static_cast<const _Float16*>(p)[i];
     return __builtin_bit_cast(float, (uint32_t)static_cast<const uint16_t*>(p)[i] << 16);
 }
-// Round to nearest even; NaN stays NaN.
-__device__ __forceinline__ uint16_t bf16_bits(float v) {
-    const uint32_t u = __builtin_bit_cast(uint32_t, v);
-    if ((u & 0x7fffffffu) > 0x7f800000u) return (uint16_t)((u >> 16) | 0x40u);
-    return (uint16_t)((u + 0x7fffu + ((u >> 16) & 1u)) >> 16);
-}
+// Round to nearest even; NaN stays NaN (one instruction for two values on this part).
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+typedef float float2_t __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t bf16_pair(float a, float b) { return __builtin_bit_cast(uint32_t, __builtin_convertvector(float2_t{a, b}, bf16x2_t)); }
+__device__ __forceinline__ uint16_t bf16_bits(float v) { return __builtin_bit_cast(uint16_t, (__bf16)v); }
 __device__ __forceinline__ void store_from_float(void* p, int64_t i, int type, float v) {
     if (type == kTypeF32) static_cast<float*>(p)[i] = v;
     else if (type == kTypeF16) static_cast<_Float16*>(p)[i] = (_Float16)v;
@@ -84,6 +86,10 @@ __device__ __forceinline__ float round_to(float v, int type) {
 
 // Eight neighbours p[i .. i + 7], of which the first `left` are there: 16-byte accesses where all are and the address allows it.
 typedef uint32_t words4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t words2_t __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ float high_half(uint32_t w) { return __builtin_bit_cast(float, w & 0xffff0000u); }
+__device__ __forceinline__ float low_half(uint32_t w) { return __builtin_bit_cast(float, w << 16); }
+
 __device__ __forceinline__ void load_eight(const void* p, int64_t i, int type, int left, float (&v)[8]) {
     const char* at = static_cast<const char*>(p) + i * (type == kTypeF32 ? 4 : 2);
     if (left >= 8 && ((uintptr_t)at & 15) == 0) {
@@ -97,7 +103,7 @@ __device__ __forceinline__ void load_eight(const void* p, int64_t i, int type, i
         } else {
             const words4_t w = *reinterpret_cast<const words4_t*>(at);
 #pragma unroll
-            for (int q = 0; q < 8; ++q) v[q] = __builtin_bit_cast(float, q & 1 ? w[q >> 1] & 0xffff0000u : w[q >> 1] << 16);
+            for (int q = 0; q < 8; ++q) v[q] = q & 1 ? high_half(w[q >> 1]) : low_half(w[q >> 1]);
         }
     } else {
 #pragma unroll
@@ -116,15 +122,55 @@ __device__ __forceinline__ void store_eight(void* p, int64_t i, int type, int le
             for (int q = 0; q < 8; ++q) h[q] = (_Float16)v[q];
             *reinterpret_cast<half8_t*>(at) = h;
         } else {
-            words4_t w;
-#pragma unroll
-            for (int q = 0; q < 4; ++q) w[q] = (uint32_t)bf16_bits(v[2 * q]) | (uint32_t)bf16_bits(v[2 * q + 1]) << 16;
-            *reinterpret_cast<words4_t*>(at) = w;
+            *reinterpret_cast<words4_t*>(at) = words4_t{bf16_pair(v[0], v[1]), bf16_pair(v[2], v[3]), bf16_pair(v[4], v[5]), bf16_pair(v[6], v[7])};
         }
     } else {
 #pragma unroll
         for (int q = 0; q < 8; ++q)
             if (q < left) store_from_float(p, i + q, type, v[q]);
+    }
+}
+
+// Four neighbours for passes that stream: the lanes of a wave lie side by side (16 bytes each in fp32, 8 in 16 bits), so that an
+// instruction covers one span; loads do not stay in the caches and stores are written through to memory (store_through).
+// `whole`: all four are there and the addresses allow it.
+template <int TYPE>
+__device__ __forceinline__ void load_four(const void* p, int64_t i, bool whole, int left, float (&v)[4]) {
+    const uintptr_t at = (uintptr_t)p + i * (TYPE == kTypeF32 ? 4 : 2);
+    if (whole) {
+        if constexpr (TYPE == kTypeF32) {
+            const float4_t w = __builtin_nontemporal_load((gptr<const float4_t>)at);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) v[q] = w[q];
+        } else if constexpr (TYPE == kTypeF16) {
+            const half4_t w = __builtin_nontemporal_load((gptr<const half4_t>)at);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) v[q] = (float)w[q];
+        } else {
+            const words2_t w = __builtin_nontemporal_load((gptr<const words2_t>)at);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) v[q] = q & 1 ? high_half(w[q >> 1]) : low_half(w[q >> 1]);
+        }
+    } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[q] = q < left ? load_as_float(p, i + q, TYPE) : 0.0f;
+    }
+}
+template <int TYPE>
+__device__ __forceinline__ void store_four(void* p, int64_t i, bool whole, int left, const float (&v)[4]) {
+    const uintptr_t at = (uintptr_t)p + i * (TYPE == kTypeF32 ? 4 : 2);
+    if (whole) {
+        if constexpr (TYPE == kTypeF32) {
+            store_through((gptr<void>)at, float4_t{v[0], v[1], v[2], v[3]});
+        } else if constexpr (TYPE == kTypeF16) {
+            store_through((gptr<void>)at, half4_t{(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]});
+        } else {
+            store_through((gptr<void>)at, words2_t{bf16_pair(v[0], v[1]), bf16_pair(v[2], v[3])});
+        }
+    } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            if (q < left) store_from_float(p, i + q, TYPE, v[q]);
     }
 }
 
@@ -189,19 +235,31 @@ struct MomentumArgs {
     int nesterov;
 };
 
+// The divisor of the gradients.  A power of two with a normal reciprocal is multiplied by that: the same bits, and a
+// division takes ten instructions that a pass over 16-bit gradients has no time for.
+struct Divisor {
+    float scale, inverse;
+    bool exact;
+    __device__ __forceinline__ explicit Divisor(const MomentumArgs& k) {
+        scale = k.scale_dev ? *k.scale_dev : k.scale;
+        inverse = 1.0f / scale;
+        exact = (__builtin_bit_cast(uint32_t, scale) & 0x7fffffu) == 0 && __builtin_isnormal(scale) && __builtin_isnormal(inverse);
+    }
+    __device__ __forceinline__ float operator()(float g) const { return exact ? g * inverse : g / scale; }
+};
+
 //     r = g / scale;   m <- m + (1 - mu) (r - m);   u = nesterov ? r + mu (m - r) : m
-__device__ __forceinline__ float momentum_update(float g, float& m, float scale, const MomentumArgs& k) {
-    const float r = g / scale;
+__device__ __forceinline__ float momentum_update(float r, float& m, const MomentumArgs& k) {
     m = m + (r - m) * k.one_minus;
     return k.nesterov ? r + (m - r) * k.momentum : m;
 }
-__device__ __forceinline__ float update_again(float g, float m, float scale, const MomentumArgs& k) {  // from the stored m
-    const float r = g / scale;
+__device__ __forceinline__ float update_again(float r, float m, const MomentumArgs& k) {  // from the stored m
     return k.nesterov ? r + (m - r) * k.momentum : m;
 }
 
 constexpr int kChunkThreads = 256;
 constexpr int kChunkElems = 8192;  // elements of one partial sum
+constexpr int kMomentumElems = 1024;  // likewise, of the momentum pass: four to a thread (8 and 16 are 4 and 12 % slower)
 
 // Sum over a workgroup of 256 in a fixed order; the result is valid in thread 0.
 __device__ __forceinline__ double block_sum(double v) {
@@ -233,6 +291,23 @@ struct alignas(16) MomentumRow {
     int64_t numel;
     int64_t first;    // chunks of the rows before this one
 };
+// Short tables travel in the arguments of the launches that use them, longer ones in those of launches that write them to
+// memory first: nothing is copied from the host, and a captured graph holds all of it.
+constexpr int kMomentumRowsPerLaunch = 64;
+struct MomentumRows {
+    MomentumRow row[kMomentumRowsPerLaunch];
+};
+// What a kernel takes: the address of a table, or the table.
+struct InMemory {
+    const MomentumRow* row;
+    int n;
+};
+struct InArguments {
+    MomentumRows rows;
+    int n;
+};
+__device__ __forceinline__ const MomentumRow* rows_of(const InMemory& t) { return t.row; }
+__device__ __forceinline__ const MomentumRow* rows_of(const InArguments& t) { return t.rows.row; }
 
 // Elements `begin` to `end` of a line, eight to a thread: calls each(first element, how many) for every piece.  With whole eights
 // all pieces of a thread are independent, so that their loads are all in flight before the first is used.
@@ -247,8 +322,10 @@ __device__ __forceinline__ void for_eights(int64_t begin, int64_t end, Each&& ea
 }
 
 // Bound by HBM: 2 + 4 bytes read and 2 + 4 written per element with 16-bit gradients and updates.
-template <int GT, int UT>
-__global__ __launch_bounds__(kChunkThreads) void fsadam_momentum_chunks(const MomentumRow* table, int n_rows, MomentumArgs k, double* partials) {
+template <int GT, int UT, typename Table>
+__global__ __launch_bounds__(kChunkThreads) void fsadam_momentum_chunks(Table tables, MomentumArgs k, double* partials) {
+    const MomentumRow* table = rows_of(tables);
+    const int n_rows = tables.n;
     int low = 0, high = n_rows - 1;
     const int64_t t = blockIdx.x;
     while (low < high) {
@@ -257,33 +334,67 @@ __global__ __launch_bounds__(kChunkThreads) void fsadam_momentum_chunks(const Mo
         else high = mid - 1;
     }
     const MomentumRow& row = table[low];
-    const int64_t begin = (t - row.first) * kChunkElems;
-    const int64_t end = begin + kChunkElems < row.numel ? begin + kChunkElems : row.numel;
-    const float scale = k.scale_dev ? *k.scale_dev : k.scale;
+    const int64_t begin = (t - row.first) * kMomentumElems;
+    const int64_t end = begin + kMomentumElems < row.numel ? begin + kMomentumElems : row.numel;
+    const Divisor by(k);
     double sum = 0.0;
-    for_eights(begin, end, [&](int64_t i, int n) {
-        float g[8], m[8], u[8];
-        load_eight(row.g, i, GT, n, g);
-        load_eight(row.m, i, kTypeF32, n, m);
+    constexpr int kPieces = kMomentumElems / 4 / kChunkThreads;
+    float g[kPieces][4], m[kPieces][4], u[kPieces][4];
+    const uintptr_t any = (uintptr_t)row.g * (GT == kTypeF32 ? 1 : 2) | (uintptr_t)row.m | (uintptr_t)row.u * (UT == kTypeF32 ? 1 : 2);
+    const bool whole = end - begin == kMomentumElems && (any & 15) == 0;
+    const int64_t i0 = begin + threadIdx.x * 4;
+    constexpr int kStep = kChunkThreads * 4;
+    auto left = [&](int n) { const int64_t here = end - (i0 + n * kStep); return here < 4 ? (int)here : 4; };
+    auto load = [&](bool whole) {
 #pragma unroll
-        for (int q = 0; q < 8; ++q) u[q] = momentum_update(g[q], m[q], scale, k);
-        store_eight(row.m, i, kTypeF32, n, m);
-        store_eight(row.u, i, UT, n, u);
-#pragma unroll
-        for (int q = 0; q < 8; ++q) {
-            const double r = q < n ? (double)round_to(u[q], UT) : 0.0;
-            sum += r * r;
+        for (int n = 0; n < kPieces; ++n) {
+            load_four<GT>(row.g, i0 + n * kStep, whole, left(n), g[n]);
+            load_four<kTypeF32>(row.m, i0 + n * kStep, whole, left(n), m[n]);
         }
-    });
+    };
+    if (whole) load(true);
+    else load(false);
+    if (by.exact) {
+#pragma unroll
+        for (int n = 0; n < kPieces; ++n)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) g[n][q] *= by.inverse;
+    } else {
+#pragma unroll
+        for (int n = 0; n < kPieces; ++n)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) g[n][q] /= by.scale;
+    }
+#pragma unroll
+    for (int n = 0; n < kPieces; ++n)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) u[n][q] = momentum_update(g[n][q], m[n][q], k);
+    auto store = [&](bool whole) {
+#pragma unroll
+        for (int n = 0; n < kPieces; ++n) {
+            store_four<kTypeF32>(row.m, i0 + n * kStep, whole, left(n), m[n]);
+            store_four<UT>(row.u, i0 + n * kStep, whole, left(n), u[n]);
+        }
+    };
+    if (whole) store(true);
+    else store(false);
+#pragma unroll
+    for (int n = 0; n < kPieces; ++n)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {  // elements past the end are zeros: g and m were loaded as such
+            const double r = (double)round_to(u[n][q], UT);
+            sum = __builtin_fma(r, r, sum);
+        }
     sum = block_sum(sum);
     if (threadIdx.x == 0) partials[t] = sum;
 }
 
 // norms[row] = sqrt of the row's sum of squares; found_inf is raised where that is not finite (a double holds the sum of
 // squares of any floats, so it is not finite exactly where an update is not).
-__global__ __launch_bounds__(kChunkThreads) void fsadam_momentum_norms(const MomentumRow* table, const double* partials, float* norms, float* found_inf) {
-    const MomentumRow& row = table[blockIdx.x];
-    const int64_t n = (row.numel + kChunkElems - 1) / kChunkElems;
+template <typename Table>
+__global__ __launch_bounds__(kChunkThreads) void fsadam_momentum_norms(Table tables, const double* partials, float* norms, float* found_inf) {
+    const MomentumRow& row = rows_of(tables)[blockIdx.x];
+    const int64_t n = (row.numel + kMomentumElems - 1) / kMomentumElems;
     const double sum = block_sum(sum_of(partials + row.first, n));
     if (threadIdx.x == 0) {
         if (norms) norms[blockIdx.x] = (float)sqrt(sum);
@@ -304,7 +415,7 @@ __global__ __launch_bounds__(kChunkThreads) void fsadam_matrix_chunks(const Matr
     const int64_t end = begin + kChunkElems < numel ? begin + kChunkElems : numel;
     double sum = 0.0;
     if constexpr (STEP) {
-        const float scale = k.scale_dev ? *k.scale_dev : k.scale;
+        const Divisor by(k);
         const int64_t base = (int64_t)matrix * numel;
         for_eights(begin, end, [&](int64_t i, int n) {
             float g[8], m[8];
@@ -312,8 +423,8 @@ __global__ __launch_bounds__(kChunkThreads) void fsadam_matrix_chunks(const Matr
             load_eight(row.buf, base + i, kTypeF32, n, m);
 #pragma unroll
             for (int q = 0; q < 8; ++q) {
-                const double u = q < n ? (double)momentum_update(g[q], m[q], scale, k) : 0.0;
-                sum += u * u;
+                const double u = q < n ? (double)momentum_update(by(g[q]), m[q], k) : 0.0;
+                sum = __builtin_fma(u, u, sum);
             }
             store_eight(row.buf, base + i, kTypeF32, n, m);
         });
@@ -323,7 +434,7 @@ __global__ __launch_bounds__(kChunkThreads) void fsadam_matrix_chunks(const Matr
             float v[8];
             load_eight(row.src, base + i, ST, n, v);
 #pragma unroll
-            for (int q = 0; q < 8; ++q) sum += q < n ? (double)v[q] * (double)v[q] : 0.0;
+            for (int q = 0; q < 8; ++q) sum = __builtin_fma((double)v[q], (double)v[q], sum);  // what is not there was loaded as 0
         });
     } else {
         const int64_t base = (int64_t)matrix * row.src_stride;
@@ -366,7 +477,7 @@ __global__ __launch_bounds__(256) void fsadam_matrix_normalise(const MatrixRow* 
     const int i0 = (int)(t / across) * 64, j0 = (int)(t % across) * 64;  // in X
     const int r0 = row.tall ? j0 : i0, c0 = row.tall ? i0 : j0;         // in the source
     const double factor = inverse[row.first_matrix + matrix] * power;
-    const float scale = STEP ? (k.scale_dev ? *k.scale_dev : k.scale) : 1.0f;
+    const Divisor by(k);
     const int64_t plane = (int64_t)row.s64 * row.l64;
     _Float16* x = work + row.x_off[0] + (int64_t)matrix * 2 * plane;
     auto put = [&](int i, int j, const float (&v)[8]) { store_planes<2>(x + (int64_t)(i0 + i) * row.l64 + j0 + j, plane, v); };
@@ -384,7 +495,7 @@ __global__ __launch_bounds__(256) void fsadam_matrix_normalise(const MatrixRow* 
                 load_eight(row.src, at, ST, left, v);
                 load_eight(row.buf, at, kTypeF32, left, m);
 #pragma unroll
-                for (int q = 0; q < 8; ++q) v[q] = q < left ? update_again(v[q], m[q], scale, k) : 0.0f;
+                for (int q = 0; q < 8; ++q) v[q] = q < left ? update_again(by(v[q]), m[q], k) : 0.0f;
             } else {
                 load_eight(row.src, (int64_t)matrix * row.src_stride + (int64_t)(r0 + r) * row.src_ld + c0 + c, ST, left, v);
             }
@@ -803,6 +914,264 @@ __global__ __launch_bounds__(64 * WM * WN) void fsadam_matrix_stage(const Matrix
     }
 }
 
+// ---- matrices that fit a compute unit's LDS -----------------------------------------------------------------------
+
+// One workgroup takes a matrix from the source to the result: X (two planes) and one square matrix stay in LDS, products
+// go through registers, nothing is written to memory in between.  All the launches and the trips to the L2 and back
+// that the stages above are made of are what such a matrix would wait for.
+struct alignas(16) ResidentRow {
+    const void* src;
+    float* buf;
+    void* dst;
+    void* copy;
+    int64_t src_ld, src_stride, dst_ld, dst_stride;
+    int32_t rows, cols;
+    int32_t first_matrix;
+    float step_ratio;
+};
+constexpr int kResidentRowsPerLaunch = 24;
+struct ResidentRows {
+    ResidentRow row[kResidentRowsPerLaunch];
+};
+struct ResidentInMemory {
+    const ResidentRow* row;
+    int n;
+};
+struct ResidentInArguments {
+    ResidentRows rows;
+    int n;
+};
+__device__ __forceinline__ const ResidentRow* rows_of(const ResidentInMemory& t) { return t.row; }
+__device__ __forceinline__ const ResidentRow* rows_of(const ResidentInArguments& t) { return t.rows.row; }
+constexpr int kMaxSteps = 32;
+struct ResidentArgs {
+    int steps, src_type, dst_type, copy_type;
+    float keep;
+    double eps, power;  // of the norm; 2^x of X0
+    float gram[kMaxSteps], linear_b[kMaxSteps], product_b[kMaxSteps], linear_x[kMaxSteps], product_x[kMaxSteps];
+};
+
+// Storage in LDS: sides padded to 32 (the depth of a matrix instruction), rows 8 halves longer than that, which spreads the 16
+// rows a fragment is read from over the banks.
+constexpr int kResidentThreads = 512, kResidentWaves = kResidentThreads / 64;
+constexpr int kResidentElems = 38912;  // of X and the square matrix, rows' ends included: 4 bytes each in 152 of the 160 KiB
+constexpr int kResidentSide = 128;
+constexpr int kResidentSquareTiles = 5;   // 16 x 16 tiles of a wave: 36 under the diagonal of 128
+__host__ __device__ constexpr int resident_pitch(int side) { return (side + 31) / 32 * 32 + 8; }
+__host__ __device__ constexpr bool resident_fits(int64_t s, int64_t l) {
+    return s <= kResidentSide && l <= kResidentElems && (s + 31) / 32 * 32 * (resident_pitch((int)l) + resident_pitch((int)s)) <= kResidentElems;
+}
+
+template <bool STEP, typename Table>
+__global__ __launch_bounds__(kResidentThreads) void fsadam_matrix_resident(Table tables, ResidentArgs k, MomentumArgs mk) {
+    extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
+    __shared__ double part[kResidentWaves];
+    const ResidentRow* table = rows_of(tables);
+    int low = 0, high = tables.n - 1;
+    while (low < high) {
+        const int mid = (low + high + 1) >> 1;
+        if (table[mid].first_matrix <= (int)blockIdx.x) low = mid;
+        else high = mid - 1;
+    }
+    const ResidentRow& row = table[low];
+    const int64_t matrix = (int)blockIdx.x - row.first_matrix;
+    const int rows = row.rows, cols = row.cols;
+    const bool tall = rows > cols;
+    const int s = tall ? cols : rows, l = tall ? rows : cols;
+    const int sp = (s + 31) / 32 * 32, lp = (l + 31) / 32 * 32, pitch_x = lp + 8, pitch_a = sp + 8;
+    const int plane_x = sp * pitch_x, plane_a = sp * pitch_a;  // halves
+    _Float16* x = reinterpret_cast<_Float16*>(lds);
+    _Float16* a = x + 2 * plane_x;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int g = lane >> 4, c = lane & 15;
+
+    // the padding is zero and stays zero
+    for (int e = tid; e < 2 * plane_x / 8; e += kResidentThreads) *reinterpret_cast<half8_t*>(x + e * 8) = half8_t{};
+    // element e of the matrix, row-major as in the source
+    const int numel = rows * cols;
+    const float per_row = 1.0f / (float)cols;
+    auto place = [&](int e, int& r, int& q) {  // e < 2^17, so half a column is far more than the rounding of the product
+        r = (int)(((float)e + 0.5f) * per_row);
+        q = e - r * cols;
+    };
+    const Divisor by(mk);
+    const int64_t base = matrix * row.src_stride, flat = matrix * numel;
+    constexpr int kBatch = 8;  // loads in flight
+    double sum = 0.0;
+    for (int e0 = tid; e0 < numel; e0 += kResidentThreads * kBatch) {
+        float v[kBatch], m[kBatch];
+#pragma unroll
+        for (int n = 0; n < kBatch; ++n) {
+            const int e = e0 + n * kResidentThreads;
+            v[n] = m[n] = 0.0f;
+            if (e < numel) {
+                if constexpr (STEP) {
+                    v[n] = load_as_float(row.src, flat + e, k.src_type);
+                    m[n] = row.buf[flat + e];
+                } else {
+                    int r, q;
+                    place(e, r, q);
+                    v[n] = load_as_float(row.src, base + r * row.src_ld + q, k.src_type);
+                }
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < kBatch; ++n) {
+            const int e = e0 + n * kResidentThreads;
+            if constexpr (STEP) {
+                v[n] = momentum_update(by(v[n]), m[n], mk);
+                if (e < numel) row.buf[flat + e] = m[n];
+            }
+            sum = __builtin_fma((double)v[n], (double)v[n], sum);
+        }
+    }
+    for (int d = 32; d > 0; d >>= 1) sum += __shfl_down(sum, d);
+    if (lane == 0) part[wave] = sum;
+    __syncthreads();
+    sum = 0.0;
+#pragma unroll
+    for (int n = 0; n < kResidentWaves; ++n) sum += part[n];
+    const double norm = sqrt(sum);
+    const double factor = __builtin_isfinite(sum) ? k.power / (norm > k.eps ? norm : k.eps) : __builtin_nan("");
+    for (int e0 = tid; e0 < numel; e0 += kResidentThreads * kBatch) {
+        float v[kBatch], m[kBatch];
+        int r[kBatch], q[kBatch];
+#pragma unroll
+        for (int n = 0; n < kBatch; ++n) {
+            const int e = e0 + n * kResidentThreads;
+            place(e, r[n], q[n]);
+            if (e < numel) {
+                if constexpr (STEP) {
+                    v[n] = load_as_float(row.src, flat + e, k.src_type);
+                    m[n] = row.buf[flat + e];
+                } else {
+                    v[n] = load_as_float(row.src, base + r[n] * row.src_ld + q[n], k.src_type);
+                }
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < kBatch; ++n) {
+            if (e0 + n * kResidentThreads >= numel) continue;
+            const float u = STEP ? update_again(by(v[n]), m[n], mk) : v[n];
+            const int at = tall ? q[n] * pitch_x + r[n] : r[n] * pitch_x + q[n];
+            split_halves((float)((double)u * factor), x[at], x[plane_x + at]);
+        }
+    }
+    __syncthreads();
+
+    auto fragment = [&](const _Float16* p, int pitch) { return *reinterpret_cast<const half8_t*>(p + c * pitch + g * 8); };  // 16 rows, 32 deep
+    auto turned = [&](const _Float16* q, int pitch) {  // 32 deep, 16 columns
+        const _Float16* at = q + (8 * g + (c >> 2)) * pitch + (c & 3) * 4;
+        const short4_t first = __builtin_amdgcn_ds_read_tr16_b64_v4i16((FM_LDS short4_t*)at);
+        const short4_t second = __builtin_amdgcn_ds_read_tr16_b64_v4i16((FM_LDS short4_t*)(at + 4 * pitch));
+        return __builtin_shufflevector(__builtin_bit_cast(half4_t, first), __builtin_bit_cast(half4_t, second), 0, 1, 2, 3, 4, 5, 6, 7);
+    };
+    // A 16 x 16 tile of M M^T, M of two planes: rows from `p` and from `q` on.
+    auto product = [&](const _Float16* p, const _Float16* q, int pitch, int plane, int depth) {
+        float4_t high = {0.0f, 0.0f, 0.0f, 0.0f}, cross = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int d = 0; d < depth; d += 32) {
+            const half8_t p0 = fragment(p + d, pitch), p1 = fragment(p + plane + d, pitch), q0 = fragment(q + d, pitch), q1 = fragment(q + plane + d, pitch);
+            cross = __builtin_amdgcn_mfma_f32_16x16x32_f16(p1, q0, cross, 0, 0, 0);
+            cross = __builtin_amdgcn_mfma_f32_16x16x32_f16(p0, q1, cross, 0, 0, 0);
+            high = __builtin_amdgcn_mfma_f32_16x16x32_f16(p0, q0, high, 0, 0, 0);
+        }
+        return high + cross;
+    };
+    const int side = sp / 16, n_square = side * (side + 1) / 2, along = lp / 16;
+    auto triangle = [&](int t, int& ti, int& tj) {
+        ti = 0;
+        while ((ti + 1) * (ti + 2) / 2 <= t) ++ti;
+        tj = t - ti * (ti + 1) / 2;
+    };
+    // lane (g, c) holds rows 4 g .. 4 g + 3 of column c of a tile
+    auto put_square = [&](int ti, int tj, const float4_t& v) {  // the lower triangle and its mirror image
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int i = ti * 16 + 4 * g + r, j = tj * 16 + c;
+            if (j > i) continue;
+            _Float16 hi, lo;
+            split_halves(v[r], hi, lo);
+            a[i * pitch_a + j] = a[j * pitch_a + i] = hi;
+            a[plane_a + i * pitch_a + j] = a[plane_a + j * pitch_a + i] = lo;
+        }
+    };
+    for (int step = 0; step < k.steps; ++step) {
+        for (int n = 0; n < kResidentSquareTiles; ++n) {
+            const int t = wave + n * kResidentWaves;
+            if (t >= n_square) break;
+            int ti, tj;
+            triangle(t, ti, tj);
+            put_square(ti, tj, product(x + ti * 16 * pitch_x, x + tj * 16 * pitch_x, pitch_x, plane_x, lp) * k.gram[step]);
+        }
+        __syncthreads();
+        float4_t b[kResidentSquareTiles];
+#pragma unroll
+        for (int n = 0; n < kResidentSquareTiles; ++n) {
+            const int t = wave + n * kResidentWaves;
+            if (t >= n_square) continue;
+            int ti, tj;
+            triangle(t, ti, tj);
+            b[n] = product(a + ti * 16 * pitch_a, a + tj * 16 * pitch_a, pitch_a, plane_a, sp) * k.product_b[step];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int at = (ti * 16 + 4 * g + r) * pitch_a + tj * 16 + c;
+                b[n][r] += k.linear_b[step] * ((float)a[at] + (float)a[plane_a + at]);
+            }
+        }
+        __syncthreads();  // A has been read: B takes its place
+#pragma unroll
+        for (int n = 0; n < kResidentSquareTiles; ++n) {
+            const int t = wave + n * kResidentWaves;
+            if (t >= n_square) continue;
+            int ti, tj;
+            triangle(t, ti, tj);
+            put_square(ti, tj, b[n]);
+        }
+        __syncthreads();
+        // A wave takes whole columns of tiles: what it overwrites, it alone has read.
+        const bool last = step + 1 == k.steps;
+        for (int tj = wave; tj < along; tj += kResidentWaves) {
+            float4_t next[kResidentSide / 16];
+#pragma unroll
+            for (int ti = 0; ti < kResidentSide / 16; ++ti) next[ti] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int d = 0; d < sp; d += 32) {
+                const half8_t q0 = turned(x + d * pitch_x + tj * 16, pitch_x), q1 = turned(x + plane_x + d * pitch_x + tj * 16, pitch_x);
+#pragma unroll
+                for (int ti = 0; ti < kResidentSide / 16; ++ti) {
+                    if (ti >= side) break;
+                    const half8_t p0 = fragment(a + ti * 16 * pitch_a + d, pitch_a), p1 = fragment(a + plane_a + ti * 16 * pitch_a + d, pitch_a);
+                    next[ti] = __builtin_amdgcn_mfma_f32_16x16x32_f16(p1, q0, next[ti], 0, 0, 0);
+                    next[ti] = __builtin_amdgcn_mfma_f32_16x16x32_f16(p0, q1, next[ti], 0, 0, 0);
+                    next[ti] = __builtin_amdgcn_mfma_f32_16x16x32_f16(p0, q0, next[ti], 0, 0, 0);
+                }
+            }
+#pragma unroll
+            for (int ti = 0; ti < kResidentSide / 16; ++ti) {
+                if (ti >= side) break;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int i = ti * 16 + 4 * g + r, j = tj * 16 + c, at = i * pitch_x + j;
+                    const float o = k.linear_x[step] * ((float)x[at] + (float)x[plane_x + at]) + k.product_x[step] * next[ti][r];
+                    if (!last) {
+                        split_halves(o, x[at], x[plane_x + at]);
+                    } else if (i < s && j < l) {
+                        const int64_t to_row = tall ? j : i, to_col = tall ? i : j;
+                        if constexpr (STEP) {
+                            const int64_t to = flat + to_row * cols + to_col;
+                            const float p = load_as_float(row.dst, to, k.dst_type) * k.keep - row.step_ratio * o;
+                            store_from_float(row.dst, to, k.dst_type, p);
+                            if (k.copy_type >= 0) store_from_float(row.copy, to, k.copy_type, p);
+                        } else {
+                            store_from_float(row.dst, matrix * row.dst_stride + to_row * row.dst_ld + to_col, k.dst_type, o);
+                        }
+                    }
+                }
+            }
+        }
+        __syncthreads();
+    }
+}
+
 // Rows of a call's table, in the arguments of the launch: nothing is allocated or copied, and a captured graph holds them.
 constexpr int kRowsPerPut = 16;
 struct MatrixRows {
@@ -813,10 +1182,10 @@ __global__ void fsadam_put_matrix_rows(MatrixRow* table, int n, MatrixRows rows)
     typedef uint32_t word_t __attribute__((ext_vector_type(4)));
     for (int e = threadIdx.x; e < n * kWords; e += blockDim.x) reinterpret_cast<word_t*>(table)[e] = reinterpret_cast<const word_t*>(rows.row)[e];
 }
-constexpr int kMomentumRowsPerPut = 64;
-struct MomentumRows {
-    MomentumRow row[kMomentumRowsPerPut];
-};
+__global__ void fsadam_put_resident_rows(ResidentRow* table, int n, ResidentRows rows) {
+    constexpr int kWords = sizeof(ResidentRow) / 16;
+    for (int e = threadIdx.x; e < n * kWords; e += blockDim.x) reinterpret_cast<words4_t*>(table)[e] = reinterpret_cast<const words4_t*>(rows.row)[e];
+}
 __global__ void fsadam_put_momentum_rows(MomentumRow* table, int n, MomentumRows rows) {
     constexpr int kWords = sizeof(MomentumRow) / 16;
     typedef uint32_t word_t __attribute__((ext_vector_type(4)));

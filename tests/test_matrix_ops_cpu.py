@@ -40,11 +40,11 @@ def up(v, m):
 
 
 @pytest.mark.parametrize("products", [1, 2])
-def test_workspace_holds_two_x_and_two_square_matrices_per_matrix(products):
+def test_workspace_holds_two_x_and_the_square_matrices_of_every_matrix(products):
     rc, got = workspace(matrices((3, 300, 170), (1, 135, 200)), options(products=products))
     assert rc == 0
     x = lambda s, l: 2 * 2 * up(s, 64) * up(l, 64) * 2  # two buffers of two planes of halves
-    a = lambda s: 2 * products * up(s, 64) ** 2 * 2
+    a = lambda s: (3 if products == 2 else 2) * products * up(s, 64) ** 2 * 2  # 22 bits: two planes, and steps in pairs need a third matrix
     body = 3 * (x(170, 300) + a(170)) + x(135, 200) + a(135)
     assert body < got < body + 4096  # and the tables
 
@@ -106,7 +106,7 @@ def test_bad_strides_alignment_and_workspaces_are_refused():
     rows = matrices((1, 4, 4), src=FAKE, dst=FAKE)
     rows[0].dst_ld = 8
     assert L.fsadam_orthogonalize(rows, 1, 0, ctypes.byref(opt), FAKE, 1 << 20, None) == -1 and b"same strides" in L.fsadam_last_error()
-    rows = matrices((1, 4, 4))
+    rows = matrices((1, 200, 200))
     size = workspace(rows, opt)[1]
     assert L.fsadam_orthogonalize(rows, 1, 0, ctypes.byref(opt), None, size, None) == -1 and b"workspace" in L.fsadam_last_error()
     assert L.fsadam_orthogonalize(rows, 1, 0, ctypes.byref(opt), FAKE, size - 1, None) == -1 and b"workspace" in L.fsadam_last_error()
@@ -132,7 +132,7 @@ def muon_rows(**change):
     dict(scale=0.0), dict(scale=math.inf), dict(scale=math.nan),
     dict(rows=muon_rows(p=0)), dict(rows=muon_rows(g=0)), dict(rows=muon_rows(m=0)), dict(rows=muon_rows(p_copy=0), types=(0, 1, 1)),
     dict(rows=muon_rows(m=FAKE + 2)), dict(rows=muon_rows(p=FAKE + 2)), dict(rows=muon_rows(ratio=math.nan)), dict(rows=muon_rows(rows=-1)),
-    dict(bytes=100),
+    dict(rows=muon_rows(rows=200, cols=200), bytes=100),
 ])
 def test_bad_steps_are_refused(call):
     opt = options()
@@ -278,3 +278,13 @@ def test_oracle_agrees_with_singular_values():
     for _ in range(5):
         s = a * s + b * s**3 + c * s**5
     assert M.relative(M.orthogonal(u), x @ torch.diag_embed(s) @ y) < 1e-12
+
+
+def test_workspace_of_matrices_that_fit_a_compute_unit():
+    """They keep everything in LDS; only a long list's table needs memory."""
+    assert workspace(matrices((1, 64, 256)), options()) == (0, 0)
+    assert workspace(matrices((100, 128, 128), (7, 1, 64)), options()) == (0, 0)
+    rc, got = workspace(matrices(*[(1, 96, 96)] * 25), options())
+    assert rc == 0 and 0 < got < 8192
+    assert workspace(matrices((1, 129, 129)), options())[1] > 0
+    assert workspace(matrices((1, 64, 4096)), options())[1] > 0
