@@ -234,7 +234,7 @@ void make_chunks(const std::vector<Source>& all, int asked, std::vector<Chunk>& 
   }
 }
 
-// The rows of the list that fit LDS.
+// The rows of the list that fit LDS, of one padded short side.
 struct Residents {
     std::vector<ResidentRow> rows;
     int64_t matrices = 0;
@@ -243,26 +243,28 @@ struct Residents {
 };
 
 struct Plan {
-    Residents residents;
+    Residents residents[kResidentSide / 32];  // by sides of 32, 64, 96, 128
     std::vector<Chunk> chunks;
     Plan(const std::vector<Source>& list, int products) {
         for (const Source& in : list) {
             if (!resident(in)) continue;
+            const int s = (int)std::min(in.rows, in.cols), l = (int)std::max(in.rows, in.cols);
+            Residents& kind = residents[(s - 1) / 32];
             ResidentRow row{};
             row.src = in.src; row.buf = in.buf; row.dst = in.dst; row.copy = in.copy;
             row.src_ld = in.src_ld; row.src_stride = in.src_stride; row.dst_ld = in.dst_ld; row.dst_stride = in.dst_stride;
             row.rows = (int32_t)in.rows; row.cols = (int32_t)in.cols;
-            row.first_matrix = (int32_t)residents.matrices;
+            row.first_matrix = (int32_t)kind.matrices;
             row.step_ratio = in.step_ratio;
-            residents.rows.push_back(row);
-            residents.matrices += in.batch;
-            const int s = std::min(row.rows, row.cols), l = std::max(row.rows, row.cols);
-            residents.lds_bytes = std::max(residents.lds_bytes, (int)up(s, 32) * (resident_pitch(s) + resident_pitch(l)) * 4);
+            kind.rows.push_back(row);
+            kind.matrices += in.batch;
+            kind.lds_bytes = std::max(kind.lds_bytes, (int)up(s, 32) * (resident_pitch(s) + resident_pitch(l)) * 4);
         }
         make_chunks(list, products, chunks);
     }
     int64_t workspace() const {
-        int64_t bytes = residents.bytes();  // the residents' table comes first and is done with when the chunks begin
+        int64_t bytes = 0;  // each part is done with the workspace when the next begins
+        for (const Residents& r : residents) bytes = std::max(bytes, r.bytes());
         for (const Chunk& c : chunks) bytes = std::max(bytes, c.bytes());
         return bytes;
     }
@@ -407,7 +409,9 @@ int run_chunk(const Chunk& c, const Call& call, void* workspace, hipStream_t str
     return FSADAM_OK;
 }
 
+template <int SIDE>
 int run_residents(const Residents& r, const Call& call, void* workspace, hipStream_t stream) {
+    if (r.rows.empty()) return FSADAM_OK;
     if (r.matrices > kMaxTiles) return fail(FSADAM_EINVAL, "the list has too many matrices for one call");
     const FsOrthOptions& o = call.options;
     ResidentArgs k{};
@@ -419,17 +423,17 @@ int run_residents(const Residents& r, const Call& call, void* workspace, hipStre
     for (int s = 0; s < o.steps; ++s) {
         const StepNumbers& n = call.numbers[s];
         const int next_x = s + 1 < o.steps ? call.numbers[s + 1].x : 0;
-        k.gram[s] = (float)std::ldexp(1.0, n.a - 2 * n.x);
-        k.linear_b[s] = (float)std::ldexp((double)o.b, n.b - n.a);
-        k.product_b[s] = (float)std::ldexp((double)o.c, n.b - 2 * n.a);
-        k.linear_x[s] = (float)std::ldexp((double)o.a, next_x - n.x);
-        k.product_x[s] = (float)std::ldexp(1.0, next_x - n.b - n.x);
+        k.factors[kFactorGram][s] = (float)std::ldexp(1.0, n.a - 2 * n.x);
+        k.factors[kFactorLinearB][s] = (float)std::ldexp((double)o.b, n.b - n.a);
+        k.factors[kFactorProductB][s] = (float)std::ldexp((double)o.c, n.b - 2 * n.a);
+        k.factors[kFactorLinearX][s] = (float)std::ldexp((double)o.a, next_x - n.x);
+        k.factors[kFactorProductX][s] = (float)std::ldexp(1.0, next_x - n.b - n.x);
     }
     auto launch = [&](const auto& table) {
         using Table = std::decay_t<decltype(table)>;
         const dim3 grid((uint32_t)r.matrices), block(kResidentThreads);
-        if (call.step) hipLaunchKernelGGL((fsadam_matrix_resident<true, Table>), grid, block, r.lds_bytes, stream, table, k, call.momentum);
-        else hipLaunchKernelGGL((fsadam_matrix_resident<false, Table>), grid, block, r.lds_bytes, stream, table, k, call.momentum);
+        if (call.step) hipLaunchKernelGGL((fsadam_matrix_resident<SIDE, true, Table>), grid, block, r.lds_bytes, stream, table, k, call.momentum);
+        else hipLaunchKernelGGL((fsadam_matrix_resident<SIDE, false, Table>), grid, block, r.lds_bytes, stream, table, k, call.momentum);
         return launched();
     };
     if (r.rows.size() <= kResidentRowsPerLaunch) {
@@ -456,9 +460,13 @@ int run_call(const Plan& plan, Call& call, void* workspace, int64_t workspace_by
     if (need && (!workspace || !aligned(workspace, 256))) return fail(FSADAM_EINVAL, "the workspace must be a device pointer aligned to 256 bytes");
     if (workspace_bytes < need)
         return fail(FSADAM_EINVAL, "the workspace holds " + std::to_string(workspace_bytes) + " bytes, this list needs " + std::to_string(need));
-    if (!plan.residents.rows.empty() && (rc = run_residents(plan.residents, call, workspace, static_cast<hipStream_t>(hip_stream)))) return rc;
+    hipStream_t stream = static_cast<hipStream_t>(hip_stream);
+    if ((rc = run_residents<2>(plan.residents[0], call, workspace, stream))) return rc;
+    if ((rc = run_residents<4>(plan.residents[1], call, workspace, stream))) return rc;
+    if ((rc = run_residents<6>(plan.residents[2], call, workspace, stream))) return rc;
+    if ((rc = run_residents<8>(plan.residents[3], call, workspace, stream))) return rc;
     for (const Chunk& c : chunks) {
-        rc = run_chunk(c, call, workspace, static_cast<hipStream_t>(hip_stream));
+        rc = run_chunk(c, call, workspace, stream);
         if (rc) return rc;
     }
     return FSADAM_OK;

@@ -944,25 +944,28 @@ struct ResidentInArguments {
 __device__ __forceinline__ const ResidentRow* rows_of(const ResidentInMemory& t) { return t.row; }
 __device__ __forceinline__ const ResidentRow* rows_of(const ResidentInArguments& t) { return t.rows.row; }
 constexpr int kMaxSteps = 32;
+enum { kFactorGram, kFactorLinearB, kFactorProductB, kFactorLinearX, kFactorProductX };
 struct ResidentArgs {
     int steps, src_type, dst_type, copy_type;
     float keep;
     double eps, power;  // of the norm; 2^x of X0
-    float gram[kMaxSteps], linear_b[kMaxSteps], product_b[kMaxSteps], linear_x[kMaxSteps], product_x[kMaxSteps];
+    float factors[5][kMaxSteps];  // [kFactor...][step]
 };
 
 // Storage in LDS: sides padded to 32 (the depth of a matrix instruction), rows 8 halves longer than that, which spreads the 16
 // rows a fragment is read from over the banks.
-constexpr int kResidentThreads = 512, kResidentWaves = kResidentThreads / 64;
+constexpr int kResidentThreads = 1024, kResidentWaves = kResidentThreads / 64;
 constexpr int kResidentElems = 38912;  // of X and the square matrix, rows' ends included: 4 bytes each in 152 of the 160 KiB
 constexpr int kResidentSide = 128;
-constexpr int kResidentSquareTiles = 5;   // 16 x 16 tiles of a wave: 36 under the diagonal of 128
+constexpr int kResidentBatch = 16;        // elements of a thread in registers
 __host__ __device__ constexpr int resident_pitch(int side) { return (side + 31) / 32 * 32 + 8; }
 __host__ __device__ constexpr bool resident_fits(int64_t s, int64_t l) {
     return s <= kResidentSide && l <= kResidentElems && (s + 31) / 32 * 32 * (resident_pitch((int)l) + resident_pitch((int)s)) <= kResidentElems;
 }
 
-template <bool STEP, typename Table>
+// SIDE: the short side in tiles of 16, padded to 32: 2, 4, 6 or 8.  A constant, so that the addresses of the square matrix's tiles
+// are one register and offsets in the instructions.
+template <int SIDE, bool STEP, typename Table>
 __global__ __launch_bounds__(kResidentThreads) void fsadam_matrix_resident(Table tables, ResidentArgs k, MomentumArgs mk) {
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
     __shared__ double part[kResidentWaves];
@@ -973,20 +976,26 @@ __global__ __launch_bounds__(kResidentThreads) void fsadam_matrix_resident(Table
         if (table[mid].first_matrix <= (int)blockIdx.x) low = mid;
         else high = mid - 1;
     }
-    const ResidentRow& row = table[low];
+    const ResidentRow row = table[low];
+    // The arguments of a launch are not in the GPU's memory: the factors of all steps are fetched together, once.
+    __shared__ float factors[5][kMaxSteps];
+    if (threadIdx.x < 5 * kMaxSteps) (&factors[0][0])[threadIdx.x] = (&k.factors[0][0])[threadIdx.x];
+    const int steps = k.steps, src_type = k.src_type, dst_type = k.dst_type, copy_type = k.copy_type;
+    const float keep = k.keep;
     const int64_t matrix = (int)blockIdx.x - row.first_matrix;
     const int rows = row.rows, cols = row.cols;
     const bool tall = rows > cols;
     const int s = tall ? cols : rows, l = tall ? rows : cols;
-    const int sp = (s + 31) / 32 * 32, lp = (l + 31) / 32 * 32, pitch_x = lp + 8, pitch_a = sp + 8;
-    const int plane_x = sp * pitch_x, plane_a = sp * pitch_a;  // halves
-    _Float16* x = reinterpret_cast<_Float16*>(lds);
-    _Float16* a = x + 2 * plane_x;
+    constexpr int sp = SIDE * 16, pitch_a = sp + 8, plane_a = sp * pitch_a;  // halves
+    const int lp = (l + 31) / 32 * 32, pitch_x = lp + 8, plane_x = sp * pitch_x;
+    _Float16* a = reinterpret_cast<_Float16*>(lds);
+    _Float16* x = a + 2 * plane_a;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int g = lane >> 4, c = lane & 15;
 
     // the padding is zero and stays zero
     for (int e = tid; e < 2 * plane_x / 8; e += kResidentThreads) *reinterpret_cast<half8_t*>(x + e * 8) = half8_t{};
+    __syncthreads();
     // element e of the matrix, row-major as in the source
     const int numel = rows * cols;
     const float per_row = 1.0f / (float)cols;
@@ -996,34 +1005,59 @@ __global__ __launch_bounds__(kResidentThreads) void fsadam_matrix_resident(Table
     };
     const Divisor by(mk);
     const int64_t base = matrix * row.src_stride, flat = matrix * numel;
-    constexpr int kBatch = 8;  // loads in flight
     double sum = 0.0;
-    for (int e0 = tid; e0 < numel; e0 += kResidentThreads * kBatch) {
-        float v[kBatch], m[kBatch];
+    float u[kResidentBatch];
+    // elements e0, e0 + 1024, ... : all loads first
+    auto fetch = [&](int e0, bool first) {
+        int64_t at[kResidentBatch];
 #pragma unroll
-        for (int n = 0; n < kBatch; ++n) {
+        for (int n = 0; n < kResidentBatch; ++n) {
             const int e = e0 + n * kResidentThreads;
-            v[n] = m[n] = 0.0f;
-            if (e < numel) {
-                if constexpr (STEP) {
-                    v[n] = load_as_float(row.src, flat + e, k.src_type);
-                    m[n] = row.buf[flat + e];
+            int r, q;
+            place(e, r, q);
+            at[n] = e >= numel ? -1 : STEP ? flat + e : base + r * row.src_ld + q;
+        }
+        if (src_type == kTypeF32) {
+#pragma unroll
+            for (int n = 0; n < kResidentBatch; ++n) u[n] = at[n] >= 0 ? static_cast<const float*>(row.src)[at[n]] : 0.0f;
+        } else {
+            uint16_t raw[kResidentBatch];
+#pragma unroll
+            for (int n = 0; n < kResidentBatch; ++n) raw[n] = at[n] >= 0 ? static_cast<const uint16_t*>(row.src)[at[n]] : (uint16_t)0;
+#pragma unroll
+            for (int n = 0; n < kResidentBatch; ++n) u[n] = src_type == kTypeF16 ? (float)__builtin_bit_cast(_Float16, raw[n]) : low_half(raw[n]);
+        }
+        if constexpr (STEP) {
+            float m[kResidentBatch];
+#pragma unroll
+            for (int n = 0; n < kResidentBatch; ++n) m[n] = at[n] >= 0 ? row.buf[at[n]] : 0.0f;
+#pragma unroll
+            for (int n = 0; n < kResidentBatch; ++n) {
+                if (first) {
+                    u[n] = momentum_update(by(u[n]), m[n], mk);
+                    if (at[n] >= 0) row.buf[at[n]] = m[n];
                 } else {
-                    int r, q;
-                    place(e, r, q);
-                    v[n] = load_as_float(row.src, base + r * row.src_ld + q, k.src_type);
+                    u[n] = update_again(by(u[n]), m[n], mk);
                 }
             }
         }
+    };
+    auto spread = [&](int e0, double factor) {
 #pragma unroll
-        for (int n = 0; n < kBatch; ++n) {
+        for (int n = 0; n < kResidentBatch; ++n) {
             const int e = e0 + n * kResidentThreads;
-            if constexpr (STEP) {
-                v[n] = momentum_update(by(v[n]), m[n], mk);
-                if (e < numel) row.buf[flat + e] = m[n];
-            }
-            sum = __builtin_fma((double)v[n], (double)v[n], sum);
+            if (e >= numel) continue;
+            int r, q;
+            place(e, r, q);
+            const int at = tall ? q * pitch_x + r : r * pitch_x + q;
+            split_halves((float)((double)u[n] * factor), x[at], x[plane_x + at]);
         }
+    };
+    constexpr int kTurn = kResidentThreads * kResidentBatch;  // elements of one turn; a matrix of no more is read once
+    for (int e0 = tid; e0 < numel; e0 += kTurn) {
+        fetch(e0, true);
+#pragma unroll
+        for (int n = 0; n < kResidentBatch; ++n) sum = __builtin_fma((double)u[n], (double)u[n], sum);
     }
     for (int d = 32; d > 0; d >>= 1) sum += __shfl_down(sum, d);
     if (lane == 0) part[wave] = sum;
@@ -1033,142 +1067,174 @@ __global__ __launch_bounds__(kResidentThreads) void fsadam_matrix_resident(Table
     for (int n = 0; n < kResidentWaves; ++n) sum += part[n];
     const double norm = sqrt(sum);
     const double factor = __builtin_isfinite(sum) ? k.power / (norm > k.eps ? norm : k.eps) : __builtin_nan("");
-    for (int e0 = tid; e0 < numel; e0 += kResidentThreads * kBatch) {
-        float v[kBatch], m[kBatch];
-        int r[kBatch], q[kBatch];
-#pragma unroll
-        for (int n = 0; n < kBatch; ++n) {
-            const int e = e0 + n * kResidentThreads;
-            place(e, r[n], q[n]);
-            if (e < numel) {
-                if constexpr (STEP) {
-                    v[n] = load_as_float(row.src, flat + e, k.src_type);
-                    m[n] = row.buf[flat + e];
-                } else {
-                    v[n] = load_as_float(row.src, base + r[n] * row.src_ld + q[n], k.src_type);
-                }
-            }
-        }
-#pragma unroll
-        for (int n = 0; n < kBatch; ++n) {
-            if (e0 + n * kResidentThreads >= numel) continue;
-            const float u = STEP ? update_again(by(v[n]), m[n], mk) : v[n];
-            const int at = tall ? q[n] * pitch_x + r[n] : r[n] * pitch_x + q[n];
-            split_halves((float)((double)u * factor), x[at], x[plane_x + at]);
+    if (numel <= kTurn) {
+        spread(tid, factor);
+    } else {
+        for (int e0 = tid; e0 < numel; e0 += kTurn) {
+            fetch(e0, false);
+            spread(e0, factor);
         }
     }
     __syncthreads();
 
-    auto fragment = [&](const _Float16* p, int pitch) { return *reinterpret_cast<const half8_t*>(p + c * pitch + g * 8); };  // 16 rows, 32 deep
-    auto turned = [&](const _Float16* q, int pitch) {  // 32 deep, 16 columns
-        const _Float16* at = q + (8 * g + (c >> 2)) * pitch + (c & 3) * 4;
+    auto read8 = [](const _Float16* p) { return *reinterpret_cast<const half8_t*>(p); };
+    auto turned = [](const _Float16* at, int pitch) {  // rows at, at + pitch, ... + 7 pitch of 16 columns: eight deep for every column
         const short4_t first = __builtin_amdgcn_ds_read_tr16_b64_v4i16((FM_LDS short4_t*)at);
         const short4_t second = __builtin_amdgcn_ds_read_tr16_b64_v4i16((FM_LDS short4_t*)(at + 4 * pitch));
         return __builtin_shufflevector(__builtin_bit_cast(half4_t, first), __builtin_bit_cast(half4_t, second), 0, 1, 2, 3, 4, 5, 6, 7);
     };
-    // A 16 x 16 tile of M M^T, M of two planes: rows from `p` and from `q` on.
-    auto product = [&](const _Float16* p, const _Float16* q, int pitch, int plane, int depth) {
-        float4_t high = {0.0f, 0.0f, 0.0f, 0.0f}, cross = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int d = 0; d < depth; d += 32) {
-            const half8_t p0 = fragment(p + d, pitch), p1 = fragment(p + plane + d, pitch), q0 = fragment(q + d, pitch), q1 = fragment(q + plane + d, pitch);
-            cross = __builtin_amdgcn_mfma_f32_16x16x32_f16(p1, q0, cross, 0, 0, 0);
-            cross = __builtin_amdgcn_mfma_f32_16x16x32_f16(p0, q1, cross, 0, 0, 0);
-            high = __builtin_amdgcn_mfma_f32_16x16x32_f16(p0, q0, high, 0, 0, 0);
-        }
-        return high + cross;
-    };
-    const int side = sp / 16, n_square = side * (side + 1) / 2, along = lp / 16;
-    auto triangle = [&](int t, int& ti, int& tj) {
+    auto mfma = [](const half8_t& p, const half8_t& q, const float4_t& v) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(p, q, v, 0, 0, 0); };
+    // lane (g, c): operands hold row c, eight deep from 8 g on; a product holds rows 4 g .. 4 g + 3 of column c
+    const _Float16* const row_a = a + c * pitch_a + g * 8;
+    const _Float16* const row_x = x + c * pitch_x + g * 8;
+    constexpr int kSquare = SIDE * (SIDE + 1) / 2, kRounds = (kSquare + kResidentWaves - 1) / kResidentWaves;
+    auto triangle = [&](int t, int& ti, int& tj) {  // row by row under the diagonal
         ti = 0;
-        while ((ti + 1) * (ti + 2) / 2 <= t) ++ti;
+#pragma unroll
+        for (int n = 1; n < SIDE; ++n) ti += t >= n * (n + 1) / 2;
         tj = t - ti * (ti + 1) / 2;
     };
-    // lane (g, c) holds rows 4 g .. 4 g + 3 of column c of a tile
     auto put_square = [&](int ti, int tj, const float4_t& v) {  // the lower triangle and its mirror image
+        half4_t hi, lo;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const int i = ti * 16 + 4 * g + r, j = tj * 16 + c;
-            if (j > i) continue;
-            _Float16 hi, lo;
-            split_halves(v[r], hi, lo);
-            a[i * pitch_a + j] = a[j * pitch_a + i] = hi;
-            a[plane_a + i * pitch_a + j] = a[plane_a + j * pitch_a + i] = lo;
+            _Float16 h, o;
+            split_halves(v[r], h, o);
+            hi[r] = h;
+            lo[r] = o;
         }
-    };
-    for (int step = 0; step < k.steps; ++step) {
-        for (int n = 0; n < kResidentSquareTiles; ++n) {
-            const int t = wave + n * kResidentWaves;
-            if (t >= n_square) break;
-            int ti, tj;
-            triangle(t, ti, tj);
-            put_square(ti, tj, product(x + ti * 16 * pitch_x, x + tj * 16 * pitch_x, pitch_x, plane_x, lp) * k.gram[step]);
-        }
-        __syncthreads();
-        float4_t b[kResidentSquareTiles];
-#pragma unroll
-        for (int n = 0; n < kResidentSquareTiles; ++n) {
-            const int t = wave + n * kResidentWaves;
-            if (t >= n_square) continue;
-            int ti, tj;
-            triangle(t, ti, tj);
-            b[n] = product(a + ti * 16 * pitch_a, a + tj * 16 * pitch_a, pitch_a, plane_a, sp) * k.product_b[step];
+        _Float16* const here = a + (ti * 16 + 4 * g) * pitch_a + tj * 16 + c;
+        _Float16* const there = a + (tj * 16 + c) * pitch_a + ti * 16 + 4 * g;
+        if (ti != tj) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const int at = (ti * 16 + 4 * g + r) * pitch_a + tj * 16 + c;
-                b[n][r] += k.linear_b[step] * ((float)a[at] + (float)a[plane_a + at]);
+                here[r * pitch_a] = hi[r];
+                here[plane_a + r * pitch_a] = lo[r];
             }
+            *reinterpret_cast<half4_t*>(there) = hi;
+            *reinterpret_cast<half4_t*>(there + plane_a) = lo;
+        } else {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                if (c > 4 * g + r) continue;
+                here[r * pitch_a] = there[r] = hi[r];
+                here[plane_a + r * pitch_a] = there[plane_a + r] = lo[r];
+            }
+        }
+    };
+    // A wave takes whole columns of tiles of X: what it overwrites, it alone has read.
+    constexpr int kAtOnce = SIDE % 4 == 0 ? 4 : 2;
+    const int along = lp / 16;
+    auto columns = [&](int step, auto&& done) {
+        const float linear = factors[kFactorLinearX][step], scale = factors[kFactorProductX][step];
+        for (int tj = wave; tj < along; tj += kResidentWaves) {
+            float4_t next[SIDE];
+#pragma unroll
+            for (int ti = 0; ti < SIDE; ++ti) next[ti] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+            const _Float16* column = x + (8 * g + (c >> 2)) * pitch_x + (c & 3) * 4 + tj * 16;
+#pragma unroll 1
+            for (int d = 0; d < SIDE / 2; ++d, column += 32 * pitch_x) {
+                const half8_t q0 = turned(column, pitch_x), q1 = turned(column + plane_x, pitch_x);
+#pragma unroll
+                for (int t0 = 0; t0 < SIDE; t0 += kAtOnce) {
+                    half8_t p0[kAtOnce], p1[kAtOnce];
+#pragma unroll
+                    for (int t = 0; t < kAtOnce; ++t) {
+                        p0[t] = read8(row_a + d * 32 + (t0 + t) * 16 * pitch_a);
+                        p1[t] = read8(row_a + d * 32 + plane_a + (t0 + t) * 16 * pitch_a);
+                    }
+#pragma unroll
+                    for (int t = 0; t < kAtOnce; ++t) next[t0 + t] = mfma(p1[t], q0, next[t0 + t]);
+#pragma unroll
+                    for (int t = 0; t < kAtOnce; ++t) next[t0 + t] = mfma(p0[t], q1, next[t0 + t]);
+#pragma unroll
+                    for (int t = 0; t < kAtOnce; ++t) next[t0 + t] = mfma(p0[t], q0, next[t0 + t]);
+                }
+            }
+            _Float16* at = x + 4 * g * pitch_x + tj * 16 + c;
+#pragma unroll
+            for (int ti = 0; ti < SIDE; ++ti, at += 16 * pitch_x) {
+                float o[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) o[r] = linear * ((float)at[r * pitch_x] + (float)at[plane_x + r * pitch_x]) + scale * next[ti][r];
+                done(at, ti * 16 + 4 * g, tj * 16 + c, o);
+            }
+        }
+    };
+    for (int step = 0; step < steps; ++step) {
+#pragma unroll
+        for (int n = 0; n < kRounds; ++n) {
+            const int t = wave + n * kResidentWaves;
+            if (t >= kSquare) break;
+            int ti, tj;
+            triangle(t, ti, tj);
+            const _Float16 *p = row_x + ti * 16 * pitch_x, *q = row_x + tj * 16 * pitch_x;
+            float4_t high = {0.0f, 0.0f, 0.0f, 0.0f}, cross = high, cross2 = high;
+            for (int d = 0; d < lp; d += 32) {
+                const half8_t p0 = read8(p + d), p1 = read8(p + plane_x + d), q0 = read8(q + d), q1 = read8(q + plane_x + d);
+                cross = mfma(p1, q0, cross);
+                cross2 = mfma(p0, q1, cross2);
+                high = mfma(p0, q0, high);
+            }
+            put_square(ti, tj, (high + (cross + cross2)) * factors[kFactorGram][step]);
+        }
+        __syncthreads();
+        float4_t b[kRounds];
+#pragma unroll
+        for (int n = 0; n < kRounds; ++n) {
+            const int t = wave + n * kResidentWaves;
+            if (t >= kSquare) break;
+            int ti, tj;
+            triangle(t, ti, tj);
+            const _Float16 *p = row_a + ti * 16 * pitch_a, *q = row_a + tj * 16 * pitch_a;
+            float4_t high = {0.0f, 0.0f, 0.0f, 0.0f}, cross = high, cross2 = high;
+#pragma unroll
+            for (int d = 0; d < sp; d += 32) {
+                const half8_t p0 = read8(p + d), p1 = read8(p + plane_a + d), q0 = read8(q + d), q1 = read8(q + plane_a + d);
+                cross = mfma(p1, q0, cross);
+                cross2 = mfma(p0, q1, cross2);
+                high = mfma(p0, q0, high);
+            }
+            const _Float16* here = a + (ti * 16 + 4 * g) * pitch_a + tj * 16 + c;
+            const float linear = factors[kFactorLinearB][step], scale = factors[kFactorProductB][step];
+            b[n] = (high + (cross + cross2)) * scale;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) b[n][r] += linear * ((float)here[r * pitch_a] + (float)here[plane_a + r * pitch_a]);
         }
         __syncthreads();  // A has been read: B takes its place
 #pragma unroll
-        for (int n = 0; n < kResidentSquareTiles; ++n) {
+        for (int n = 0; n < kRounds; ++n) {
             const int t = wave + n * kResidentWaves;
-            if (t >= n_square) continue;
+            if (t >= kSquare) break;
             int ti, tj;
             triangle(t, ti, tj);
             put_square(ti, tj, b[n]);
         }
         __syncthreads();
-        // A wave takes whole columns of tiles: what it overwrites, it alone has read.
-        const bool last = step + 1 == k.steps;
-        for (int tj = wave; tj < along; tj += kResidentWaves) {
-            float4_t next[kResidentSide / 16];
+        if (step + 1 < steps) {
+            columns(step, [&](_Float16* at, int, int, const float (&o)[4]) {
 #pragma unroll
-            for (int ti = 0; ti < kResidentSide / 16; ++ti) next[ti] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
-            for (int d = 0; d < sp; d += 32) {
-                const half8_t q0 = turned(x + d * pitch_x + tj * 16, pitch_x), q1 = turned(x + plane_x + d * pitch_x + tj * 16, pitch_x);
-#pragma unroll
-                for (int ti = 0; ti < kResidentSide / 16; ++ti) {
-                    if (ti >= side) break;
-                    const half8_t p0 = fragment(a + ti * 16 * pitch_a + d, pitch_a), p1 = fragment(a + plane_a + ti * 16 * pitch_a + d, pitch_a);
-                    next[ti] = __builtin_amdgcn_mfma_f32_16x16x32_f16(p1, q0, next[ti], 0, 0, 0);
-                    next[ti] = __builtin_amdgcn_mfma_f32_16x16x32_f16(p0, q1, next[ti], 0, 0, 0);
-                    next[ti] = __builtin_amdgcn_mfma_f32_16x16x32_f16(p0, q0, next[ti], 0, 0, 0);
-                }
-            }
-#pragma unroll
-            for (int ti = 0; ti < kResidentSide / 16; ++ti) {
-                if (ti >= side) break;
+                for (int r = 0; r < 4; ++r) split_halves(o[r], at[r * pitch_x], at[plane_x + r * pitch_x]);
+            });
+            __syncthreads();
+        } else {
+            columns(step, [&](_Float16*, int i, int j, const float (&o)[4]) {
+                const int64_t step_i = tall ? 1 : STEP ? cols : row.dst_ld, step_j = tall ? (STEP ? cols : row.dst_ld) : 1;
+                const int64_t to = (STEP ? flat : matrix * row.dst_stride) + i * step_i + j * step_j;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const int i = ti * 16 + 4 * g + r, j = tj * 16 + c, at = i * pitch_x + j;
-                    const float o = k.linear_x[step] * ((float)x[at] + (float)x[plane_x + at]) + k.product_x[step] * next[ti][r];
-                    if (!last) {
-                        split_halves(o, x[at], x[plane_x + at]);
-                    } else if (i < s && j < l) {
-                        const int64_t to_row = tall ? j : i, to_col = tall ? i : j;
-                        if constexpr (STEP) {
-                            const int64_t to = flat + to_row * cols + to_col;
-                            const float p = load_as_float(row.dst, to, k.dst_type) * k.keep - row.step_ratio * o;
-                            store_from_float(row.dst, to, k.dst_type, p);
-                            if (k.copy_type >= 0) store_from_float(row.copy, to, k.copy_type, p);
-                        } else {
-                            store_from_float(row.dst, matrix * row.dst_stride + to_row * row.dst_ld + to_col, k.dst_type, o);
-                        }
+                    if (i + r >= s || j >= l) continue;
+                    if constexpr (STEP) {
+                        const float p = load_as_float(row.dst, to + r * step_i, dst_type) * keep - row.step_ratio * o[r];
+                        store_from_float(row.dst, to + r * step_i, dst_type, p);
+                        if (copy_type >= 0) store_from_float(row.copy, to + r * step_i, copy_type, p);
+                    } else {
+                        store_from_float(row.dst, to + r * step_i, dst_type, o[r]);
                     }
                 }
-            }
+                __builtin_amdgcn_sched_barrier(0);  // one tile's addresses at a time: the registers do not hold those of eight
+            });
         }
-        __syncthreads();
     }
 }
 
