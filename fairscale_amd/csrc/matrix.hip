@@ -151,7 +151,8 @@ int64_t add_to_chunk(Chunk& chunk, const MatrixRow& proto, int64_t batch) {
     const int64_t per = 2 * x + squares * a, room = kChunkBytes / 2 - chunk.halves;
     int64_t n = std::min(batch, room / per);
     int64_t most = kMaxTiles;
-    for (int k = 0; k < kTileKinds; ++k) most = std::min(most, (kMaxTiles - chunk.tiles[k]) / proto.n[k]);
+    for (int k = 0; k < kTileKinds; ++k)
+        if (proto.n[k]) most = std::min(most, (kMaxTiles - chunk.tiles[k]) / proto.n[k]);
     n = std::min(n, most);
     if (n < 1) {
         if (!chunk.rows.empty()) return 0;
@@ -189,6 +190,14 @@ struct Source {  // what a list entry's row starts from
 // call waits for.
 constexpr int64_t kAlwaysSplit = 128;
 
+// A Gram matrix of few tiles and long inner products keeps a few compute units busy for long: parts of kPartDepth are summed by
+// workgroups of their own and joined in order by a second launch.  By the matrix alone, so that its bits do not depend on the
+// list.  32 matrices of 128 x 4096: 39 -> 13 us.
+int gram_parts(int64_t s64, int64_t l64) {
+    if (s64 > 384 || l64 < 2 * kPartDepth) return 1;
+    return (int)((l64 + kPartDepth - 1) / kPartDepth);
+}
+
 bool resident(const Source& in) { return resident_fits(std::min(in.rows, in.cols), std::max(in.rows, in.cols)); }
 
 void make_chunks(const std::vector<Source>& all, int asked, std::vector<Chunk>& chunks) {
@@ -208,12 +217,14 @@ void make_chunks(const std::vector<Source>& all, int asked, std::vector<Chunk>& 
         row.dst_ld = in.dst_ld; row.dst_stride = in.dst_stride;
         row.step_ratio = in.step_ratio;
         row.chunks = (int32_t)(up(in.rows * in.cols, kChunkElems) / kChunkElems);
-        row.n[kTilesSym64] = (int32_t)symmetric_tiles(row.s64, 64);
-        row.n[kTilesFull64] = (int32_t)full_tiles(row.s64, row.l64, 64);
-        row.n[kTilesSym128] = (int32_t)symmetric_tiles(row.s64, 128);
-        row.n[kTilesFull128] = (int32_t)full_tiles(row.s64, row.l64, 128);
-        row.n[kTilesSym256] = (int32_t)symmetric_tiles(row.s64, 256);
-        row.n[kTilesFull256] = (int32_t)full_tiles(row.s64, row.l64, 256);
+        row.parts = gram_parts(row.s64, row.l64);
+        for (int t = 64, k = kTilesSym64; t <= 256; t *= 2, k += 3) {
+            row.n[k] = (int32_t)symmetric_tiles(row.s64, t);
+            row.n[k + 1] = (int32_t)full_tiles(row.s64, row.l64, t);
+            row.n[k + 2] = row.parts > 1 ? 0 : row.n[k];  // the Gram matrix
+        }
+        row.n[kTilesJoin] = row.parts > 1 ? row.n[kTilesSym64] : 0;
+        row.n[kTilesPart] = row.n[kTilesJoin] * row.parts;
         row.n[kTilesPrep] = (int32_t)full_tiles(row.s64, row.l64, 64);
         row.n[kTilesChunk] = row.chunks;
         int64_t done = 0;
@@ -282,8 +293,9 @@ int check_shape(int64_t t, int64_t batch, int64_t rows, int64_t cols) {
 
 template <int STAGE, int PLANES>
 void launch_tiles(const Chunk& c, const MatrixRow* table, const StageArgs& k, _Float16* work, hipStream_t stream) {
-    constexpr bool kSym = STAGE == kStageGram || STAGE == kStageSquare;
-    const int64_t t64 = c.tiles[kSym ? kTilesSym64 : kTilesFull64], t128 = c.tiles[kSym ? kTilesSym128 : kTilesFull128], t256 = c.tiles[kSym ? kTilesSym256 : kTilesFull256];
+    constexpr int kind = STAGE == kStageGram ? 2 : STAGE == kStageSquare ? 0 : 1;
+    const int64_t t64 = c.tiles[kTilesSym64 + kind], t128 = c.tiles[kTilesSym128 + kind], t256 = c.tiles[kTilesSym256 + kind];
+    if (t64 == 0) return;  // every Gram matrix is split
     const int n = (int)c.rows.size();
     static const int force = getenv("FM_TILE") ? atoi(getenv("FM_TILE")) : 0;
 #define FM_LAUNCH(TILE, WM, WN, BK, DEPTH, COUNT)     hipLaunchKernelGGL((fsadam_matrix_stage<STAGE, TILE, TILE, WM, WN, BK, DEPTH, PLANES>), dim3((uint32_t)COUNT), dim3(64 * WM * WN), 0, stream, table, n, k, work)
@@ -302,7 +314,14 @@ void launch_tiles(const Chunk& c, const MatrixRow* table, const StageArgs& k, _F
 template <int PLANES>
 int launch_stage(int stage, const Chunk& c, const MatrixRow* table, const StageArgs& k, _Float16* work, hipStream_t stream) {
     switch (stage) {
-        case kStageGram: launch_tiles<kStageGram, PLANES>(c, table, k, work, stream); break;
+        case kStageGram:
+            launch_tiles<kStageGram, PLANES>(c, table, k, work, stream);
+            if (c.tiles[kTilesPart]) {
+                const int n = (int)c.rows.size();
+                hipLaunchKernelGGL((fsadam_matrix_stage<kStagePart, 64, 64, 2, 2, 64, 2, PLANES>), dim3((uint32_t)c.tiles[kTilesPart]), dim3(256), 0, stream, table, n, k, work);
+                hipLaunchKernelGGL((fsadam_matrix_stage<kStageJoin, 64, 64, 2, 2, 64, 2, PLANES>), dim3((uint32_t)c.tiles[kTilesJoin]), dim3(256), 0, stream, table, n, k, work);
+            }
+            break;
         case kStageSquare: launch_tiles<kStageSquare, PLANES>(c, table, k, work, stream); break;
         case kStageUpdate: launch_tiles<kStageUpdate, PLANES>(c, table, k, work, stream); break;
         case kStageOut: launch_tiles<kStageOut, PLANES>(c, table, k, work, stream); break;

@@ -40,7 +40,10 @@ typedef float float4_t __attribute__((ext_vector_type(4)));
 enum { kTypeF32 = 0, kTypeF16 = 1, kTypeBF16 = 2 };
 
 // Which of a row's tile counts a launch goes by.
-enum { kTilesSym64, kTilesFull64, kTilesSym128, kTilesFull128, kTilesSym256, kTilesFull256, kTilesPrep, kTilesChunk, kTileKinds };
+enum {
+    kTilesSym64, kTilesFull64, kTilesGram64, kTilesSym128, kTilesFull128, kTilesGram128, kTilesSym256, kTilesFull256, kTilesGram256,
+    kTilesPart, kTilesJoin, kTilesPrep, kTilesChunk, kTileKinds
+};
 
 // One row of a call's table: `batch` matrices of one shape, equally spaced.
 struct alignas(16) MatrixRow {
@@ -51,12 +54,12 @@ struct alignas(16) MatrixRow {
     int64_t src_ld, src_stride, dst_ld, dst_stride;  // elements from row to row, from matrix to matrix
     int64_t x_off[2];  // workspace: X and its successor (halves from the workspace's start)
     int64_t sq_off[3]; // workspace: square matrices (A and B; a pair of steps uses all three)
-    int64_t unused;
     int32_t batch, rows, cols;
     int32_t s, l, s64, l64;
     int32_t tall;      // rows > cols: X is the transpose
     int32_t first_matrix;           // index of the row's first matrix in the chunk
     int32_t chunks;                 // partial sums per matrix
+    int32_t parts;                  // of the Gram matrix's inner products; 1: not split
     float step_ratio;               // step: lr * ratio of this shape
     int32_t first[kTileKinds];      // tiles of the rows before this one
     int32_t n[kTileKinds];          // tiles of one matrix
@@ -523,7 +526,10 @@ __global__ __launch_bounds__(256) void fsadam_matrix_normalise(const MatrixRow* 
 
 // ---- the products -------------------------------------------------------------------------------------------------
 
-enum { kStageGram, kStageSquare, kStageUpdate, kStageOut, kStageStep };
+enum { kStagePart, kStageJoin, kStageGram, kStageSquare, kStageUpdate, kStageOut, kStageStep };
+
+// Depth of a part of a Gram matrix's inner products, where they are split.
+constexpr int kPartDepth = 512;
 
 struct StageArgs {
     int from, to;       // which of the two X buffers is read and written
@@ -746,18 +752,25 @@ struct Product {
 // One stage of the iteration over every matrix of the chunk.
 template <int STAGE, int TM, int TN, int WM, int WN, int BK, int DEPTH, int PLANES>
 __global__ __launch_bounds__(64 * WM * WN) void fsadam_matrix_stage(const MatrixRow* table, int n_rows, StageArgs k, _Float16* work) {
-    constexpr bool kSym = STAGE == kStageGram || STAGE == kStageSquare;
+    constexpr bool kSym = STAGE <= kStageSquare;
     constexpr bool kNN = !kSym;
     using Prod = Product<TM, TN, WM, WN, BK, DEPTH, PLANES, kNN>;
     constexpr int kSlab = 64, kStride = TN + 4;  // the accumulators pass through LDS 64 rows at a time
     constexpr int kLdsBytes = Prod::kLdsHalves * 2 > kSlab * kStride * 4 ? Prod::kLdsHalves * 2 : kSlab * kStride * 4;
     __shared__ __attribute__((aligned(1024))) unsigned char lds[kLdsBytes];
 
-    constexpr int kind = TM == 64 ? (kSym ? kTilesSym64 : kTilesFull64) : TM == 128 ? (kSym ? kTilesSym128 : kTilesFull128) : (kSym ? kTilesSym256 : kTilesFull256);
+    constexpr int kind = STAGE == kStagePart ? kTilesPart : STAGE == kStageJoin ? kTilesJoin
+                         : (TM == 64 ? kTilesSym64 : TM == 128 ? kTilesSym128 : kTilesSym256) + (STAGE == kStageGram ? 2 : kSym ? 0 : 1);
+    static_assert(kTilesFull64 == kTilesSym64 + 1 && kTilesGram64 == kTilesSym64 + 2 && kTilesGram128 == kTilesSym128 + 2 && kTilesGram256 == kTilesSym256 + 2);
     int matrix;
     uint32_t tile;
     const MatrixRow& row = find_tile(table, n_rows, kind, xcd_contiguous(blockIdx.x, gridDim.x), matrix, tile);
     const int s64 = row.s64, l64 = row.l64;
+    uint32_t part_of = 0;  // which part of a split inner product
+    if constexpr (STAGE == kStagePart) {
+        part_of = tile % (uint32_t)row.parts;
+        tile /= (uint32_t)row.parts;
+    }
     int ti, tj;
     if constexpr (kSym) {  // row by row under the diagonal
         ti = (int)((__builtin_sqrtf(8.0f * (float)tile + 1.0f) - 1.0f) * 0.5f);
@@ -775,7 +788,33 @@ __global__ __launch_bounds__(64 * WM * WN) void fsadam_matrix_stage(const Matrix
     const int i0 = ti * TM, j0 = tj * TN;
 
     Prod prod;
-    if constexpr (STAGE == kStageGram)
+    // The partial sums of a split product, in the X buffer that the next update writes: tile by tile, part by part, every lane's
+    // accumulators side by side.
+    float4_t* partial = nullptr;
+    if constexpr (STAGE == kStagePart || STAGE == kStageJoin) {
+        constexpr int kTile = TM * TN / 4;  // float4
+        partial = reinterpret_cast<float4_t*>(work + row.x_off[k.to] + (int64_t)matrix * 2 * plane_x) + ((int64_t)tile * row.parts + part_of) * kTile + threadIdx.x;
+    }
+    if constexpr (STAGE == kStagePart) {
+        const int from = (int)part_of * kPartDepth, depth = l64 - from < kPartDepth ? l64 - from : kPartDepth;
+        prod.run(x + (int64_t)i0 * l64 + from, l64, plane_x, s64 - i0, x + (int64_t)j0 * l64 + from, l64, plane_x, s64 - j0, depth, reinterpret_cast<_Float16*>(lds));
+#pragma unroll
+        for (int i = 0; i < Prod::MI; ++i)
+#pragma unroll
+            for (int j = 0; j < Prod::NJ; ++j) partial[(i * Prod::NJ + j) * Prod::kThreads] = prod.acc[i][j];
+        return;
+    } else if constexpr (STAGE == kStageJoin) {
+#pragma unroll
+        for (int i = 0; i < Prod::MI; ++i)
+#pragma unroll
+            for (int j = 0; j < Prod::NJ; ++j) prod.acc[i][j] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+        for (int n = 0; n < row.parts; ++n)  // in their order
+#pragma unroll
+            for (int i = 0; i < Prod::MI; ++i)
+#pragma unroll
+                for (int j = 0; j < Prod::NJ; ++j) prod.acc[i][j] += partial[n * (TM * TN / 4) + (i * Prod::NJ + j) * Prod::kThreads];
+    } else if constexpr (STAGE == kStageGram)
         prod.run(x + (int64_t)i0 * l64, l64, plane_x, s64 - i0, x + (int64_t)j0 * l64, l64, plane_x, s64 - j0, l64, reinterpret_cast<_Float16*>(lds));
     else if constexpr (STAGE == kStageSquare)
         prod.run(square(k.p) + (int64_t)i0 * s64, s64, plane_a, s64 - i0, square(k.q) + (int64_t)j0 * s64, s64, plane_a, s64 - j0, s64,
@@ -1239,7 +1278,7 @@ __global__ __launch_bounds__(kResidentThreads) void fsadam_matrix_resident(Table
 }
 
 // Rows of a call's table, in the arguments of the launch: nothing is allocated or copied, and a captured graph holds them.
-constexpr int kRowsPerPut = 16;
+constexpr int kRowsPerPut = 14;
 struct MatrixRows {
     MatrixRow row[kRowsPerPut];
 };
