@@ -225,6 +225,7 @@ void make_chunks(const std::vector<Source>& all, int asked, std::vector<Chunk>& 
         }
         row.n[kTilesJoin] = row.parts > 1 ? row.n[kTilesSym64] : 0;
         row.n[kTilesPart] = row.n[kTilesJoin] * row.parts;
+        row.n[kTilesAllParts] = row.n[kTilesSym64] * row.parts;
         row.n[kTilesPrep] = (int32_t)full_tiles(row.s64, row.l64, 64);
         row.n[kTilesChunk] = row.chunks;
         int64_t done = 0;
@@ -245,7 +246,7 @@ void make_chunks(const std::vector<Source>& all, int asked, std::vector<Chunk>& 
   }
 }
 
-// The rows of the list that fit LDS, of one padded short side.
+// The rows of the list that fit LDS.
 struct Residents {
     std::vector<ResidentRow> rows;
     int64_t matrices = 0;
@@ -254,28 +255,26 @@ struct Residents {
 };
 
 struct Plan {
-    Residents residents[kResidentSide / 32];  // by sides of 32, 64, 96, 128
+    Residents residents;
     std::vector<Chunk> chunks;
     Plan(const std::vector<Source>& list, int products) {
         for (const Source& in : list) {
             if (!resident(in)) continue;
             const int s = (int)std::min(in.rows, in.cols), l = (int)std::max(in.rows, in.cols);
-            Residents& kind = residents[(s - 1) / 32];
             ResidentRow row{};
             row.src = in.src; row.buf = in.buf; row.dst = in.dst; row.copy = in.copy;
             row.src_ld = in.src_ld; row.src_stride = in.src_stride; row.dst_ld = in.dst_ld; row.dst_stride = in.dst_stride;
             row.rows = (int32_t)in.rows; row.cols = (int32_t)in.cols;
-            row.first_matrix = (int32_t)kind.matrices;
+            row.first_matrix = (int32_t)residents.matrices;
             row.step_ratio = in.step_ratio;
-            kind.rows.push_back(row);
-            kind.matrices += in.batch;
-            kind.lds_bytes = std::max(kind.lds_bytes, (int)up(s, 32) * (resident_pitch(s) + resident_pitch(l)) * 4);
+            residents.rows.push_back(row);
+            residents.matrices += in.batch;
+            residents.lds_bytes = std::max(residents.lds_bytes, (int)up(s, 32) * (resident_pitch(s) + resident_pitch(l)) * 4);
         }
         make_chunks(list, products, chunks);
     }
     int64_t workspace() const {
-        int64_t bytes = 0;  // each part is done with the workspace when the next begins
-        for (const Residents& r : residents) bytes = std::max(bytes, r.bytes());
+        int64_t bytes = residents.bytes();  // their table is done with when the chunks begin
         for (const Chunk& c : chunks) bytes = std::max(bytes, c.bytes());
         return bytes;
     }
@@ -291,41 +290,41 @@ int check_shape(int64_t t, int64_t batch, int64_t rows, int64_t cols) {
 
 // ---- launches -----------------------------------------------------------------------------------------------------
 
-template <int STAGE, int PLANES>
-void launch_tiles(const Chunk& c, const MatrixRow* table, const StageArgs& k, _Float16* work, hipStream_t stream) {
-    constexpr int kind = STAGE == kStageGram ? 2 : STAGE == kStageSquare ? 0 : 1;
-    const int64_t t64 = c.tiles[kTilesSym64 + kind], t128 = c.tiles[kTilesSym128 + kind], t256 = c.tiles[kTilesSym256 + kind];
-    if (t64 == 0) return;  // every Gram matrix is split
-    const int n = (int)c.rows.size();
-    static const int force = getenv("FM_TILE") ? atoi(getenv("FM_TILE")) : 0;
-#define FM_LAUNCH(TILE, WM, WN, BK, DEPTH, COUNT)     hipLaunchKernelGGL((fsadam_matrix_stage<STAGE, TILE, TILE, WM, WN, BK, DEPTH, PLANES>), dim3((uint32_t)COUNT), dim3(64 * WM * WN), 0, stream, table, n, k, work)
-    if (force == 256) FM_LAUNCH(256, 2, 4, (PLANES == 2 ? 32 : 64), 2, t256);
-    else if (force == 1288) FM_LAUNCH(128, 2, 4, (PLANES == 2 ? 32 : 64), 2, t128);
-    else if (force == 642) FM_LAUNCH(64, 2, 2, 64, 2, t64);
-    else {
-        const auto cost = [](int64_t tiles, int64_t unit) { return (tiles + 255) / 256 * unit; };
-        const int64_t c64 = cost(t64, 13), c128 = cost(t128, 30), c256 = cost(t256, 92);
-        if (c256 < c128 && c256 < c64) FM_LAUNCH(256, 2, 4, (PLANES == 2 ? 32 : 64), 2, t256);
-        else if (c128 < c64) FM_LAUNCH(128, 2, 4, (PLANES == 2 ? 32 : 64), 2, t128);
-        else FM_LAUNCH(64, 2, 2, 64, 2, t64);
-    }
-#undef FM_LAUNCH
+// The tile of a launch: 64, 128 or 256 square, by what the busiest compute unit is given to do.  A unit of 64 x 64 is 13, what
+// takes 0.65 us per 64 of depth with 22-bit products; 128 takes 1.5 us and 256 takes 4.6 us, so that the larger tiles do 1.7 and
+// 2.2 times the work in the same time -- where there are enough of them for 256 compute units.  (11-bit products: about half
+// the times in the same proportion.)  Six matrices of 768 x 2304 and six of 768 x 768: update 101 / 99 / 73 us with
+// 64 / 128 / 256, square products 33 / 33 / 65.
+struct Tiles {
+    int size;
+    int64_t count;
+};
+Tiles choose_tiles(int64_t t64, int64_t t128, int64_t t256) {
+    const auto cost = [](int64_t tiles, int64_t unit) { return (tiles + 255) / 256 * unit; };
+    const int64_t c64 = cost(t64, 13), c128 = cost(t128, 30), c256 = cost(t256, 92);
+    if (c256 < c128 && c256 < c64) return {256, t256};
+    if (c128 < c64) return {128, t128};
+    return {64, t64};
 }
-template <int PLANES>
-int launch_stage(int stage, const Chunk& c, const MatrixRow* table, const StageArgs& k, _Float16* work, hipStream_t stream) {
-    switch (stage) {
-        case kStageGram:
-            launch_tiles<kStageGram, PLANES>(c, table, k, work, stream);
-            if (c.tiles[kTilesPart]) {
-                const int n = (int)c.rows.size();
-                hipLaunchKernelGGL((fsadam_matrix_stage<kStagePart, 64, 64, 2, 2, 64, 2, PLANES>), dim3((uint32_t)c.tiles[kTilesPart]), dim3(256), 0, stream, table, n, k, work);
-                hipLaunchKernelGGL((fsadam_matrix_stage<kStageJoin, 64, 64, 2, 2, 64, 2, PLANES>), dim3((uint32_t)c.tiles[kTilesJoin]), dim3(256), 0, stream, table, n, k, work);
-            }
-            break;
-        case kStageSquare: launch_tiles<kStageSquare, PLANES>(c, table, k, work, stream); break;
-        case kStageUpdate: launch_tiles<kStageUpdate, PLANES>(c, table, k, work, stream); break;
-        case kStageOut: launch_tiles<kStageOut, PLANES>(c, table, k, work, stream); break;
-        case kStageStep: launch_tiles<kStageStep, PLANES>(c, table, k, work, stream); break;
+
+template <int STAGE, int TILE, int PLANES>
+void launch_tile(int64_t count, int n_rows, const MatrixRow* table, const StageArgs& k, _Float16* work, hipStream_t stream) {
+    constexpr int WM = 2, WN = TILE == 64 ? 2 : 4, BK = TILE > 64 && PLANES == 2 ? 32 : 64;
+    if (count) hipLaunchKernelGGL((fsadam_matrix_stage<STAGE, TILE, TILE, WM, WN, BK, 2, PLANES>), dim3((uint32_t)count), dim3(64 * WM * WN), 0, stream, table, n_rows, k, work);
+}
+
+template <int STAGE, int PLANES>
+int launch_stage(const Chunk& c, const MatrixRow* table, StageArgs k, _Float16* work, hipStream_t stream) {
+    constexpr int kind = STAGE == kStageGram ? 2 : STAGE == kStageSquare ? 0 : 1;
+    const int n = (int)c.rows.size();
+    const Tiles t = choose_tiles(c.tiles[kTilesSym64 + kind], c.tiles[kTilesSym128 + kind], c.tiles[kTilesSym256 + kind]);
+    if (t.size == 256) launch_tile<STAGE, 256, PLANES>(t.count, n, table, k, work, stream);
+    else if (t.size == 128) launch_tile<STAGE, 128, PLANES>(t.count, n, table, k, work, stream);
+    else if (STAGE != kStageGram) launch_tile<STAGE, 64, PLANES>(t.count, n, table, k, work, stream);
+    if constexpr (STAGE == kStageGram) {  // split products are in tiles of 64; the others join their launch where they are too
+        k.kind = t.size == 64 ? kTilesAllParts : kTilesPart;
+        launch_tile<kStageGram, 64, PLANES>(c.tiles[k.kind], n, table, k, work, stream);
+        launch_tile<kStageJoin, 64, PLANES>(c.tiles[kTilesJoin], n, table, k, work, stream);
     }
     return launched();
 }
@@ -383,27 +382,32 @@ int run_chunk(const Chunk& c, const Call& call, void* workspace, hipStream_t str
     k.dst_type = call.dst_type;
     k.copy_type = call.copy_type;
     k.keep = call.keep;
-    auto stage = [&](int which) {
-        return c.products == FSADAM_PRODUCTS_SPLIT ? launch_stage<2>(which, c, table, k, work, stream) : launch_stage<1>(which, c, table, k, work, stream);
+    auto stage = [&](auto which) {
+        constexpr int kStage = decltype(which)::value;
+        return c.products == FSADAM_PRODUCTS_SPLIT ? launch_stage<kStage, 2>(c, table, k, work, stream) : launch_stage<kStage, 1>(c, table, k, work, stream);
     };
+    constexpr std::integral_constant<int, kStageGram> gram{};
+    constexpr std::integral_constant<int, kStageSquare> square_stage{};
+    constexpr std::integral_constant<int, kStageUpdate> update{};
+    constexpr std::integral_constant<int, kStageOut> out{};
+    constexpr std::integral_constant<int, kStageStep> step{};
     auto square = [&](int p, int q, int add, double linear, int linear_exp, double product, int product_exp, double diagonal, int into) {
         k.p = p; k.q = q; k.add = add; k.into = into;
         k.linear = (float)std::ldexp(linear, linear_exp);
         k.product = (float)std::ldexp(product, product_exp);
         k.diagonal = (float)diagonal;
-        return stage(kStageSquare);
+        return stage(square_stage);
     };
     int s = 0, from = 0;
     while (s < o.steps) {
         const bool pair = c.pairs() && s + 2 <= o.steps;
         const StepNumbers& n0 = n[s];
         const int after = s + (pair ? 2 : 1), next_x = after < o.steps ? n[after].x : 0;
-        const int last = after < o.steps ? kStageUpdate : call.step ? kStageStep : kStageOut;
         k.from = from;
         k.to = from ^ 1;
         k.into = 0;
         k.product = (float)std::ldexp(1.0, n0.a - 2 * n0.x);
-        if ((rc = stage(kStageGram))) return rc;  // 0: A
+        if ((rc = stage(gram))) return rc;  // 0: A
         if (pair) {
             const StepNumbers& n1 = n[s + 1];
             const int q = exponent_for(n0.q_bound * n1.q_bound);
@@ -421,14 +425,13 @@ int run_chunk(const Chunk& c, const Call& call, void* workspace, hipStream_t str
             k.linear = (float)std::ldexp((double)o.a, next_x - n0.x);
             k.product = (float)std::ldexp(1.0, next_x - n0.b - n0.x);
         }
-        if ((rc = stage(last))) return rc;
+        if ((rc = after < o.steps ? stage(update) : call.step ? stage(step) : stage(out))) return rc;
         from ^= 1;
         s = after;
     }
     return FSADAM_OK;
 }
 
-template <int SIDE>
 int run_residents(const Residents& r, const Call& call, void* workspace, hipStream_t stream) {
     if (r.rows.empty()) return FSADAM_OK;
     if (r.matrices > kMaxTiles) return fail(FSADAM_EINVAL, "the list has too many matrices for one call");
@@ -451,8 +454,8 @@ int run_residents(const Residents& r, const Call& call, void* workspace, hipStre
     auto launch = [&](const auto& table) {
         using Table = std::decay_t<decltype(table)>;
         const dim3 grid((uint32_t)r.matrices), block(kResidentThreads);
-        if (call.step) hipLaunchKernelGGL((fsadam_matrix_resident<SIDE, true, Table>), grid, block, r.lds_bytes, stream, table, k, call.momentum);
-        else hipLaunchKernelGGL((fsadam_matrix_resident<SIDE, false, Table>), grid, block, r.lds_bytes, stream, table, k, call.momentum);
+        if (call.step) hipLaunchKernelGGL((fsadam_matrix_resident<true, Table>), grid, block, r.lds_bytes, stream, table, k, call.momentum);
+        else hipLaunchKernelGGL((fsadam_matrix_resident<false, Table>), grid, block, r.lds_bytes, stream, table, k, call.momentum);
         return launched();
     };
     if (r.rows.size() <= kResidentRowsPerLaunch) {
@@ -480,10 +483,7 @@ int run_call(const Plan& plan, Call& call, void* workspace, int64_t workspace_by
     if (workspace_bytes < need)
         return fail(FSADAM_EINVAL, "the workspace holds " + std::to_string(workspace_bytes) + " bytes, this list needs " + std::to_string(need));
     hipStream_t stream = static_cast<hipStream_t>(hip_stream);
-    if ((rc = run_residents<2>(plan.residents[0], call, workspace, stream))) return rc;
-    if ((rc = run_residents<4>(plan.residents[1], call, workspace, stream))) return rc;
-    if ((rc = run_residents<6>(plan.residents[2], call, workspace, stream))) return rc;
-    if ((rc = run_residents<8>(plan.residents[3], call, workspace, stream))) return rc;
+    if ((rc = run_residents(plan.residents, call, workspace, stream))) return rc;
     for (const Chunk& c : chunks) {
         rc = run_chunk(c, call, workspace, stream);
         if (rc) return rc;

@@ -42,7 +42,7 @@ enum { kTypeF32 = 0, kTypeF16 = 1, kTypeBF16 = 2 };
 // Which of a row's tile counts a launch goes by.
 enum {
     kTilesSym64, kTilesFull64, kTilesGram64, kTilesSym128, kTilesFull128, kTilesGram128, kTilesSym256, kTilesFull256, kTilesGram256,
-    kTilesPart, kTilesJoin, kTilesPrep, kTilesChunk, kTileKinds
+    kTilesPart, kTilesAllParts, kTilesJoin, kTilesPrep, kTilesChunk, kTileKinds
 };
 
 // One row of a call's table: `batch` matrices of one shape, equally spaced.
@@ -526,7 +526,7 @@ __global__ __launch_bounds__(256) void fsadam_matrix_normalise(const MatrixRow* 
 
 // ---- the products -------------------------------------------------------------------------------------------------
 
-enum { kStagePart, kStageJoin, kStageGram, kStageSquare, kStageUpdate, kStageOut, kStageStep };
+enum { kStageJoin, kStageGram, kStageSquare, kStageUpdate, kStageOut, kStageStep };
 
 // Depth of a part of a Gram matrix's inner products, where they are split.
 constexpr int kPartDepth = 512;
@@ -537,6 +537,7 @@ struct StageArgs {
     float linear, product;  // result = linear * (what is added) + product * (accumulator), powers of two included
     float diagonal;     // square matrices: added on the diagonal
     float keep;         // step: 1 - lr * weight_decay
+    int kind;           // Gram matrix in tiles of 64: which tile counts the launch goes by
     int dst_type, copy_type;  // out, step: kType*; copy_type < 0: no copies
 };
 
@@ -759,7 +760,7 @@ __global__ __launch_bounds__(64 * WM * WN) void fsadam_matrix_stage(const Matrix
     constexpr int kLdsBytes = Prod::kLdsHalves * 2 > kSlab * kStride * 4 ? Prod::kLdsHalves * 2 : kSlab * kStride * 4;
     __shared__ __attribute__((aligned(1024))) unsigned char lds[kLdsBytes];
 
-    constexpr int kind = STAGE == kStagePart ? kTilesPart : STAGE == kStageJoin ? kTilesJoin
+    const int kind = STAGE == kStageGram && TM == 64 ? k.kind : STAGE == kStageJoin ? kTilesJoin
                          : (TM == 64 ? kTilesSym64 : TM == 128 ? kTilesSym128 : kTilesSym256) + (STAGE == kStageGram ? 2 : kSym ? 0 : 1);
     static_assert(kTilesFull64 == kTilesSym64 + 1 && kTilesGram64 == kTilesSym64 + 2 && kTilesGram128 == kTilesSym128 + 2 && kTilesGram256 == kTilesSym256 + 2);
     int matrix;
@@ -767,7 +768,7 @@ __global__ __launch_bounds__(64 * WM * WN) void fsadam_matrix_stage(const Matrix
     const MatrixRow& row = find_tile(table, n_rows, kind, xcd_contiguous(blockIdx.x, gridDim.x), matrix, tile);
     const int s64 = row.s64, l64 = row.l64;
     uint32_t part_of = 0;  // which part of a split inner product
-    if constexpr (STAGE == kStagePart) {
+    if constexpr (STAGE == kStageGram && TM == 64) {
         part_of = tile % (uint32_t)row.parts;
         tile /= (uint32_t)row.parts;
     }
@@ -790,19 +791,22 @@ __global__ __launch_bounds__(64 * WM * WN) void fsadam_matrix_stage(const Matrix
     Prod prod;
     // The partial sums of a split product, in the X buffer that the next update writes: tile by tile, part by part, every lane's
     // accumulators side by side.
-    float4_t* partial = nullptr;
-    if constexpr (STAGE == kStagePart || STAGE == kStageJoin) {
-        constexpr int kTile = TM * TN / 4;  // float4
-        partial = reinterpret_cast<float4_t*>(work + row.x_off[k.to] + (int64_t)matrix * 2 * plane_x) + ((int64_t)tile * row.parts + part_of) * kTile + threadIdx.x;
-    }
-    if constexpr (STAGE == kStagePart) {
-        const int from = (int)part_of * kPartDepth, depth = l64 - from < kPartDepth ? l64 - from : kPartDepth;
+    constexpr int kTile = TM * TN / 4;  // float4
+    auto partial = [&](int part) {
+        return reinterpret_cast<float4_t*>(work + row.x_off[k.to] + (int64_t)matrix * 2 * plane_x) + ((int64_t)tile * row.parts + part) * kTile + threadIdx.x;
+    };
+    if constexpr (STAGE == kStageGram && TM == 64) {
+        const int from = (int)part_of * kPartDepth, left = l64 - from;
+        const int depth = row.parts > 1 && left > kPartDepth ? kPartDepth : left;
         prod.run(x + (int64_t)i0 * l64 + from, l64, plane_x, s64 - i0, x + (int64_t)j0 * l64 + from, l64, plane_x, s64 - j0, depth, reinterpret_cast<_Float16*>(lds));
+        if (row.parts > 1) {
+            float4_t* to = partial((int)part_of);
 #pragma unroll
-        for (int i = 0; i < Prod::MI; ++i)
+            for (int i = 0; i < Prod::MI; ++i)
 #pragma unroll
-            for (int j = 0; j < Prod::NJ; ++j) partial[(i * Prod::NJ + j) * Prod::kThreads] = prod.acc[i][j];
-        return;
+                for (int j = 0; j < Prod::NJ; ++j) to[(i * Prod::NJ + j) * Prod::kThreads] = prod.acc[i][j];
+            return;
+        }
     } else if constexpr (STAGE == kStageJoin) {
 #pragma unroll
         for (int i = 0; i < Prod::MI; ++i)
@@ -813,7 +817,7 @@ __global__ __launch_bounds__(64 * WM * WN) void fsadam_matrix_stage(const Matrix
 #pragma unroll
             for (int i = 0; i < Prod::MI; ++i)
 #pragma unroll
-                for (int j = 0; j < Prod::NJ; ++j) prod.acc[i][j] += partial[n * (TM * TN / 4) + (i * Prod::NJ + j) * Prod::kThreads];
+                for (int j = 0; j < Prod::NJ; ++j) prod.acc[i][j] += partial(n)[(i * Prod::NJ + j) * Prod::kThreads];
     } else if constexpr (STAGE == kStageGram)
         prod.run(x + (int64_t)i0 * l64, l64, plane_x, s64 - i0, x + (int64_t)j0 * l64, l64, plane_x, s64 - j0, l64, reinterpret_cast<_Float16*>(lds));
     else if constexpr (STAGE == kStageSquare)
@@ -914,6 +918,21 @@ __global__ __launch_bounds__(64 * WM * WN) void fsadam_matrix_stage(const Matrix
                 // their rows at a time
                 const int64_t numel = (int64_t)row.rows * row.cols;
                 const float ratio = row.step_ratio;
+                if (row.tall) {  // a X + B X along the rows of X first, in the slab: its columns are what is written
+                    for (int e = threadIdx.x; e < kPieces; e += Prod::kThreads) {
+                        const int i = e / (TN / 8), j = (e % (TN / 8)) * 8;
+                        if (j0 + j >= l64) continue;
+                        float o[8], w[8];
+                        along_row(i, j, o);
+                        load_planes<2>(x + (int64_t)(r0 + i) * l64 + j0 + j, plane_x, w);
+#pragma unroll
+                        for (int q = 0; q < 8; ++q) o[q] = k.linear * w[q] + k.product * o[q];
+                        float4_t* to = reinterpret_cast<float4_t*>(at_slab(i, j));
+                        to[0] = float4_t{o[0], o[1], o[2], o[3]};
+                        to[1] = float4_t{o[4], o[5], o[6], o[7]};
+                    }
+                    __syncthreads();
+                }
                 for (int e = threadIdx.x; e < kPieces; e += Prod::kThreads) {
                     int i, j;
                     float o[8], w[8];
@@ -922,18 +941,15 @@ __global__ __launch_bounds__(64 * WM * WN) void fsadam_matrix_stage(const Matrix
                         i = (e % (kSlab / 8)) * 8;
                         if (r0 + i >= row.s || j0 + j >= row.l) continue;
                         along_column(i, j, o);
-                        const _Float16* from = x + (int64_t)(r0 + i) * l64 + j0 + j;
-#pragma unroll
-                        for (int q = 0; q < 8; ++q) w[q] = (float)from[(int64_t)q * l64] + (float)from[plane_x + (int64_t)q * l64];
                     } else {
                         i = e / (TN / 8);
                         j = (e % (TN / 8)) * 8;
                         if (r0 + i >= row.s || j0 + j >= row.l) continue;
                         along_row(i, j, o);
                         load_planes<2>(x + (int64_t)(r0 + i) * l64 + j0 + j, plane_x, w);
-                    }
 #pragma unroll
-                    for (int q = 0; q < 8; ++q) o[q] = k.linear * w[q] + k.product * o[q];
+                        for (int q = 0; q < 8; ++q) o[q] = k.linear * w[q] + k.product * o[q];
+                    }
                     const int64_t r = row.tall ? j0 + j : r0 + i, c = row.tall ? r0 + i : j0 + j;
                     const int left = row.cols - (int)c;  // elements of the row from here on
                     if constexpr (STAGE == kStageOut) {
@@ -1004,21 +1020,9 @@ __host__ __device__ constexpr bool resident_fits(int64_t s, int64_t l) {
 
 // SIDE: the short side in tiles of 16, padded to 32: 2, 4, 6 or 8.  A constant, so that the addresses of the square matrix's tiles
 // are one register and offsets in the instructions.
-template <int SIDE, bool STEP, typename Table>
-__global__ __launch_bounds__(kResidentThreads) void fsadam_matrix_resident(Table tables, ResidentArgs k, MomentumArgs mk) {
-    extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
-    __shared__ double part[kResidentWaves];
-    const ResidentRow* table = rows_of(tables);
-    int low = 0, high = tables.n - 1;
-    while (low < high) {
-        const int mid = (low + high + 1) >> 1;
-        if (table[mid].first_matrix <= (int)blockIdx.x) low = mid;
-        else high = mid - 1;
-    }
-    const ResidentRow row = table[low];
-    // The arguments of a launch are not in the GPU's memory: the factors of all steps are fetched together, once.
-    __shared__ float factors[5][kMaxSteps];
-    if (threadIdx.x < 5 * kMaxSteps) (&factors[0][0])[threadIdx.x] = (&k.factors[0][0])[threadIdx.x];
+template <int SIDE, bool STEP>
+__device__ __forceinline__ void resident_matrix(const ResidentRow& row, const ResidentArgs& k, const MomentumArgs& mk, unsigned char* lds, double* part,
+                                                const float (*factors)[kMaxSteps]) {
     const int steps = k.steps, src_type = k.src_type, dst_type = k.dst_type, copy_type = k.copy_type;
     const float keep = k.keep;
     const int64_t matrix = (int)blockIdx.x - row.first_matrix;
@@ -1274,6 +1278,29 @@ __global__ __launch_bounds__(kResidentThreads) void fsadam_matrix_resident(Table
                 __builtin_amdgcn_sched_barrier(0);  // one tile's addresses at a time: the registers do not hold those of eight
             });
         }
+    }
+}
+
+template <bool STEP, typename Table>
+__global__ __launch_bounds__(kResidentThreads) void fsadam_matrix_resident(Table tables, ResidentArgs k, MomentumArgs mk) {
+    extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
+    __shared__ double part[kResidentWaves];
+    const ResidentRow* table = rows_of(tables);
+    int low = 0, high = tables.n - 1;
+    while (low < high) {
+        const int mid = (low + high + 1) >> 1;
+        if (table[mid].first_matrix <= (int)blockIdx.x) low = mid;
+        else high = mid - 1;
+    }
+    const ResidentRow row = table[low];
+    // The arguments of a launch are not in the GPU's memory: the factors of all steps are fetched together, once.
+    __shared__ float factors[5][kMaxSteps];
+    if (threadIdx.x < 5 * kMaxSteps) (&factors[0][0])[threadIdx.x] = (&k.factors[0][0])[threadIdx.x];
+    switch (((row.rows < row.cols ? row.rows : row.cols) + 31) / 32) {
+        case 1: resident_matrix<2, STEP>(row, k, mk, lds, part, factors); break;
+        case 2: resident_matrix<4, STEP>(row, k, mk, lds, part, factors); break;
+        case 3: resident_matrix<6, STEP>(row, k, mk, lds, part, factors); break;
+        default: resident_matrix<8, STEP>(row, k, mk, lds, part, factors); break;
     }
 }
 

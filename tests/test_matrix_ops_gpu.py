@@ -542,3 +542,15 @@ def test_same_inputs_give_the_same_bits():
     for _ in range(3):
         assert all(torch.equal(a, b) for a, b in zip(first, orthogonalize(us)))
     gc.collect()
+
+
+@pytest.mark.parametrize("products", ["half", "split"])
+@pytest.mark.parametrize("others", [[(1100, 1024)] * 30, [(4096, 2048)] * 12, [(5, 7)]], ids=["30_of_1100", "12_of_4096", "small"])
+def test_what_a_matrix_gives_does_not_depend_on_the_list(products, others):
+    """The list decides the tiles (64, 128 or 256) of every launch, and so which of them run into the ends of the matrix."""
+    us = [randn(700, 900), randn(901, 640), randn(333, 2049), randn(130, 4100), randn(64, 256), randn(200, 130), randn(2, 310, 515)]
+    alone = [orthogonalize([u], products=products)[0] for u in us]
+    rest = [randn(*others[0], seed=9)] * len(others)
+    for k, (a, b) in enumerate(zip(alone, orthogonalize(us + rest, products=products))):
+        assert torch.equal(a, b), us[k].shape
+    check_orth(us, alone, products)
