@@ -59,25 +59,25 @@ constexpr int64_t kChunkBytes = int64_t(4) << 30;
 
 // ---- numbers of the iteration -------------------------------------------------------------------------------------
 
-// Largest magnitude of c[0] + c[1] t + ... + c[n] t^n on [0, top]: at the ends, or where the derivative vanishes (found by
-// bisection between samples where it changes sign; the polynomials are of low degree and far from the bounds).
-double largest(const double* c, int n, double top) {
-    auto value = [&](double t) { double v = 0.0; for (int i = n; i >= 0; --i) v = v * t + c[i]; return v; };
-    auto slope = [&](double t) { double v = 0.0; for (int i = n; i >= 1; --i) v = v * t + i * c[i]; return v; };
-    constexpr int kSamples = 32;
-    double most = std::max(std::fabs(value(0.0)), std::fabs(value(top)));
-    for (int i = 0; i < kSamples; ++i) {
-        double low = top * i / kSamples, high = top * (i + 1) / kSamples;
-        most = std::max(most, std::fabs(value(low)));
-        if ((slope(low) < 0.0) == (slope(high) < 0.0)) continue;
-        const bool down = slope(low) < 0.0;
-        for (int k = 0; k < 30; ++k) {
-            const double mid = 0.5 * (low + high);
-            if ((slope(mid) < 0.0) == down) low = mid;
-            else high = mid;
-        }
-        most = std::max(most, std::fabs(value(low)));
+// Where u + v t + w t^2 vanishes: up to two values of t, NaN where there are fewer.
+void roots(double u, double v, double w, double (&t)[2]) {
+    t[0] = t[1] = std::nan("");
+    if (w == 0.0) {
+        if (v != 0.0) t[0] = -u / v;
+        return;
     }
+    const double d = v * v - 4.0 * u * w;
+    if (d < 0.0) return;
+    const double h = -0.5 * (v + std::copysign(std::sqrt(d), v));  // no cancellation: the other root is u / h
+    t[0] = h / w;
+    t[1] = h != 0.0 ? u / h : 0.0;
+}
+// Largest |f(t)| on [0, top]: at the ends, or at `at` (where its derivative vanishes).
+template <typename F>
+double largest(const F& f, double top, const double (&at)[2]) {
+    double most = std::max(std::fabs(f(0.0)), std::fabs(f(top)));
+    for (double t : at)
+        if (t > 0.0 && t < top) most = std::max(most, std::fabs(f(t)));
     return most;
 }
 
@@ -95,15 +95,21 @@ int exponent_for(double bound) {  // the largest k with bound * 2^k <= 60000 (ha
 // How large the eigenvalues of those matrices can be at every step, when the singular values of X0 are in [0, 1].  2 % a step stands
 // for what rounding adds.
 int step_bounds(const FsOrthOptions& o, std::vector<StepNumbers>& numbers) {
-    const double q[] = {o.a, o.b, o.c}, b[] = {0.0, o.b, o.c}, t[] = {0.0, o.a, o.b, o.c};
-    const double p2[] = {0.0, q[0] * q[0], 2 * q[0] * q[1], q[1] * q[1] + 2 * q[0] * q[2], 2 * q[1] * q[2], q[2] * q[2]};  // t q(t)^2: the next t
+    const double a = o.a, b = o.b, c = o.c;
+    const auto q = [&](double t) { return a + t * (b + t * c); };
+    double q_flat[2], t_flat[2], p_flat[2];
+    roots(b, 2.0 * c, 0.0, q_flat);          // of q and of b t + c t^2
+    roots(a, 2.0 * b, 3.0 * c, t_flat);      // of t q(t)
+    roots(a, 3.0 * b, 5.0 * c, p_flat);      // of t q(t)^2, but for the zeros of q
     numbers.clear();
     double m = 1.0;
     for (int k = 0; k < o.steps; ++k) {
         m *= 1.02;
         StepNumbers n;
-        const double top = m * m, most_q = largest(q, 2, top), most_b = largest(b, 2, top), most_t = largest(t, 3, top);
-        m = std::sqrt(largest(p2, 5, top));
+        const double top = m * m, most_q = largest(q, top, q_flat);
+        const double most_b = largest([&](double t) { return t * (b + t * c); }, top, q_flat);
+        const double most_t = largest([&](double t) { return t * q(t); }, top, t_flat);
+        m = std::sqrt(largest([&](double t) { return t * q(t) * q(t); }, top, p_flat));
         if (!(m <= 1024.0))
             return fail(FSADAM_EINVAL, "the coefficients let singular values in [0, 1] grow past 1024 by step " + std::to_string(k + 1));
         n.x = exponent_for(std::sqrt(top));

@@ -15,6 +15,7 @@
 
 #include <cstdint>
 #include <string>
+#include <unordered_set>
 
 namespace py = pybind11;
 
@@ -293,6 +294,57 @@ py::tuple fill_grad_rows(py::list grads, int dtype_code, int device, uintptr_t r
     return as_tuple(r);
 }
 
+// Rows of the matrix operators (include/fsadam.h: FsMomentumTensor, FsMuonTensor): `words` int64 a row, the pointers of the
+// lists' tensors first (0 where a list is None), then, for FsMomentumTensor, numel.  Tensors of a row are dense, contiguous, on one
+// device and of one shape; those of the lists named in `written` do not share memory with another of their list.
+// dtype codes: 0 float32, 1 float16, 2 bfloat16.
+//
+// fill_matrix_rows(lists, dtype_codes, written, device_index, rows_address, words, with_numel) -> (status, list, index, None)
+py::tuple fill_matrix_rows(py::tuple lists, py::tuple dtype_codes, py::tuple written, int device, uintptr_t rows_address, int64_t words, bool with_numel) {
+    Result r;
+    const int64_t depth = (int64_t)py::len(lists);
+    auto stop = [&](int status, int64_t list, int64_t index) {
+        r.status = status;
+        r.list = list;
+        r.index = index;
+        return as_tuple(r);
+    };
+    if (depth < 1 || depth > 4 || (int64_t)py::len(dtype_codes) != depth || !PyList_Check(PyTuple_GET_ITEM(lists.ptr(), 0)) || !rows_address || words < depth + 1)
+        return stop(kLength, 0, -1);
+    const int64_t n = PyList_GET_SIZE(PyTuple_GET_ITEM(lists.ptr(), 0));
+    int64_t* rows = reinterpret_cast<int64_t*>(rows_address);
+    try {
+        std::unordered_set<const void*> seen;
+        for (int64_t d = 0; d < depth; ++d) {
+            PyObject* lst = PyTuple_GET_ITEM(lists.ptr(), d);
+            if (lst == Py_None) {
+                for (int64_t t = 0; t < n; ++t) rows[t * words + d] = 0;
+                continue;
+            }
+            if (!PyList_Check(lst) || PyList_GET_SIZE(lst) != n) return stop(kLength, d, -1);
+            const int code = dtype_codes[d].cast<int>();
+            const c10::ScalarType dtype = code == 2 ? c10::ScalarType::BFloat16 : dtype_of_code(code);
+            const bool unshared = written.contains(py::int_(d));
+            seen.clear();
+            for (int64_t t = 0; t < n; ++t) {
+                const at::Tensor* x = plain_tensor(PyList_GET_ITEM(lst, t));
+                const at::Tensor* x0 = plain_tensor(PyList_GET_ITEM(PyTuple_GET_ITEM(lists.ptr(), 0), t));
+                if (!x || !x0) return stop(kNotTensor, d, t);
+                const int bad = check_tensor(*x, dtype, device, x0->numel());
+                if (bad) return stop(bad, d, t);
+                if (x->sizes() != x0->sizes()) return stop(kNumel, d, t);
+                if (unshared && x->numel() && !seen.insert(x->data_ptr()).second) return stop(kStale, d, t);
+                rows[t * words + d] = reinterpret_cast<int64_t>(x->data_ptr());
+                if (d == 0 && with_numel) rows[t * words + depth] = x->numel();
+            }
+        }
+    } catch (const std::exception& e) {
+        r.status = kError;
+        return as_tuple(r, py::str(e.what()));
+    }
+    return as_tuple(r);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_tensor_rows, m) {
@@ -300,6 +352,7 @@ PYBIND11_MODULE(_tensor_rows, m) {
     m.def("fill_rows", &fill_rows);
     m.def("gather", &gather);
     m.def("fill_grad_rows", &fill_grad_rows);
+    m.def("fill_matrix_rows", &fill_matrix_rows);
     m.attr("UNCHANGED") = (int)kUnchanged;
     m.attr("CHANGED") = (int)kChanged;
     m.attr("NOT_TENSOR") = (int)kNotTensor;

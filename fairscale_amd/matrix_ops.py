@@ -11,9 +11,10 @@ from __future__ import annotations
 import ctypes
 from typing import List, NamedTuple, Optional, Sequence, Tuple, Union
 
+import numpy as np
 import torch
 
-from . import _cabi
+from . import _cabi, _rows
 
 __all__ = ["MomentumStats", "momentum_pass", "orthogonalize"]
 
@@ -67,6 +68,34 @@ def refuse_shared(tensors: Sequence[torch.Tensor], what: str) -> None:
             seen.add(t.data_ptr())
 
 
+def fill_rows(lists: Sequence[Optional[List[torch.Tensor]]], dtypes: Sequence[torch.dtype], written: Tuple[int, ...], device: torch.device,
+              rows: np.ndarray, with_numel: bool = False) -> bool:
+    """The lists' pointers into ``rows``, with every check that can be made of them, in one C++ loop.  False when the helper is not
+    built or found something to refuse: the Python checks of the caller then name it."""
+    native = _rows.native
+    return native is not None and native.fill_matrix_rows(tuple(lists), tuple(TYPE_CODE[d] for d in dtypes), written, device.index,
+                                                          rows.ctypes.data, rows.shape[1], with_numel)[0] >= 0
+
+
+def rows_pointer(rows: np.ndarray, row_type):
+    return ctypes.cast(rows.ctypes.data, ctypes.POINTER(row_type))
+
+
+def _check_momentum_lists(grads, momenta, updates, device, dtype, update_dtype) -> None:
+    for g, m in zip(grads, momenta):
+        if g.device != device or g.dtype != dtype or m.device != device:
+            raise RuntimeError("gradients of one pass must share dtype, and device with their momenta")
+        if g.layout != torch.strided or m.layout != torch.strided or not g.is_contiguous() or not m.is_contiguous():
+            raise RuntimeError("gradients and momenta must be dense, contiguous device tensors")
+        if m.dtype != torch.float32 or m.shape != g.shape:
+            raise RuntimeError("momenta must be float32 tensors of the gradients' shapes")
+    for g, u in zip(grads, updates):
+        if u.dtype != update_dtype or u.device != device or u.shape != g.shape or u.layout != torch.strided or not u.is_contiguous():
+            raise RuntimeError("updates must be dense, contiguous tensors of one dtype with the gradients' shapes and device")
+    refuse_shared(momenta, "momenta")
+    refuse_shared(updates, "updates")
+
+
 @torch.no_grad()
 def momentum_pass(grads: Sequence[torch.Tensor], momenta: Sequence[torch.Tensor], momentum: float = 0.95, *, nesterov: bool = True,
                   scale: Union[float, torch.Tensor] = 1.0, updates: Optional[Sequence[torch.Tensor]] = None,
@@ -94,36 +123,28 @@ def momentum_pass(grads: Sequence[torch.Tensor], momenta: Sequence[torch.Tensor]
         raise RuntimeError(f"gradients must be float32, float16 or bfloat16, got {dtype}")
     if device.type != "cuda":
         raise RuntimeError("gradients must be dense, contiguous device tensors")
-    for g, m in zip(grads, momenta):
-        if g.device != device or g.dtype != dtype or m.device != device:
-            raise RuntimeError("gradients of one pass must share dtype, and device with their momenta")
-        if g.layout != torch.strided or m.layout != torch.strided or not g.is_contiguous() or not m.is_contiguous():
-            raise RuntimeError("gradients and momenta must be dense, contiguous device tensors")
-        if m.dtype != torch.float32 or m.shape != g.shape:
-            raise RuntimeError("momenta must be float32 tensors of the gradients' shapes")
     if updates is None:
         updates = [torch.empty_like(g, memory_format=torch.contiguous_format) for g in grads]
     updates = list(updates)
     update_dtype = updates[0].dtype
     if update_dtype not in TYPE_CODE:
         raise RuntimeError(f"updates must be float32, float16 or bfloat16, got {update_dtype}")
-    for g, u in zip(grads, updates):
-        if u.dtype != update_dtype or u.device != device or u.shape != g.shape or u.layout != torch.strided or not u.is_contiguous():
-            raise RuntimeError("updates must be dense, contiguous tensors of one dtype with the gradients' shapes and device")
-    refuse_shared(momenta, "momenta")
-    refuse_shared(updates, "updates")
+    rows = np.empty((len(grads), 4), dtype=np.int64)
+    if not fill_rows((grads, momenta, updates), (dtype, torch.float32, update_dtype), (1, 2), device, rows, True):
+        _check_momentum_lists(grads, momenta, updates, device, dtype, update_dtype)
+        rows[:] = [(g.data_ptr(), m.data_ptr(), u.data_ptr(), g.numel()) for g, m, u in zip(grads, momenta, updates)]
     if found_inf is None:
         found_inf = torch.zeros(1, dtype=torch.float32, device=device)
     elif found_inf.dtype != torch.float32 or found_inf.device != device or found_inf.numel() != 1:
         raise RuntimeError("found_inf must be a float32 tensor with one element on the gradients' device")
     value, pointer = scale_arguments(scale, device)
-    rows = (_cabi.FsMomentumTensor * len(grads))(*[(g.data_ptr(), m.data_ptr(), u.data_ptr(), g.numel()) for g, m, u in zip(grads, momenta, updates)])
     lib = _cabi.lib()
+    pointer_to_rows = rows_pointer(rows, _cabi.FsMomentumTensor)
     with torch.cuda.device(device):
-        workspace, size = workspace_for(lib.fsadam_momentum_workspace, device, rows, len(grads))
+        workspace, size = workspace_for(lib.fsadam_momentum_workspace, device, pointer_to_rows, len(grads))
         norms = torch.empty(len(grads), dtype=torch.float32, device=device)
         _cabi.check(lib.fsadam_momentum_pass(
-            rows, len(grads), TYPE_CODE[dtype], TYPE_CODE[update_dtype], float(momentum), 1 if nesterov else 0, value, pointer,
+            pointer_to_rows, len(grads), TYPE_CODE[dtype], TYPE_CODE[update_dtype], float(momentum), 1 if nesterov else 0, value, pointer,
             norms.data_ptr(), found_inf.data_ptr(), workspace.data_ptr(), size, int(torch.cuda.current_stream(device).cuda_stream)))
     return MomentumStats(updates, norms, found_inf)
 

@@ -11,13 +11,16 @@ import ctypes
 import math
 from typing import Any, Callable, Dict, List, Optional, Sequence, Tuple, Union
 
+import numpy as np
 import torch
 
 from .. import _cabi
-from ..matrix_ops import NS_COEFFICIENTS, TYPE_CODE, orth_options, refuse_shared, scale_arguments, workspace_for
+from ..matrix_ops import NS_COEFFICIENTS, TYPE_CODE, fill_rows, orth_options, refuse_shared, rows_pointer, scale_arguments, workspace_for
 from .adam import Precision
 
 __all__ = ["Muon"]
+
+_SETTINGS = ("lr", "weight_decay", "momentum", "nesterov", "ns_coefficients", "eps", "ns_steps", "adjust_lr_fn", "row_blocks")
 
 
 class Muon(torch.optim.Optimizer):
@@ -94,7 +97,12 @@ class Muon(torch.optim.Optimizer):
 
     # ------------------------------------------------------------------ groups and state
 
-    def _check_group(self, group: Dict[str, Any]) -> None:
+    def _check_group(self, group: Dict[str, Any], step: bool = False) -> None:
+        """Raises ValueError for settings the step cannot take; before a step only when they changed since they were looked at."""
+        settings = tuple(group[name] for name in _SETTINGS) + (self.products,)
+        checked = self.__dict__.setdefault("_checked", {})
+        if step and checked.get(id(group)) == settings:
+            return
         if not 0.0 <= group["lr"] < math.inf:
             raise ValueError(f"Invalid learning rate: {group['lr']}")
         if not 0.0 <= group["weight_decay"] < math.inf:
@@ -119,6 +127,7 @@ class Muon(torch.optim.Optimizer):
                 raise ValueError(f"Muon optimizes matrices, got a parameter of shape {tuple(p.shape)} (Adam takes it)")
             if p.shape[-2] % blocks:
                 raise ValueError(f"{p.shape[-2]} rows cannot be split into {blocks} blocks")
+        checked[id(group)] = settings
 
     def _add_masters(self, group: Dict[str, Any]) -> None:
         masters = []
@@ -160,35 +169,73 @@ class Muon(torch.optim.Optimizer):
 
     # ------------------------------------------------------------------ the step
 
-    def _gather(self, gi: int, group: Dict[str, Any]) -> Dict[torch.device, List[Tuple]]:
-        """(parameter or master, gradient, momentum, copy, ratio) of what takes part, by device.  Raises before anything is changed
-        but for momenta that are made."""
-        batches: Dict[torch.device, List[Tuple]] = {}
+    def _gather(self, gi: int, group: Dict[str, Any]) -> Dict[torch.device, Tuple[List[torch.Tensor], ...]]:
+        """(parameters or masters, gradients, momenta, copies) of what takes part, by device.  Changes nothing but for momenta that are made."""
+        batches: Dict[torch.device, Tuple[List[torch.Tensor], ...]] = {}
         masters = self.fp32_param_groups[gi]["params"] if self.mixed_precision else None
         for k, p in enumerate(group["params"]):
             grad = p.grad
             if grad is None:
                 continue
-            if grad.layout != torch.strided:
-                raise RuntimeError("Muon does not support sparse gradients")
-            if not p.is_cuda or not p.is_contiguous() or not grad.is_contiguous() or grad.device != p.device:
-                raise RuntimeError("parameters and gradients must be dense, contiguous tensors on one device each")
-            if grad.dtype != p.dtype or grad.shape != p.shape:
-                raise RuntimeError("gradients must have their parameter's dtype and shape")
-            if p.dtype != self._dtype:
-                raise RuntimeError(f"a parameter has changed its dtype from {self._dtype} to {p.dtype}")
             state = self.state[p]
-            if state.get("momentum_buffer") is None:
+            buf = state.get("momentum_buffer")
+            if buf is None:
+                self._check_row(p, p, grad, None)
                 if torch.cuda.is_current_stream_capturing():
                     raise RuntimeError("a graph that makes the momentum would clear it at every replay: step once before the capture")
-                state["momentum_buffer"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
-            buf = state["momentum_buffer"]
-            master = masters[k] if masters is not None else None
-            for t in (buf, master):
-                if t is not None and (t.dtype != torch.float32 or t.device != p.device or t.shape != p.shape or not t.is_contiguous()):
-                    raise RuntimeError("momentum and master copies must be contiguous float32 tensors with their parameter's shape and device")
-            batches.setdefault(p.device, []).append((p if master is None else master, grad, buf, p if master is not None else None))
+                buf = state["momentum_buffer"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
+            lists = batches.get(p.device)
+            if lists is None:
+                lists = batches[p.device] = ([], [], [], [])
+            lists[0].append(p if masters is None else masters[k])
+            lists[1].append(grad)
+            lists[2].append(buf)
+            lists[3].append(p)
         return batches
+
+    def _check_row(self, p: torch.Tensor, like: torch.Tensor, grad: torch.Tensor, buf: Optional[torch.Tensor]) -> None:
+        """What the kernels rely on, by name (the native walk checks the same of all rows in one loop)."""
+        if grad.layout != torch.strided:
+            raise RuntimeError("Muon does not support sparse gradients")
+        if not like.is_cuda or not like.is_contiguous() or not grad.is_contiguous() or grad.device != like.device:
+            raise RuntimeError("parameters and gradients must be dense, contiguous tensors on one device each")
+        if grad.dtype != like.dtype or grad.shape != like.shape:
+            raise RuntimeError("gradients must have their parameter's dtype and shape")
+        if like.dtype != self._dtype:
+            raise RuntimeError(f"a parameter has changed its dtype from {self._dtype} to {like.dtype}")
+        for t in ((buf,) if p is like else (buf, p)):
+            if t is not None and (t.dtype != torch.float32 or t.device != like.device or t.shape != like.shape or not t.is_contiguous()):
+                raise RuntimeError("momentum and master copies must be contiguous float32 tensors with their parameter's shape and device")
+
+    def _rows(self, group: Dict[str, Any], device: torch.device, lists: Tuple[List[torch.Tensor], ...]) -> np.ndarray:
+        """FsMuonTensor rows of one call."""
+        params, grads, bufs, likes = lists
+        blocks, how = int(group["row_blocks"]), group["adjust_lr_fn"]
+        rows = np.empty((len(params), 8), dtype=np.int64)
+        copies = likes if self.mixed_precision else None
+        stored = torch.float32 if self.mixed_precision else self._dtype
+        if device.type != "cuda" or not fill_rows((params, grads, bufs, copies), (stored, self._dtype, torch.float32, self._dtype), (0, 2), device, rows):
+            for p, like, grad, buf in zip(params, likes, grads, bufs):
+                self._check_row(p, like, grad, buf)
+            refuse_shared(params, "parameters")
+            refuse_shared(bufs, "momenta")
+            rows[:, :4] = [(p.data_ptr(), g.data_ptr(), m.data_ptr(), c.data_ptr() if copies else 0) for p, g, m, c in zip(params, grads, bufs, likes)]
+        # batch, rows, cols and ratio go by the shapes alone
+        shapes = (blocks, how, tuple(p.shape for p in params))
+        cached = self.__dict__.setdefault("_geometry", {}).get(id(group))
+        if cached is None or cached[0] != shapes:
+            cells = np.empty((len(params), 4), dtype=np.int64)
+            ratios = cells.view(np.float64)
+            for k, p in enumerate(params):
+                height, cols = p.shape[-2] // blocks, p.shape[-1]
+                cells[k, :3] = p.numel() // (height * cols) if p.numel() else 0, height, cols
+                if how == "match_rms_adamw":
+                    ratios[k, 3] = 0.2 * math.sqrt(max(height, cols))
+                else:
+                    ratios[k, 3] = math.sqrt(max(1.0, height / cols)) if cols else 1.0
+            cached = self._geometry[id(group)] = (shapes, cells)
+        rows[:, 4:] = cached[1]
+        return rows
 
     def step(self, closure: Optional[Callable[[], float]] = None, *, scale: Union[float, torch.Tensor] = 1.0) -> Optional[float]:
         """One optimization step.
@@ -203,33 +250,26 @@ class Muon(torch.optim.Optimizer):
         loss = closure() if closure is not None else None
         calls = []
         for gi, group in enumerate(self.param_groups):
-            self._check_group(group)
-            for device, batch in self._gather(gi, group).items():
-                refuse_shared([row[0] for row in batch], "parameters")
-                refuse_shared([row[2] for row in batch], "momenta")
-                calls.append((group, device, batch, *scale_arguments(scale, device)))
-        with torch.autograd.profiler.record_function("fairscale_amd::muon::fused_step"):
+            self._check_group(group, step=True)
+            for device, lists in self._gather(gi, group).items():
+                calls.append((group, device, self._rows(group, device, lists), *scale_arguments(scale, device)))
+        if torch.autograd._profiler_enabled():
+            with torch.autograd.profiler.record_function("fairscale_amd::muon::fused_step"):
+                for call in calls:
+                    self._launch(*call)
+        else:
             for call in calls:
                 self._launch(*call)
         return loss
 
-    def _launch(self, group: Dict[str, Any], device: torch.device, batch: List[Tuple], scale: float, scale_pointer: Optional[int]) -> None:
-        blocks = int(group["row_blocks"])
-        rows = (_cabi.FsMuonTensor * len(batch))()
-        for row, (p, g, m, copy) in zip(rows, batch):
-            height, cols = p.shape[-2] // blocks, p.shape[-1]
-            row.p, row.g, row.m, row.p_copy = p.data_ptr(), g.data_ptr(), m.data_ptr(), None if copy is None else copy.data_ptr()
-            row.batch, row.rows, row.cols = (p.numel() // (height * cols) if p.numel() else 0), height, cols
-            if group["adjust_lr_fn"] == "match_rms_adamw":
-                row.ratio = 0.2 * math.sqrt(max(height, cols))
-            else:
-                row.ratio = math.sqrt(max(1.0, height / cols)) if cols else 1.0
+    def _launch(self, group: Dict[str, Any], device: torch.device, rows: np.ndarray, scale: float, scale_pointer: Optional[int]) -> None:
         options = orth_options(group["ns_steps"], group["ns_coefficients"], group["eps"], self.products)
         code = TYPE_CODE[self._dtype]
         lib = _cabi.lib()
-        with torch.cuda.device(device), torch.no_grad():
-            workspace, size = workspace_for(lib.fsadam_muon_workspace, device, rows, len(batch), ctypes.byref(options))
+        pointer = rows_pointer(rows, _cabi.FsMuonTensor)
+        with torch.cuda.device(device):
+            workspace, size = workspace_for(lib.fsadam_muon_workspace, device, pointer, len(rows), ctypes.byref(options))
             _cabi.check(lib.fsadam_muon_step(
-                rows, len(batch), _cabi.TYPE_F32 if self.mixed_precision else code, code, code if self.mixed_precision else -1, ctypes.byref(options),
+                pointer, len(rows), _cabi.TYPE_F32 if self.mixed_precision else code, code, code if self.mixed_precision else -1, ctypes.byref(options),
                 float(group["lr"]), float(group["momentum"]), 1 if group["nesterov"] else 0, float(group["weight_decay"]), scale, scale_pointer,
                 workspace.data_ptr(), size, int(torch.cuda.current_stream(device).cuda_stream)))
