@@ -56,6 +56,7 @@ struct alignas(16) MatrixRow {
     int64_t sq_off[3]; // workspace: square matrices (A and B; a pair of steps uses all three)
     int32_t batch, rows, cols;
     int32_t s, l, s64, l64;
+    int32_t ld_x, ld_a;             // elements from row to row of X and of the square matrices
     int32_t tall;      // rows > cols: X is the transpose
     int32_t first_matrix;           // index of the row's first matrix in the chunk
     int32_t chunks;                 // partial sums per matrix
@@ -481,9 +482,9 @@ __global__ __launch_bounds__(256) void fsadam_matrix_normalise(const MatrixRow* 
     const int r0 = row.tall ? j0 : i0, c0 = row.tall ? i0 : j0;         // in the source
     const double factor = inverse[row.first_matrix + matrix] * power;
     const Divisor by(k);
-    const int64_t plane = (int64_t)row.s64 * row.l64;
+    const int64_t plane = (int64_t)row.s64 * row.ld_x;
     _Float16* x = work + row.x_off[0] + (int64_t)matrix * 2 * plane;
-    auto put = [&](int i, int j, const float (&v)[8]) { store_planes<2>(x + (int64_t)(i0 + i) * row.l64 + j0 + j, plane, v); };
+    auto put = [&](int i, int j, const float (&v)[8]) { store_planes<2>(x + (int64_t)(i0 + i) * row.ld_x + j0 + j, plane, v); };
 #pragma unroll
     for (int part = 0; part < 2; ++part) {
         const int e = threadIdx.x + part * 256, r = e >> 3, c = (e & 7) * 8;  // eight neighbours in the source
@@ -706,7 +707,48 @@ struct Product {
                 }
         };
         const _Float16* now = lds;
-        if constexpr (kAhead) {
+        if constexpr (kWaves == 8 && PLANES == 2) {
+            // (22 bits: 1.86 -> 1.79 ms on the update of 5120 x 13824.  With 11 bits the loads are the longer part, and two waves of a SIMD
+            // in step, each a slice ahead of itself, are faster: 1.69 against 1.83 ms on a layer of the 7B list.)
+            // Two groups of four waves, one of each on every SIMD, half a slice apart: while one multiplies, the other reads its
+            // operands and sends for the next panel, so that the matrix cores always have a wave that has nothing else to do.
+            // Time goes in ticks between barriers.  Group 0 reads slice j in tick 2j and multiplies it in 2j + 1, group 1 a tick
+            // later.  A panel of S slices is read for the last time (by group 1) in the tick before group 0 reads the first slice of the
+            // next: from that tick on its buffer may be filled again, and both groups send for the panel after next in it, group 0 as
+            // it reads, group 1 as it multiplies.  Before group 0 reads a panel, every wave has waited for its own loads of it and passed a barrier:
+            // group 0 after multiplying the last slice of the panel before, group 1 after reading it.
+            static_assert(DEPTH == 2, "two buffers");
+            const bool late = wave >= 4;
+            auto tick = [] {
+                __builtin_amdgcn_sched_barrier(0);
+                asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+                __builtin_amdgcn_sched_barrier(0);
+            };
+            loads_arrived<0>();
+            tick();
+            if (late) {
+                if (n_k > 1) fetch(lds_at + kStageHalves * 2);
+                tick();
+            }
+            for (int panel = 0; panel < n_k; ++panel) {
+                const _Float16* here = lds + (panel & 1) * kStageHalves;
+#pragma unroll
+                for (int kk = 0; kk < kSlices; ++kk) {
+                    Slice f;
+                    read(f, here, kk);
+                    if (kk == 0 && !late && panel + 1 < n_k) fetch(lds_at + ((panel + 1) & 1) * kStageHalves * 2);
+                    if (kk == kSlices - 1 && late) loads_arrived<0>();
+                    tick();
+                    if (kk == kSlices - 1 && late && panel + 2 < n_k) fetch(lds_at + (panel & 1) * kStageHalves * 2);
+                    __builtin_amdgcn_s_setprio(1);
+                    multiply(f);
+                    __builtin_amdgcn_s_setprio(0);
+                    if (kk == kSlices - 1 && !late) loads_arrived<0>();
+                    tick();
+                }
+            }
+            if (!late) tick();
+        } else if constexpr (kAhead) {
             // the next slice is read while this one is multiplied, across the barrier between panels too
             constexpr int kReads = PLANES * (MI + NJ * (NN ? 2 : 1)), kProducts = MI * NJ * (PLANES == 2 ? 3 : 1);
             Slice f[2];
@@ -766,7 +808,7 @@ __global__ __launch_bounds__(64 * WM * WN) void fsadam_matrix_stage(const Matrix
     int matrix;
     uint32_t tile;
     const MatrixRow& row = find_tile(table, n_rows, kind, xcd_contiguous(blockIdx.x, gridDim.x), matrix, tile);
-    const int s64 = row.s64, l64 = row.l64;
+    const int s64 = row.s64, l64 = row.l64, ld_x = row.ld_x, ld_a = row.ld_a;
     uint32_t part_of = 0;  // which part of a split inner product
     if constexpr (STAGE == kStageGram && TM == 64) {
         part_of = tile % (uint32_t)row.parts;
@@ -783,7 +825,7 @@ __global__ __launch_bounds__(64 * WM * WN) void fsadam_matrix_stage(const Matrix
         ti = (int)(tile % (uint32_t)down);
         tj = (int)(tile / (uint32_t)down);
     }
-    const int64_t plane_x = (int64_t)s64 * l64, plane_a = (int64_t)s64 * s64;
+    const int64_t plane_x = (int64_t)s64 * ld_x, plane_a = (int64_t)s64 * ld_a;
     const _Float16* x = work + row.x_off[k.from] + (int64_t)matrix * 2 * plane_x;
     auto square = [&](int which) { return work + row.sq_off[which] + (int64_t)matrix * PLANES * plane_a; };
     const int i0 = ti * TM, j0 = tj * TN;
@@ -798,7 +840,7 @@ __global__ __launch_bounds__(64 * WM * WN) void fsadam_matrix_stage(const Matrix
     if constexpr (STAGE == kStageGram && TM == 64) {
         const int from = (int)part_of * kPartDepth, left = l64 - from;
         const int depth = row.parts > 1 && left > kPartDepth ? kPartDepth : left;
-        prod.run(x + (int64_t)i0 * l64 + from, l64, plane_x, s64 - i0, x + (int64_t)j0 * l64 + from, l64, plane_x, s64 - j0, depth, reinterpret_cast<_Float16*>(lds));
+        prod.run(x + (int64_t)i0 * ld_x + from, ld_x, plane_x, s64 - i0, x + (int64_t)j0 * ld_x + from, ld_x, plane_x, s64 - j0, depth, reinterpret_cast<_Float16*>(lds));
         if (row.parts > 1) {
             float4_t* to = partial((int)part_of);
 #pragma unroll
@@ -819,12 +861,12 @@ __global__ __launch_bounds__(64 * WM * WN) void fsadam_matrix_stage(const Matrix
 #pragma unroll
                 for (int j = 0; j < Prod::NJ; ++j) prod.acc[i][j] += partial(n)[(i * Prod::NJ + j) * Prod::kThreads];
     } else if constexpr (STAGE == kStageGram)
-        prod.run(x + (int64_t)i0 * l64, l64, plane_x, s64 - i0, x + (int64_t)j0 * l64, l64, plane_x, s64 - j0, l64, reinterpret_cast<_Float16*>(lds));
+        prod.run(x + (int64_t)i0 * ld_x, ld_x, plane_x, s64 - i0, x + (int64_t)j0 * ld_x, ld_x, plane_x, s64 - j0, l64, reinterpret_cast<_Float16*>(lds));
     else if constexpr (STAGE == kStageSquare)
-        prod.run(square(k.p) + (int64_t)i0 * s64, s64, plane_a, s64 - i0, square(k.q) + (int64_t)j0 * s64, s64, plane_a, s64 - j0, s64,
+        prod.run(square(k.p) + (int64_t)i0 * ld_a, ld_a, plane_a, s64 - i0, square(k.q) + (int64_t)j0 * ld_a, ld_a, plane_a, s64 - j0, s64,
                  reinterpret_cast<_Float16*>(lds));
     else
-        prod.run(square(k.p) + (int64_t)i0 * s64, s64, plane_a, s64 - i0, x + j0, l64, plane_x, l64 - j0, s64, reinterpret_cast<_Float16*>(lds));
+        prod.run(square(k.p) + (int64_t)i0 * ld_a, ld_a, plane_a, s64 - i0, x + j0, ld_x, plane_x, l64 - j0, s64, reinterpret_cast<_Float16*>(lds));
 
     float* slab = reinterpret_cast<float*>(lds);
     // element (i, j) of the slab; columns are exchanged in blocks of 8 by the rows' block of 8, so that reading eight
@@ -859,8 +901,24 @@ __global__ __launch_bounds__(64 * WM * WN) void fsadam_matrix_stage(const Matrix
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / WN, wn = wave % WN;
     constexpr int kWaveRows = TM / WM, kPieces = kSlab * TN / 8;  // pieces of eight elements
     constexpr int kPer = (kSlab < kWaveRows ? kSlab : kWaveRows) / 16;  // blocks of 16 rows a wave has in a slab
+    constexpr int kMine = kPieces / Prod::kThreads;  // pieces of a thread
+    static_assert(kMine * Prod::kThreads == kPieces, "slabs divide among the threads");
+    constexpr bool kAddsX = STAGE >= kStageUpdate;
 #pragma unroll
     for (int part = 0; part < TM / kSlab; ++part) {
+        // What is added to the slab's product is on its way while the slab is written.
+        half8_t add_hi[kMine], add_lo[kMine];
+        if constexpr (kAddsX) {
+#pragma unroll
+            for (int n = 0; n < kMine; ++n) {
+                const int e = threadIdx.x + n * Prod::kThreads, i = e / (TN / 8), j = (e % (TN / 8)) * 8;
+                if (i0 + part * kSlab < s64 && j0 + j < l64) {
+                    const _Float16* from = x + (int64_t)(i0 + part * kSlab + i) * ld_x + j0 + j;
+                    add_hi[n] = *reinterpret_cast<const half8_t*>(from);
+                    add_lo[n] = *reinterpret_cast<const half8_t*>(from + plane_x);
+                }
+            }
+        }
         if (kWaveRows > kSlab ? wm == part * kSlab / kWaveRows : wm * kWaveRows / kSlab == part) {
             const int first = (part * kSlab % kWaveRows) / 16;  // of the wave's blocks
             const int down = kWaveRows < kSlab ? wm * kWaveRows % kSlab : 0;  // its rows in the slab
@@ -876,15 +934,16 @@ __global__ __launch_bounds__(64 * WM * WN) void fsadam_matrix_stage(const Matrix
         const int r0 = i0 + part * kSlab;  // the slab's first row in the result
         if (r0 < s64) {  // sizes are multiples of 64: all rows of the slab are there, or none
             if constexpr (STAGE <= kStageUpdate) {
-                const int width = kSym ? s64 : l64;
-                for (int e = threadIdx.x; e < kPieces; e += Prod::kThreads) {
-                    const int i = e / (TN / 8), j = (e % (TN / 8)) * 8;
+                const int width = kSym ? s64 : l64, ld = kSym ? ld_a : ld_x;
+#pragma unroll
+                for (int n = 0; n < kMine; ++n) {
+                    const int e = threadIdx.x + n * Prod::kThreads, i = e / (TN / 8), j = (e % (TN / 8)) * 8;
                     if (j0 + j >= width) continue;
                     // Every element of a symmetric result is its lower triangle's, also in a tile on the diagonal: what a matrix
                     // gives does not depend on the tiles, and so not on the rest of the list.
                     if (kSym && j0 + j > r0 + i) continue;
-                    const int64_t at = (int64_t)(r0 + i) * width + j0 + j;
-                    float v[8], w[8];
+                    const int64_t at = (int64_t)(r0 + i) * ld + j0 + j;
+                    float v[8];
                     along_row(i, j, v);
                     if constexpr (kSym) {
                         if (j0 + j + 7 > r0 + i) {  // the diagonal runs through these eight
@@ -895,9 +954,8 @@ __global__ __launch_bounds__(64 * WM * WN) void fsadam_matrix_stage(const Matrix
                         }
                         finish(v, at, r0 + i - (j0 + j));
                     } else {
-                        load_planes<2>(x + at, plane_x, w);
 #pragma unroll
-                        for (int q = 0; q < 8; ++q) v[q] = k.linear * w[q] + k.product * v[q];
+                        for (int q = 0; q < 8; ++q) v[q] = k.linear * ((float)add_hi[n][q] + (float)add_lo[n][q]) + k.product * v[q];
                         store_planes<2>(work + row.x_off[k.to] + (int64_t)matrix * 2 * plane_x + at, plane_x, v);
                     }
                 }
@@ -906,7 +964,7 @@ __global__ __launch_bounds__(64 * WM * WN) void fsadam_matrix_stage(const Matrix
                         for (int e = threadIdx.x; e < kPieces; e += Prod::kThreads) {
                             const int j = e / (kSlab / 8), i = (e % (kSlab / 8)) * 8;
                             if (j0 + j >= s64 || (j0 + j) / 8 >= (r0 + i) / 8) continue;
-                            const int64_t at = (int64_t)(j0 + j) * s64 + r0 + i;
+                            const int64_t at = (int64_t)(j0 + j) * ld_a + r0 + i;
                             float v[8];
                             along_column(i, j, v);
                             finish(v, at, -8);
@@ -919,21 +977,23 @@ __global__ __launch_bounds__(64 * WM * WN) void fsadam_matrix_stage(const Matrix
                 const int64_t numel = (int64_t)row.rows * row.cols;
                 const float ratio = row.step_ratio;
                 if (row.tall) {  // a X + B X along the rows of X first, in the slab: its columns are what is written
-                    for (int e = threadIdx.x; e < kPieces; e += Prod::kThreads) {
-                        const int i = e / (TN / 8), j = (e % (TN / 8)) * 8;
-                        if (j0 + j >= l64) continue;
-                        float o[8], w[8];
-                        along_row(i, j, o);
-                        load_planes<2>(x + (int64_t)(r0 + i) * l64 + j0 + j, plane_x, w);
 #pragma unroll
-                        for (int q = 0; q < 8; ++q) o[q] = k.linear * w[q] + k.product * o[q];
+                    for (int n = 0; n < kMine; ++n) {
+                        const int e = threadIdx.x + n * Prod::kThreads, i = e / (TN / 8), j = (e % (TN / 8)) * 8;
+                        if (j0 + j >= l64) continue;
+                        float o[8];
+                        along_row(i, j, o);
+#pragma unroll
+                        for (int q = 0; q < 8; ++q) o[q] = k.linear * ((float)add_hi[n][q] + (float)add_lo[n][q]) + k.product * o[q];
                         float4_t* to = reinterpret_cast<float4_t*>(at_slab(i, j));
                         to[0] = float4_t{o[0], o[1], o[2], o[3]};
                         to[1] = float4_t{o[4], o[5], o[6], o[7]};
                     }
                     __syncthreads();
                 }
-                for (int e = threadIdx.x; e < kPieces; e += Prod::kThreads) {
+#pragma unroll
+                for (int n = 0; n < kMine; ++n) {
+                    const int e = threadIdx.x + n * Prod::kThreads;
                     int i, j;
                     float o[8], w[8];
                     if (row.tall) {
@@ -946,9 +1006,8 @@ __global__ __launch_bounds__(64 * WM * WN) void fsadam_matrix_stage(const Matrix
                         j = (e % (TN / 8)) * 8;
                         if (r0 + i >= row.s || j0 + j >= row.l) continue;
                         along_row(i, j, o);
-                        load_planes<2>(x + (int64_t)(r0 + i) * l64 + j0 + j, plane_x, w);
 #pragma unroll
-                        for (int q = 0; q < 8; ++q) o[q] = k.linear * w[q] + k.product * o[q];
+                        for (int q = 0; q < 8; ++q) o[q] = k.linear * ((float)add_hi[n][q] + (float)add_lo[n][q]) + k.product * o[q];
                     }
                     const int64_t r = row.tall ? j0 + j : r0 + i, c = row.tall ? r0 + i : j0 + j;
                     const int left = row.cols - (int)c;  // elements of the row from here on
