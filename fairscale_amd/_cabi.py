@@ -115,8 +115,8 @@ SIGNATURES = {
     "fsadam_grad_pass_noalloc": (_i32, [ctypes.POINTER(FsGradTensor), _i64, _i32, _f32, _vp, _i32, _vp, _vp, _vp, _vp]),
     "fsadam_clear_cache": (_i32, []),
     "fsadam_momentum_workspace": (_i32, [ctypes.POINTER(FsMomentumTensor), _i64, ctypes.POINTER(_i64)]),
-    # tensors, n, grad_type, update_type, momentum, nesterov, scale, scale_dev, norms, found_inf, workspace, bytes, stream
-    "fsadam_momentum_pass": (_i32, [ctypes.POINTER(FsMomentumTensor), _i64, _i32, _i32, _f64, _i32, _f32, _vp, _vp, _vp, _vp, _i64, _vp]),
+    # tensors, n, grad_type, update_type, momentum, nesterov, scale, scale_dev, norms, found_inf, clear, workspace, bytes, stream
+    "fsadam_momentum_pass": (_i32, [ctypes.POINTER(FsMomentumTensor), _i64, _i32, _i32, _f64, _i32, _f32, _vp, _vp, _vp, _i32, _vp, _i64, _vp]),
     "fsadam_orth_workspace": (_i32, [ctypes.POINTER(FsMatrix), _i64, ctypes.POINTER(FsOrthOptions), ctypes.POINTER(_i64)]),
     "fsadam_orthogonalize": (_i32, [ctypes.POINTER(FsMatrix), _i64, _i32, ctypes.POINTER(FsOrthOptions), _vp, _i64, _vp]),
     "fsadam_muon_workspace": (_i32, [ctypes.POINTER(FsMuonTensor), _i64, ctypes.POINTER(FsOrthOptions), ctypes.POINTER(_i64)]),

@@ -588,7 +588,7 @@ int fsadam_momentum_workspace(const FsMomentumTensor* tensors, int64_t n_tensors
 }
 
 int fsadam_momentum_pass(const FsMomentumTensor* tensors, int64_t n_tensors, int grad_type, int update_type, double momentum, int nesterov,
-                         float scale, const float* scale_dev, float* norms_dev, float* found_inf_dev, void* workspace,
+                         float scale, const float* scale_dev, float* norms_dev, float* found_inf_dev, int clear_found_inf, void* workspace,
                          int64_t workspace_bytes, void* hip_stream) {
     return guarded([&] {
         if (!valid_type(grad_type) || !valid_type(update_type)) return fail(FSADAM_EINVAL, "unknown type");
@@ -612,11 +612,13 @@ int fsadam_momentum_pass(const FsMomentumTensor* tensors, int64_t n_tensors, int
         hipStream_t stream = static_cast<hipStream_t>(hip_stream);
         double* partials = reinterpret_cast<double*>(static_cast<char*>(workspace) + momentum_table_bytes(n_tensors));
         const MomentumArgs k = momentum_args(momentum, nesterov, scale, scale_dev);
+        float* cleared = clear_found_inf ? found_inf_dev : nullptr;
+        if (cleared && !chunks) hipLaunchKernelGGL(fsadam_clear_flag, dim3(1), dim3(1), 0, stream, cleared);
         auto launch = [&](const auto& table) {
             using Table = std::decay_t<decltype(table)>;
             const dim3 grid((uint32_t)chunks), block(kChunkThreads);
 #define FM_PASS(G, U) \
-    if (grad_type == G && update_type == U) hipLaunchKernelGGL((fsadam_momentum_chunks<G, U, Table>), grid, block, 0, stream, table, k, partials)
+    if (grad_type == G && update_type == U) hipLaunchKernelGGL((fsadam_momentum_chunks<G, U, Table>), grid, block, 0, stream, table, k, partials, cleared)
             if (chunks) {
                 FM_PASS(kTypeF32, kTypeF32); FM_PASS(kTypeF32, kTypeF16); FM_PASS(kTypeF32, kTypeBF16);
                 FM_PASS(kTypeF16, kTypeF32); FM_PASS(kTypeF16, kTypeF16); FM_PASS(kTypeF16, kTypeBF16);
@@ -624,7 +626,7 @@ int fsadam_momentum_pass(const FsMomentumTensor* tensors, int64_t n_tensors, int
             }
 #undef FM_PASS
             if (norms_dev || found_inf_dev)
-                hipLaunchKernelGGL((fsadam_momentum_norms<Table>), dim3((uint32_t)n_tensors), block, 0, stream, table, (const double*)partials, norms_dev, found_inf_dev);
+                hipLaunchKernelGGL((fsadam_momentum_norms<Table>), dim3((uint32_t)n_tensors), dim3(kNormThreads), 0, stream, table, (const double*)partials, norms_dev, found_inf_dev);
             return launched();
         };
         if (table_in_arguments(n_tensors, chunks)) {

@@ -265,22 +265,27 @@ constexpr int kChunkThreads = 256;
 constexpr int kChunkElems = 8192;  // elements of one partial sum
 constexpr int kMomentumElems = 1024;  // likewise, of the momentum pass: four to a thread (8 and 16 are 4 and 12 % slower)
 
-// Sum over a workgroup of 256 in a fixed order; the result is valid in thread 0.
+// Sum over a workgroup in a fixed order; the result is valid in thread 0.
+template <int THREADS = kChunkThreads>
 __device__ __forceinline__ double block_sum(double v) {
-    __shared__ double part[4];
+    __shared__ double part[THREADS / 64];
     for (int d = 32; d > 0; d >>= 1) v += __shfl_down(v, d);
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
     __syncthreads();
-    return part[0] + part[1] + part[2] + part[3];
+    v = 0.0;
+#pragma unroll
+    for (int n = 0; n < THREADS / 64; ++n) v += part[n];
+    return v;
 }
 
 // A thread's share of the sum of p[0 .. n - 1], eight loads at a time in flight.
+template <int THREADS = kChunkThreads>
 __device__ __forceinline__ double sum_of(const double* p, int64_t n) {
     double sum = 0.0;
-    for (int64_t i = threadIdx.x; i < n; i += 8 * kChunkThreads) {
+    for (int64_t i = threadIdx.x; i < n; i += 8 * THREADS) {
         double v[8];
 #pragma unroll
-        for (int q = 0; q < 8; ++q) v[q] = i + q * kChunkThreads < n ? p[i + q * kChunkThreads] : 0.0;
+        for (int q = 0; q < 8; ++q) v[q] = i + q * THREADS < n ? p[i + q * THREADS] : 0.0;
 #pragma unroll
         for (int q = 0; q < 8; ++q) sum += v[q];
     }
@@ -327,7 +332,8 @@ __device__ __forceinline__ void for_eights(int64_t begin, int64_t end, Each&& ea
 
 // Bound by HBM: 2 + 4 bytes read and 2 + 4 written per element with 16-bit gradients and updates.
 template <int GT, int UT, typename Table>
-__global__ __launch_bounds__(kChunkThreads) void fsadam_momentum_chunks(Table tables, MomentumArgs k, double* partials) {
+__global__ __launch_bounds__(kChunkThreads) void fsadam_momentum_chunks(Table tables, MomentumArgs k, double* partials, float* cleared) {
+    if (cleared && blockIdx.x == 0 && threadIdx.x == 0) *cleared = 0.0f;
     const MomentumRow* table = rows_of(tables);
     const int n_rows = tables.n;
     int low = 0, high = n_rows - 1;
@@ -395,11 +401,12 @@ __global__ __launch_bounds__(kChunkThreads) void fsadam_momentum_chunks(Table ta
 
 // norms[row] = sqrt of the row's sum of squares; found_inf is raised where that is not finite (a double holds the sum of
 // squares of any floats, so it is not finite exactly where an update is not).
+constexpr int kNormThreads = 1024;  // a tensor of 45 million elements has 44000 partial sums
 template <typename Table>
-__global__ __launch_bounds__(kChunkThreads) void fsadam_momentum_norms(Table tables, const double* partials, float* norms, float* found_inf) {
+__global__ __launch_bounds__(kNormThreads) void fsadam_momentum_norms(Table tables, const double* partials, float* norms, float* found_inf) {
     const MomentumRow& row = rows_of(tables)[blockIdx.x];
     const int64_t n = (row.numel + kMomentumElems - 1) / kMomentumElems;
-    const double sum = block_sum(sum_of(partials + row.first, n));
+    const double sum = block_sum<kNormThreads>(sum_of<kNormThreads>(partials + row.first, n));
     if (threadIdx.x == 0) {
         if (norms) norms[blockIdx.x] = (float)sqrt(sum);
         if (found_inf && !__builtin_isfinite(sum)) *found_inf = 1.0f;
@@ -1377,6 +1384,7 @@ __global__ void fsadam_put_resident_rows(ResidentRow* table, int n, ResidentRows
     constexpr int kWords = sizeof(ResidentRow) / 16;
     for (int e = threadIdx.x; e < n * kWords; e += blockDim.x) reinterpret_cast<words4_t*>(table)[e] = reinterpret_cast<const words4_t*>(rows.row)[e];
 }
+__global__ void fsadam_clear_flag(float* flag) { *flag = 0.0f; }
 __global__ void fsadam_put_momentum_rows(MomentumRow* table, int n, MomentumRows rows) {
     constexpr int kWords = sizeof(MomentumRow) / 16;
     typedef uint32_t word_t __attribute__((ext_vector_type(4)));

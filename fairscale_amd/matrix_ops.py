@@ -133,8 +133,9 @@ def momentum_pass(grads: Sequence[torch.Tensor], momenta: Sequence[torch.Tensor]
     if not fill_rows((grads, momenta, updates), (dtype, torch.float32, update_dtype), (1, 2), device, rows, True):
         _check_momentum_lists(grads, momenta, updates, device, dtype, update_dtype)
         rows[:] = [(g.data_ptr(), m.data_ptr(), u.data_ptr(), g.numel()) for g, m, u in zip(grads, momenta, updates)]
-    if found_inf is None:
-        found_inf = torch.zeros(1, dtype=torch.float32, device=device)
+    fresh = found_inf is None
+    if fresh:
+        found_inf = torch.empty(1, dtype=torch.float32, device=device)  # the call clears it
     elif found_inf.dtype != torch.float32 or found_inf.device != device or found_inf.numel() != 1:
         raise RuntimeError("found_inf must be a float32 tensor with one element on the gradients' device")
     value, pointer = scale_arguments(scale, device)
@@ -145,7 +146,7 @@ def momentum_pass(grads: Sequence[torch.Tensor], momenta: Sequence[torch.Tensor]
         norms = torch.empty(len(grads), dtype=torch.float32, device=device)
         _cabi.check(lib.fsadam_momentum_pass(
             pointer_to_rows, len(grads), TYPE_CODE[dtype], TYPE_CODE[update_dtype], float(momentum), 1 if nesterov else 0, value, pointer,
-            norms.data_ptr(), found_inf.data_ptr(), workspace.data_ptr(), size, int(torch.cuda.current_stream(device).cuda_stream)))
+            norms.data_ptr(), found_inf.data_ptr(), 1 if fresh else 0, workspace.data_ptr(), size, int(torch.cuda.current_stream(device).cuda_stream)))
     return MomentumStats(updates, norms, found_inf)
 
 

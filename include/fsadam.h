@@ -297,7 +297,7 @@ int fsadam_grad_pass_noalloc(const FsGradTensor* grads, int64_t n_tensors, int g
  *     r = g / scale;   m <- m + (r - m) * (1 - momentum);   u = nesterov ? r + (m - r) * momentum : m
  * m is updated in place; u is stored in update_type (u may be g itself where the types are the same: updates over the
  * gradients).  norms_dev[t] (may be NULL) is the L2 norm of tensor t's update as stored, summed in fp64 in a fixed order;
- * found_inf_dev[0] (may be NULL) is set to 1.0f, never cleared, where a stored update is not finite.
+ * found_inf_dev[0] (may be NULL) is set to 1.0f where a stored update is not finite; clear_found_inf != 0: and to 0.0f before.
  * scale_dev, when not NULL, is a device float[1] read in place of scale. */
 typedef struct FsMomentumTensor {
     const void* g;
@@ -307,7 +307,7 @@ typedef struct FsMomentumTensor {
 } FsMomentumTensor;
 int fsadam_momentum_workspace(const FsMomentumTensor* tensors, int64_t n_tensors, int64_t* bytes);
 int fsadam_momentum_pass(const FsMomentumTensor* tensors, int64_t n_tensors, int grad_type, int update_type, double momentum, int nesterov,
-                         float scale, const float* scale_dev, float* norms_dev, float* found_inf_dev, void* workspace,
+                         float scale, const float* scale_dev, float* norms_dev, float* found_inf_dev, int clear_found_inf, void* workspace,
                          int64_t workspace_bytes, void* hip_stream);
 
 /* Orthogonalisation by Newton-Schulz products.  For every matrix U (rows x cols), with X = U / max(|U|_F, eps), `steps` times

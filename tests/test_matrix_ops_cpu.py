@@ -159,7 +159,7 @@ def momentum_rows(**change):
 ])
 def test_bad_momentum_passes_are_refused(call):
     g, u = call.get("types", (0, 0))
-    rc = L.fsadam_momentum_pass(call.get("rows", momentum_rows()), 1, g, u, call.get("momentum", 0.9), 1, call.get("scale", 1.0), None, None, None, FAKE,
+    rc = L.fsadam_momentum_pass(call.get("rows", momentum_rows()), 1, g, u, call.get("momentum", 0.9), 1, call.get("scale", 1.0), None, None, None, 0, FAKE,
                                 call.get("bytes", 100), None)
     assert rc == -1 and L.fsadam_last_error()
 

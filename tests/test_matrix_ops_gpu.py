@@ -554,3 +554,8 @@ def test_what_a_matrix_gives_does_not_depend_on_the_list(products, others):
     for k, (a, b) in enumerate(zip(alone, orthogonalize(us + rest, products=products))):
         assert torch.equal(a, b), us[k].shape
     check_orth(us, alone, products)
+
+
+def test_momentum_pass_over_empty_tensors_only():
+    got = momentum_pass([torch.zeros(0, device="cuda"), torch.zeros(3, 0, device="cuda")], [torch.zeros(0, device="cuda"), torch.zeros(3, 0, device="cuda")])
+    assert got.found_inf.item() == 0.0 and (got.norms == 0).all()
