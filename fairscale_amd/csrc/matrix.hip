@@ -152,7 +152,7 @@ int64_t full_tiles(int64_t s, int64_t l, int64_t t) { return ((s + t - 1) / t) *
 // Adds up to `batch` matrices of a row to the chunk; returns how many fit.  A chunk takes at least one.
 int64_t add_to_chunk(Chunk& chunk, const MatrixRow& proto, int64_t batch) {
     const int64_t products = chunk.products;
-    const int64_t x = 2 * (int64_t)proto.s64 * proto.ld_x, a = products * (int64_t)proto.s64 * proto.ld_a;  // halves of one matrix, one buffer
+    const int64_t x = 2 * (int64_t)proto.s64 * proto.l64, a = products * (int64_t)proto.s64 * proto.s64;  // halves of one matrix, one buffer
     const int squares = chunk.pairs() ? 3 : 2;
     const int64_t per = 2 * x + squares * a, room = kChunkBytes / 2 - chunk.halves;
     int64_t n = std::min(batch, room / per);
@@ -182,10 +182,6 @@ int64_t add_to_chunk(Chunk& chunk, const MatrixRow& proto, int64_t batch) {
     chunk.rows.push_back(row);
     return n;
 }
-
-// Rows of an odd number of 128-byte lines: a tile's rows at one depth then lie in different channels of the L2, where a power of two
-// between them would put all of them into one.
-int64_t odd_lines(int64_t columns) { return columns / 64 % 2 ? columns : columns + 64; }
 
 struct Source {  // what a list entry's row starts from
     const void* src; float* buf; void* dst; void* copy;
@@ -223,8 +219,6 @@ void make_chunks(const std::vector<Source>& all, int asked, std::vector<Chunk>& 
         row.l = row.tall ? row.rows : row.cols;
         row.s64 = (int32_t)up(row.s, 64);
         row.l64 = (int32_t)up(row.l, 64);
-        row.ld_x = (int32_t)odd_lines(row.l64);
-        row.ld_a = (int32_t)odd_lines(row.s64);
         row.src_ld = in.src_ld; row.src_stride = in.src_stride;
         row.dst_ld = in.dst_ld; row.dst_stride = in.dst_stride;
         row.step_ratio = in.step_ratio;
@@ -321,8 +315,8 @@ Tiles choose_tiles(int64_t t64, int64_t t128, int64_t t256) {
 
 template <int STAGE, int TILE, int PLANES>
 void launch_tile(int64_t count, int n_rows, const MatrixRow* table, const StageArgs& k, _Float16* work, hipStream_t stream) {
-    constexpr int WM = 2, WN = TILE == 64 ? 2 : 4, BK = TILE > 64 && PLANES == 2 ? 32 : 64;
-    if (count) hipLaunchKernelGGL((fsadam_matrix_stage<STAGE, TILE, TILE, WM, WN, BK, 2, PLANES>), dim3((uint32_t)count), dim3(64 * WM * WN), 0, stream, table, n_rows, k, work);
+    constexpr int WM = 2, WN = TILE == 64 ? 2 : 4, BK = column_block(PLANES), DEPTH = TILE == 64 && PLANES == 2 ? 4 : 2;
+    if (count) hipLaunchKernelGGL((fsadam_matrix_stage<STAGE, TILE, TILE, WM, WN, BK, DEPTH, PLANES>), dim3((uint32_t)count), dim3(64 * WM * WN), 0, stream, table, n_rows, k, work);
 }
 
 template <int STAGE, int PLANES>
@@ -358,7 +352,7 @@ void launch_prepare(const Chunk& c, const Call& call, const MatrixRow* table, do
 #define FM_TYPE(T, EACH) \
     if (call.src_type == T) { EACH(T); }
 #define FM_CHUNKS(T) hipLaunchKernelGGL((fsadam_matrix_chunks<T, STEP>), chunks, block, 0, stream, table, n, call.momentum, partials)
-#define FM_NORMALISE(T) hipLaunchKernelGGL((fsadam_matrix_normalise<T, STEP>), tiles, block, 0, stream, table, n, call.momentum, (const double*)inverse, power, work)
+#define FM_NORMALISE(T) hipLaunchKernelGGL((fsadam_matrix_normalise<T, STEP>), tiles, block, 0, stream, table, n, call.momentum, (const double*)inverse, power, c.products == FSADAM_PRODUCTS_SPLIT ? 5 : 6, work)
     FM_TYPE(kTypeF32, FM_CHUNKS) FM_TYPE(kTypeF16, FM_CHUNKS) FM_TYPE(kTypeBF16, FM_CHUNKS)
     hipLaunchKernelGGL(fsadam_matrix_norms, matrices, block, 0, stream, table, n, (double)call.options.eps, (const double*)partials, inverse);
     FM_TYPE(kTypeF32, FM_NORMALISE) FM_TYPE(kTypeF16, FM_NORMALISE) FM_TYPE(kTypeBF16, FM_NORMALISE)

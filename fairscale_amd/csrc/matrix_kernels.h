@@ -19,7 +19,10 @@
 // Sums are held in fp32 (matrix instructions), norms in fp64.
 //
 // Storage in the workspace, all sizes padded to 64 with zeros (zero rows and columns stay zero through the iteration,
-// so no product needs a mask): X is s64 x l64, A and B are s64 x s64, row-major, the planes one behind the other.
+// so no product needs a mask): X is s64 x l64, A and B are s64 x s64, the planes one behind the other.  A matrix lies in blocks of
+// kBlock columns (what a panel of a product is deep: 64 halves, 32 with two planes), each block's rows one behind the other: a
+// panel's rows, wherever it is cut, are then one contiguous span, every load of a wave 1 KiB of it.  Row-major, a wave's load
+// of 64-byte pieces fills half lines only and gets through at half the rate (62 against 115 GB/s for a compute unit).
 #pragma once
 
 #include <cstdint>
@@ -56,7 +59,6 @@ struct alignas(16) MatrixRow {
     int64_t sq_off[3]; // workspace: square matrices (A and B; a pair of steps uses all three)
     int32_t batch, rows, cols;
     int32_t s, l, s64, l64;
-    int32_t ld_x, ld_a;             // elements from row to row of X and of the square matrices
     int32_t tall;      // rows > cols: X is the transpose
     int32_t first_matrix;           // index of the row's first matrix in the chunk
     int32_t chunks;                 // partial sums per matrix
@@ -207,6 +209,12 @@ __device__ __forceinline__ void load_planes(const _Float16* at, int64_t plane, f
 #pragma unroll
         for (int q = 0; q < 8; ++q) v[q] += (float)lo[q];
     }
+}
+
+constexpr int column_block(int planes) { return planes == 2 ? 32 : 64; }
+// Where element (i, j) of a matrix of `rows` rows lies.
+__device__ __forceinline__ int64_t in_blocks(int i, int j, int rows, int log_block) {
+    return (((int64_t)(j >> log_block) * rows + i) << log_block) + (j & ((1 << log_block) - 1));
 }
 
 // Workgroups are handed to the 8 XCDs in turn, each with an L2 of its own: give every XCD a contiguous range of tiles.
@@ -479,7 +487,8 @@ __global__ __launch_bounds__(kChunkThreads) void fsadam_matrix_norms(const Matri
 
 // X0 * 2^k as two halves, 64 x 64 elements a workgroup, turned where the matrix is tall; the padding is written as zeros.
 template <int ST, bool STEP>
-__global__ __launch_bounds__(256) void fsadam_matrix_normalise(const MatrixRow* table, int n_rows, MomentumArgs k, const double* inverse, double power, _Float16* work) {
+__global__ __launch_bounds__(256) void fsadam_matrix_normalise(const MatrixRow* table, int n_rows, MomentumArgs k, const double* inverse, double power, int log_block,
+                                                                _Float16* work) {
     __shared__ float tile[64][65];
     int matrix;
     uint32_t t;
@@ -489,9 +498,9 @@ __global__ __launch_bounds__(256) void fsadam_matrix_normalise(const MatrixRow* 
     const int r0 = row.tall ? j0 : i0, c0 = row.tall ? i0 : j0;         // in the source
     const double factor = inverse[row.first_matrix + matrix] * power;
     const Divisor by(k);
-    const int64_t plane = (int64_t)row.s64 * row.ld_x;
+    const int64_t plane = (int64_t)row.s64 * row.l64;
     _Float16* x = work + row.x_off[0] + (int64_t)matrix * 2 * plane;
-    auto put = [&](int i, int j, const float (&v)[8]) { store_planes<2>(x + (int64_t)(i0 + i) * row.ld_x + j0 + j, plane, v); };
+    auto put = [&](int i, int j, const float (&v)[8]) { store_planes<2>(x + in_blocks(i0 + i, j0 + j, row.s64, log_block), plane, v); };
 #pragma unroll
     for (int part = 0; part < 2; ++part) {
         const int e = threadIdx.x + part * 256, r = e >> 3, c = (e & 7) * 8;  // eight neighbours in the source
@@ -555,21 +564,28 @@ template <int BK>
 __device__ __forceinline__ int swizzle_nt(int row) {
     return BK == 64 ? (row & 7) : ((row >> 1) & 3);
 }
-// K x columns ("NN", read with the transposing LDS loads): pairs of chunks (32 bytes, 16 columns) exchanged so that the rows
-// one load touches (8g + 0..3 for the four groups g of 16 lanes) spread over the banks.  A row of 64 columns has four pairs only.
-template <int COLS>
+// K x columns ("NN", read with the transposing LDS loads): blocks of BK columns as in memory, pairs of chunks (32 bytes, 16
+// columns) of a row exchanged so that the rows one load touches (8g + 0..3 for the four groups g of 16 lanes) spread over the banks.
+template <int BK>
 __device__ __forceinline__ int swizzle_nn(int row) {
-    return (row & 3) | (COLS > 64 ? ((row >> 3) & 1) << 2 : 0);
+    return BK == 32 ? (row >> 3) & 1 : ((row >> 1) & 1) | (((row >> 3) & 1) << 1);
 }
 
-// 1 KiB straight from memory into LDS: every lane gives the address of 16 bytes, which land at dst + 16 * lane.
+// An address that all lanes hold, in scalar registers.
+__device__ __forceinline__ const _Float16* uniform(const _Float16* p) {
+    const uint64_t a = (uint64_t)p;
+    return (const _Float16*)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(a >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)a));
+}
+
+// 1 KiB straight from memory into LDS: 16 bytes from src + `bytes` of every lane land at dst + 16 * lane.
 // From assembly because of the wait: behind the builtin the compiler places a wait for ALL loads before the next read
 // of LDS (it cannot tell the buffer being filled from the one being read), which takes away the overlap the two
 // buffers are there for.  The statement has no output register; what it writes is LDS, and nothing reads that before
 // loads_arrived() and the barrier behind it.  m0 is a reserved register: the compiler writes it right before each use of
-// its own and keeps nothing in it.  The s_nop: a write of m0 needs one wait state before the load that uses it.
-__device__ __forceinline__ void load_to_lds(const _Float16* src, uint32_t dst) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(dst), "v"((const FM_GLOBAL void*)src) : "memory");
+// its own and keeps nothing in it.  The s_nop: a write of m0 needs one wait state before the load that uses
+// it, a vector instruction's write of the scalar address (readfirstlane) five, and the compiler does not look into the statement.
+__device__ __forceinline__ void load_to_lds(const _Float16* src, uint32_t bytes, uint32_t dst) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(dst), "v"(bytes), "s"(src) : "memory");
 }
 template <int LEFT>
 __device__ __forceinline__ void loads_arrived() {  // all but the last LEFT loads of this wave
@@ -595,53 +611,52 @@ struct Product {
 
     float4_t acc[MI][NJ];
 
-    // p: first row of the panel, rows_p: how many rows there are from it on (further ones are read as the last);
-    // q: NT as p; NN the panel's first column, cols_q columns from it on.
-    __device__ __forceinline__ void run(const _Float16* p, int64_t ld_p, int64_t plane_p, int rows_p, const _Float16* q, int64_t ld_q, int64_t plane_q,
-                                        int rows_q, int k_total, _Float16* lds) {
+    // p: element (first row, first depth) of a matrix of `rows` rows, in blocks of BK columns; rows_p: how many rows there are from it
+    // on (further ones are read as the last).  q: NT as p; NN element (first depth, first column), blocks_q blocks of columns from it on.
+    __device__ __forceinline__ void run(const _Float16* p, int rows, int64_t plane_p, int rows_p, const _Float16* q, int64_t plane_q, int rows_q, int blocks_q,
+                                        int k_total, _Float16* lds) {
         const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         const int wm = wave / WN, wn = wave % WN;
-        uint32_t off_p[kLoadsP], off_q[kLoadsQ];
+        constexpr int kRowsPerLoad = 512 / BK, kChunks = BK / 8;  // of 1 KiB; 16-byte chunks of a row
+        uint32_t off_p[kLoadsP], off_q[kLoadsQ];                  // bytes
 #pragma unroll
         for (int n = 0; n < kLoadsP; ++n) {
-            int r = (wave * kLoadsP + n) * (512 / BK) + lane / (BK / 8);
-            const int chunk = (lane % (BK / 8)) ^ swizzle_nt<BK>(r);
+            int r = (wave * kLoadsP + n) * kRowsPerLoad + lane / kChunks;
+            const int chunk = (lane % kChunks) ^ swizzle_nt<BK>(r);
             r = r < rows_p ? r : rows_p - 1;
-            off_p[n] = (uint32_t)(r * ld_p + chunk * 8);
+            off_p[n] = (uint32_t)(r * BK + chunk * 8) * 2;
         }
 #pragma unroll
         for (int n = 0; n < kLoadsQ; ++n) {
+            const int at = (wave * kLoadsQ + n) * kRowsPerLoad + lane / kChunks, slot = lane % kChunks;
             if constexpr (NN) {
-                constexpr int kChunks = TN / 8;  // of a row
-                const int r = (wave * kLoadsQ + n) * (64 / kChunks) + lane / kChunks;
-                const int slot = lane % kChunks;
-                int chunk = (((slot >> 1) ^ swizzle_nn<TN>(r)) << 1) | (slot & 1);
-                const int last = rows_q / 8 - 1;
-                chunk = chunk < last ? chunk : last;
-                off_q[n] = (uint32_t)(r * ld_q + chunk * 8);
+                const int r = at % BK;
+                int block = at / BK;
+                block = block < blocks_q ? block : blocks_q - 1;
+                const int chunk = (((slot >> 1) ^ swizzle_nn<BK>(r)) << 1) | (slot & 1);
+                off_q[n] = (uint32_t)((block * rows + r) * BK + chunk * 8) * 2;
             } else {
-                int r = (wave * kLoadsQ + n) * (512 / BK) + lane / (BK / 8);
-                const int chunk = (lane % (BK / 8)) ^ swizzle_nt<BK>(r);
-                r = r < rows_q ? r : rows_q - 1;
-                off_q[n] = (uint32_t)(r * ld_q + chunk * 8);
+                const int r = at < rows_q ? at : rows_q - 1;
+                off_q[n] = (uint32_t)(r * BK + (slot ^ swizzle_nt<BK>(at)) * 8) * 2;
             }
         }
-        const int64_t advance_q = NN ? (int64_t)BK * ld_q : BK;
+        const int64_t next_p = (int64_t)__builtin_amdgcn_readfirstlane(rows) * BK, next_q = NN ? BK * BK : next_p;
+        p = uniform(p), q = uniform(q);
+        const _Float16 *low_p = uniform(p + plane_p), *low_q = uniform(q + plane_q);
         const uint32_t lds_at = __builtin_amdgcn_readfirstlane((int)lds_address(lds));
         auto fetch = [&](uint32_t stage) {
 #pragma unroll
             for (int plane = 0; plane < PLANES; ++plane) {
-                const _Float16* gp = p + plane * plane_p;
-                const _Float16* gq = q + plane * plane_q;
+                const _Float16 *gp = plane ? low_p : p, *gq = plane ? low_q : q;
                 const uint32_t lp = stage + 2 * (plane * kPanelP + wave * kLoadsP * 512);
                 const uint32_t lq = stage + 2 * (PLANES * kPanelP + plane * kPanelQ + wave * kLoadsQ * 512);
 #pragma unroll
-                for (int n = 0; n < kLoadsP; ++n) load_to_lds(gp + off_p[n], lp + n * 1024);
+                for (int n = 0; n < kLoadsP; ++n) load_to_lds(gp, off_p[n], lp + n * 1024);
 #pragma unroll
-                for (int n = 0; n < kLoadsQ; ++n) load_to_lds(gq + off_q[n], lq + n * 1024);
+                for (int n = 0; n < kLoadsQ; ++n) load_to_lds(gq, off_q[n], lq + n * 1024);
             }
-            p += BK;
-            q += advance_q;
+            p += next_p, low_p += next_p;
+            q += next_q, low_q += next_q;
         };
 #pragma unroll
         for (int i = 0; i < MI; ++i)
@@ -655,7 +670,10 @@ struct Product {
         if constexpr (NN) {
             const int r = 8 * g + (c >> 2);
 #pragma unroll
-            for (int j = 0; j < NJ; ++j) nn_at[j] = r * TN + (((wn * (TN / WN) / 16 + j) ^ swizzle_nn<TN>(r)) * 16) + (c & 3) * 4;
+            for (int j = 0; j < NJ; ++j) {
+                const int column = wn * (TN / WN) + j * 16;
+                nn_at[j] = column / BK * (BK * BK) + r * BK + ((column % BK / 16) ^ swizzle_nn<BK>(r)) * 16 + (c & 3) * 4;
+            }
         }
 
         constexpr int kLoads = PLANES * (kLoadsP + kLoadsQ);  // of a wave for one panel pair
@@ -689,8 +707,8 @@ struct Product {
 #pragma unroll
                 for (int j = 0; j < NJ; ++j) {
                     if constexpr (NN) {
-                        const short4_t low = __builtin_amdgcn_ds_read_tr16_b64_v4i16((FM_LDS short4_t*)(lq + nn_at[j] + kk * 32 * TN));
-                        const short4_t high = __builtin_amdgcn_ds_read_tr16_b64_v4i16((FM_LDS short4_t*)(lq + nn_at[j] + (kk * 32 + 4) * TN));
+                        const short4_t low = __builtin_amdgcn_ds_read_tr16_b64_v4i16((FM_LDS short4_t*)(lq + nn_at[j] + kk * 32 * BK));
+                        const short4_t high = __builtin_amdgcn_ds_read_tr16_b64_v4i16((FM_LDS short4_t*)(lq + nn_at[j] + (kk * 32 + 4) * BK));
                         const half4_t l4 = __builtin_bit_cast(half4_t, low), h4 = __builtin_bit_cast(half4_t, high);
                         f.q[plane][j] = __builtin_shufflevector(l4, h4, 0, 1, 2, 3, 4, 5, 6, 7);
                     } else {
@@ -815,7 +833,10 @@ __global__ __launch_bounds__(64 * WM * WN) void fsadam_matrix_stage(const Matrix
     int matrix;
     uint32_t tile;
     const MatrixRow& row = find_tile(table, n_rows, kind, xcd_contiguous(blockIdx.x, gridDim.x), matrix, tile);
-    const int s64 = row.s64, l64 = row.l64, ld_x = row.ld_x, ld_a = row.ld_a;
+    const int s64 = row.s64, l64 = row.l64;
+    constexpr int kLog = PLANES == 2 ? 5 : 6;
+    static_assert(BK == column_block(PLANES) && BK == 1 << kLog, "a panel is as deep as a block");
+    auto place = [&](int i, int j) { return in_blocks(i, j, s64, kLog); };
     uint32_t part_of = 0;  // which part of a split inner product
     if constexpr (STAGE == kStageGram && TM == 64) {
         part_of = tile % (uint32_t)row.parts;
@@ -832,7 +853,7 @@ __global__ __launch_bounds__(64 * WM * WN) void fsadam_matrix_stage(const Matrix
         ti = (int)(tile % (uint32_t)down);
         tj = (int)(tile / (uint32_t)down);
     }
-    const int64_t plane_x = (int64_t)s64 * ld_x, plane_a = (int64_t)s64 * ld_a;
+    const int64_t plane_x = (int64_t)s64 * l64, plane_a = (int64_t)s64 * s64;
     const _Float16* x = work + row.x_off[k.from] + (int64_t)matrix * 2 * plane_x;
     auto square = [&](int which) { return work + row.sq_off[which] + (int64_t)matrix * PLANES * plane_a; };
     const int i0 = ti * TM, j0 = tj * TN;
@@ -847,7 +868,7 @@ __global__ __launch_bounds__(64 * WM * WN) void fsadam_matrix_stage(const Matrix
     if constexpr (STAGE == kStageGram && TM == 64) {
         const int from = (int)part_of * kPartDepth, left = l64 - from;
         const int depth = row.parts > 1 && left > kPartDepth ? kPartDepth : left;
-        prod.run(x + (int64_t)i0 * ld_x + from, ld_x, plane_x, s64 - i0, x + (int64_t)j0 * ld_x + from, ld_x, plane_x, s64 - j0, depth, reinterpret_cast<_Float16*>(lds));
+        prod.run(x + place(i0, from), s64, plane_x, s64 - i0, x + place(j0, from), plane_x, s64 - j0, 0, depth, reinterpret_cast<_Float16*>(lds));
         if (row.parts > 1) {
             float4_t* to = partial((int)part_of);
 #pragma unroll
@@ -868,12 +889,12 @@ __global__ __launch_bounds__(64 * WM * WN) void fsadam_matrix_stage(const Matrix
 #pragma unroll
                 for (int j = 0; j < Prod::NJ; ++j) prod.acc[i][j] += partial(n)[(i * Prod::NJ + j) * Prod::kThreads];
     } else if constexpr (STAGE == kStageGram)
-        prod.run(x + (int64_t)i0 * ld_x, ld_x, plane_x, s64 - i0, x + (int64_t)j0 * ld_x, ld_x, plane_x, s64 - j0, l64, reinterpret_cast<_Float16*>(lds));
+        prod.run(x + place(i0, 0), s64, plane_x, s64 - i0, x + place(j0, 0), plane_x, s64 - j0, 0, l64, reinterpret_cast<_Float16*>(lds));
     else if constexpr (STAGE == kStageSquare)
-        prod.run(square(k.p) + (int64_t)i0 * ld_a, ld_a, plane_a, s64 - i0, square(k.q) + (int64_t)j0 * ld_a, ld_a, plane_a, s64 - j0, s64,
+        prod.run(square(k.p) + place(i0, 0), s64, plane_a, s64 - i0, square(k.q) + place(j0, 0), plane_a, s64 - j0, 0, s64,
                  reinterpret_cast<_Float16*>(lds));
     else
-        prod.run(square(k.p) + (int64_t)i0 * ld_a, ld_a, plane_a, s64 - i0, x + j0, ld_x, plane_x, l64 - j0, s64, reinterpret_cast<_Float16*>(lds));
+        prod.run(square(k.p) + place(i0, 0), s64, plane_a, s64 - i0, x + place(0, j0), plane_x, 0, (l64 - j0) / BK, s64, reinterpret_cast<_Float16*>(lds));
 
     float* slab = reinterpret_cast<float*>(lds);
     // element (i, j) of the slab; columns are exchanged in blocks of 8 by the rows' block of 8, so that reading eight
@@ -909,6 +930,18 @@ __global__ __launch_bounds__(64 * WM * WN) void fsadam_matrix_stage(const Matrix
     constexpr int kWaveRows = TM / WM, kPieces = kSlab * TN / 8;  // pieces of eight elements
     constexpr int kPer = (kSlab < kWaveRows ? kSlab : kWaveRows) / 16;  // blocks of 16 rows a wave has in a slab
     constexpr int kMine = kPieces / Prod::kThreads;  // pieces of a thread
+    // The n-th piece of this thread.  Where results lie in blocks, lanes go through a block's rows (contiguous); where they lie in rows of
+    // their own, along those.
+    auto piece = [&](int n, int& i, int& j) {
+        const int e = threadIdx.x + n * Prod::kThreads;
+        if constexpr (STAGE > kStageUpdate) {
+            i = e / (TN / 8);
+            j = e % (TN / 8) * 8;
+        } else {
+            i = e / (BK / 8) % kSlab;
+            j = e / (BK / 8 * kSlab) * BK + e % (BK / 8) * 8;
+        }
+    };
     static_assert(kMine * Prod::kThreads == kPieces, "slabs divide among the threads");
     constexpr bool kAddsX = STAGE >= kStageUpdate;
 #pragma unroll
@@ -918,9 +951,10 @@ __global__ __launch_bounds__(64 * WM * WN) void fsadam_matrix_stage(const Matrix
         if constexpr (kAddsX) {
 #pragma unroll
             for (int n = 0; n < kMine; ++n) {
-                const int e = threadIdx.x + n * Prod::kThreads, i = e / (TN / 8), j = (e % (TN / 8)) * 8;
+                int i, j;
+                piece(n, i, j);
                 if (i0 + part * kSlab < s64 && j0 + j < l64) {
-                    const _Float16* from = x + (int64_t)(i0 + part * kSlab + i) * ld_x + j0 + j;
+                    const _Float16* from = x + place(i0 + part * kSlab + i, j0 + j);
                     add_hi[n] = *reinterpret_cast<const half8_t*>(from);
                     add_lo[n] = *reinterpret_cast<const half8_t*>(from + plane_x);
                 }
@@ -941,15 +975,16 @@ __global__ __launch_bounds__(64 * WM * WN) void fsadam_matrix_stage(const Matrix
         const int r0 = i0 + part * kSlab;  // the slab's first row in the result
         if (r0 < s64) {  // sizes are multiples of 64: all rows of the slab are there, or none
             if constexpr (STAGE <= kStageUpdate) {
-                const int width = kSym ? s64 : l64, ld = kSym ? ld_a : ld_x;
+                const int width = kSym ? s64 : l64;
 #pragma unroll
                 for (int n = 0; n < kMine; ++n) {
-                    const int e = threadIdx.x + n * Prod::kThreads, i = e / (TN / 8), j = (e % (TN / 8)) * 8;
+                    int i, j;
+                    piece(n, i, j);
                     if (j0 + j >= width) continue;
                     // Every element of a symmetric result is its lower triangle's, also in a tile on the diagonal: what a matrix
                     // gives does not depend on the tiles, and so not on the rest of the list.
                     if (kSym && j0 + j > r0 + i) continue;
-                    const int64_t at = (int64_t)(r0 + i) * ld + j0 + j;
+                    const int64_t at = place(r0 + i, j0 + j);
                     float v[8];
                     along_row(i, j, v);
                     if constexpr (kSym) {
@@ -969,9 +1004,10 @@ __global__ __launch_bounds__(64 * WM * WN) void fsadam_matrix_stage(const Matrix
                 if constexpr (kSym) {
                     {  // the mirror image
                         for (int e = threadIdx.x; e < kPieces; e += Prod::kThreads) {
-                            const int j = e / (kSlab / 8), i = (e % (kSlab / 8)) * 8;
+                            // rows j of the result: lanes through the rows of a block of its columns
+                            const int j = e / (BK / 8) % TN, i = e / (BK / 8 * TN) * BK + e % (BK / 8) * 8;
                             if (j0 + j >= s64 || (j0 + j) / 8 >= (r0 + i) / 8) continue;
-                            const int64_t at = (int64_t)(j0 + j) * ld_a + r0 + i;
+                            const int64_t at = place(j0 + j, r0 + i);
                             float v[8];
                             along_column(i, j, v);
                             finish(v, at, -8);
@@ -986,7 +1022,8 @@ __global__ __launch_bounds__(64 * WM * WN) void fsadam_matrix_stage(const Matrix
                 if (row.tall) {  // a X + B X along the rows of X first, in the slab: its columns are what is written
 #pragma unroll
                     for (int n = 0; n < kMine; ++n) {
-                        const int e = threadIdx.x + n * Prod::kThreads, i = e / (TN / 8), j = (e % (TN / 8)) * 8;
+                        int i, j;
+                        piece(n, i, j);
                         if (j0 + j >= l64) continue;
                         float o[8];
                         along_row(i, j, o);
@@ -1000,17 +1037,16 @@ __global__ __launch_bounds__(64 * WM * WN) void fsadam_matrix_stage(const Matrix
                 }
 #pragma unroll
                 for (int n = 0; n < kMine; ++n) {
-                    const int e = threadIdx.x + n * Prod::kThreads;
                     int i, j;
                     float o[8], w[8];
                     if (row.tall) {
+                        const int e = threadIdx.x + n * Prod::kThreads;
                         j = e / (kSlab / 8);
                         i = (e % (kSlab / 8)) * 8;
                         if (r0 + i >= row.s || j0 + j >= row.l) continue;
                         along_column(i, j, o);
                     } else {
-                        i = e / (TN / 8);
-                        j = (e % (TN / 8)) * 8;
+                        piece(n, i, j);
                         if (r0 + i >= row.s || j0 + j >= row.l) continue;
                         along_row(i, j, o);
 #pragma unroll

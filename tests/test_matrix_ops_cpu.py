@@ -43,9 +43,8 @@ def up(v, m):
 def test_workspace_holds_two_x_and_the_square_matrices_of_every_matrix(products):
     rc, got = workspace(matrices((3, 300, 170), (1, 135, 200)), options(products=products))
     assert rc == 0
-    odd = lambda n: up(n, 64) if up(n, 64) // 64 % 2 else up(n, 64) + 64  # rows of an odd number of lines
-    x = lambda s, l: 2 * 2 * up(s, 64) * odd(l) * 2  # two buffers of two planes of halves
-    a = lambda s: (3 if products == 2 else 2) * products * up(s, 64) * odd(s) * 2  # 22 bits: two planes, and steps in pairs need a third matrix
+    x = lambda s, l: 2 * 2 * up(s, 64) * up(l, 64) * 2  # two buffers of two planes of halves
+    a = lambda s: (3 if products == 2 else 2) * products * up(s, 64) ** 2 * 2  # 22 bits: two planes, and steps in pairs need a third matrix
     body = 3 * (x(170, 300) + a(170)) + x(135, 200) + a(135)
     assert body < got < body + 4096  # and the tables
 
