@@ -509,12 +509,11 @@ int sources_of(const FsMatrix* m, int64_t n, int size, std::vector<Source>& list
         if (!aligned(r.src, size) || !aligned(r.dst, size)) return fail(FSADAM_EINVAL, name + ": pointer not aligned to its element size");
         for (int64_t ld : {r.src_ld, r.dst_ld})
             if (ld < r.cols || ld > (int64_t(1) << 40)) return fail(FSADAM_EINVAL, name + ": rows overlap (ld < cols), or lie too far apart");
-        const int64_t src_end = (r.rows - 1) * r.src_ld + r.cols, dst_end = (r.rows - 1) * r.dst_ld + r.cols;
+        const int64_t dst_end = (r.rows - 1) * r.dst_ld + r.cols;
         if (r.batch > 1 && (r.src_stride < 0 || r.dst_stride < dst_end || r.src_stride > (int64_t(1) << 40) || r.dst_stride > (int64_t(1) << 40)))
             return fail(FSADAM_EINVAL, name + ": matrices of the batch overlap, or lie too far apart");
         if (r.src == r.dst && (r.src_ld != r.dst_ld || (r.batch > 1 && r.src_stride != r.dst_stride)))
             return fail(FSADAM_EINVAL, name + ": results over the matrices need the same strides");
-        (void)src_end;
         list.push_back({r.src, nullptr, r.dst, nullptr, r.batch, r.rows, r.cols, r.src_ld, r.src_stride, r.dst_ld, r.dst_stride, 0.0f, size, size, 0});
     }
     return FSADAM_OK;

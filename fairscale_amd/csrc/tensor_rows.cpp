@@ -13,9 +13,10 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <pybind11/pybind11.h>
 
+#include <algorithm>
 #include <cstdint>
 #include <string>
-#include <unordered_set>
+#include <vector>
 
 namespace py = pybind11;
 
@@ -296,7 +297,7 @@ py::tuple fill_grad_rows(py::list grads, int dtype_code, int device, uintptr_t r
 
 // Rows of the matrix operators (include/fsadam.h: FsMomentumTensor, FsMuonTensor): `words` int64 a row, the pointers of the
 // lists' tensors first (0 where a list is None), then, for FsMomentumTensor, numel.  Tensors of a row are dense, contiguous, on one
-// device and of one shape; those of the lists named in `written` do not share memory with another of their list.
+// device and of one shape; those of the lists named in `written` share memory with nothing else.
 // dtype codes: 0 float32, 1 float16, 2 bfloat16.
 //
 // fill_matrix_rows(lists, dtype_codes, written, device_index, rows_address, words, with_numel) -> (status, list, index, None)
@@ -314,7 +315,14 @@ py::tuple fill_matrix_rows(py::tuple lists, py::tuple dtype_codes, py::tuple wri
     const int64_t n = PyList_GET_SIZE(PyTuple_GET_ITEM(lists.ptr(), 0));
     int64_t* rows = reinterpret_cast<int64_t*>(rows_address);
     try {
-        std::unordered_set<const void*> seen;
+        struct Span {
+            uintptr_t from, to;
+            bool written;
+        };
+        std::vector<Span> spans;  // of the tensors in memory
+        spans.reserve((size_t)(n * depth));
+        const bool in_place = with_numel;  // the momentum pass: updates (list 2) may lie over their own gradients (list 0)
+        std::vector<size_t> first_span(in_place ? (size_t)n : 0);
         for (int64_t d = 0; d < depth; ++d) {
             PyObject* lst = PyTuple_GET_ITEM(lists.ptr(), d);
             if (lst == Py_None) {
@@ -324,8 +332,7 @@ py::tuple fill_matrix_rows(py::tuple lists, py::tuple dtype_codes, py::tuple wri
             if (!PyList_Check(lst) || PyList_GET_SIZE(lst) != n) return stop(kLength, d, -1);
             const int code = dtype_codes[d].cast<int>();
             const c10::ScalarType dtype = code == 2 ? c10::ScalarType::BFloat16 : dtype_of_code(code);
-            const bool unshared = written.contains(py::int_(d));
-            seen.clear();
+            const bool writes = written.contains(py::int_(d));
             for (int64_t t = 0; t < n; ++t) {
                 const at::Tensor* x = plain_tensor(PyList_GET_ITEM(lst, t));
                 const at::Tensor* x0 = plain_tensor(PyList_GET_ITEM(PyTuple_GET_ITEM(lists.ptr(), 0), t));
@@ -333,10 +340,22 @@ py::tuple fill_matrix_rows(py::tuple lists, py::tuple dtype_codes, py::tuple wri
                 const int bad = check_tensor(*x, dtype, device, x0->numel());
                 if (bad) return stop(bad, d, t);
                 if (x->sizes() != x0->sizes()) return stop(kNumel, d, t);
-                if (unshared && x->numel() && !seen.insert(x->data_ptr()).second) return stop(kStale, d, t);
-                rows[t * words + d] = reinterpret_cast<int64_t>(x->data_ptr());
+                const uintptr_t at = reinterpret_cast<uintptr_t>(x->data_ptr()), end = at + x->nbytes();
+                rows[t * words + d] = (int64_t)at;
                 if (d == 0 && with_numel) rows[t * words + depth] = x->numel();
+                if (x->numel() == 0) continue;
+                if (in_place && d == 2 && spans[first_span[t]].from == at && spans[first_span[t]].to == end) spans[first_span[t]].written = true;
+                else spans.push_back({at, end, writes});
+                if (in_place && d == 0) first_span[t] = spans.size() - 1;
             }
+        }
+        // what is written may share memory with nothing else
+        std::sort(spans.begin(), spans.end(), [](const Span& a, const Span& b) { return a.from < b.from; });
+        uintptr_t end = 0, written_end = 0;
+        for (const Span& a : spans) {
+            if (a.from < (a.written ? end : written_end)) return stop(kStale, 0, -1);
+            end = std::max(end, a.to);
+            if (a.written) written_end = std::max(written_end, a.to);
         }
     } catch (const std::exception& e) {
         r.status = kError;

@@ -58,14 +58,15 @@ def workspace_for(size_call, device: torch.device, *arguments) -> Tuple[torch.Te
     return torch.empty(max(int(size.value), 256), dtype=torch.uint8, device=device), int(size.value)
 
 
-def refuse_shared(tensors: Sequence[torch.Tensor], what: str) -> None:
-    """A tensor that is written may be in a list only once."""
-    seen = set()
-    for t in tensors:
-        if t.numel():
-            if t.data_ptr() in seen:
-                raise RuntimeError(f"{what}: the same memory is in the list twice")
-            seen.add(t.data_ptr())
+def refuse_shared(written: Sequence[torch.Tensor], read: Sequence[torch.Tensor] = ()) -> None:
+    """Raises when a tensor that is written shares memory with another one (all contiguous)."""
+    spans = [(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), w) for ts, w in ((written, True), (read, False)) for t in ts if t.numel()]
+    end = written_end = 0
+    for start, stop, writes in sorted(spans):
+        if start < (end if writes else written_end):
+            raise RuntimeError("a tensor that is written shares memory with another one of the call (the same tensor twice, or overlapping views)")
+        end = max(end, stop)
+        written_end = max(written_end, stop) if writes else written_end
 
 
 def fill_rows(lists: Sequence[Optional[List[torch.Tensor]]], dtypes: Sequence[torch.dtype], written: Tuple[int, ...], device: torch.device,
@@ -92,8 +93,8 @@ def _check_momentum_lists(grads, momenta, updates, device, dtype, update_dtype) 
     for g, u in zip(grads, updates):
         if u.dtype != update_dtype or u.device != device or u.shape != g.shape or u.layout != torch.strided or not u.is_contiguous():
             raise RuntimeError("updates must be dense, contiguous tensors of one dtype with the gradients' shapes and device")
-    refuse_shared(momenta, "momenta")
-    refuse_shared(updates, "updates")
+    in_place = [u.data_ptr() == g.data_ptr() and u.element_size() == g.element_size() for g, u in zip(grads, updates)]
+    refuse_shared([*momenta, *updates], [g for g, own in zip(grads, in_place) if not own])
 
 
 @torch.no_grad()
@@ -109,8 +110,8 @@ def momentum_pass(grads: Sequence[torch.Tensor], momenta: Sequence[torch.Tensor]
         grads: tensors of one device and dtype (fp32, fp16 or bf16), dense and contiguous; any shapes.
         momenta: fp32 tensors of the same shapes, updated in place.
         scale: the gradients are divided by this: a float, or a one-element float32 tensor the kernel reads when it runs.
-        updates: tensors to write the updates to, of one dtype (any of the three); may be ``grads`` themselves.
-            Made in the gradients' dtype when None.
+        updates: tensors to write the updates to, of one dtype (any of the three); each may be its own gradient, if
+            their elements have one size, but share memory with nothing else.  Made in the gradients' dtype when None.
         found_inf: float32[1] device tensor to raise; a zeroed one is made when None.
     """
     grads, momenta = list(grads), list(momenta)
@@ -192,9 +193,10 @@ def orthogonalize(matrices: Sequence[torch.Tensor], *, steps: int = 5, coefficie
             count matrices (experts, heads: ``w.view(heads, -1, w.shape[-1])``).  Rows or columns must have neighbouring
             elements: slices of rows or columns and transposed matrices are taken as they are, others are refused.
         products: ``"half"`` multiplies 11 bits of the operands (error about 2e-3 of the result's norm), ``"split"`` 22 bits
-            (errors like fp32 products, at three times the matrix work; always taken where the short side is 128 or less).  None: as many as the results can hold, i.e.
-            ``"half"`` for bf16 and ``"split"`` for fp16 and fp32.
-        out: tensors to write the results to (of the same shapes, dtype and order of strides); may be ``matrices``.
+            (errors like fp32 products, at three times the matrix work; always taken where the short side is 128 or less).
+            None: as many as the results can hold, i.e. ``"half"`` for bf16 and ``"split"`` for fp16 and fp32.
+        out: tensors to write the results to (of the same shapes, dtype and order of strides).  Each may be its own matrix, but share
+            memory with no other one of the call; side by side in the columns of one tensor is no sharing.
     """
     matrices = list(matrices)
     if out is not None and len(out) != len(matrices):
@@ -217,7 +219,8 @@ def orthogonalize(matrices: Sequence[torch.Tensor], *, steps: int = 5, coefficie
         if layout is None:
             raise RuntimeError(f"a matrix needs rows or columns of neighbouring elements, got strides {tuple(t.stride())} for {tuple(t.shape)}")
         layouts.append(layout)
-    if out is None:
+    given = out is not None
+    if not given:
         out = [torch.empty(t.shape[:-2] + (t.shape[-1], t.shape[-2]), dtype=dtype, device=device).transpose(-2, -1) if layout[0]
                else torch.empty(t.shape, dtype=dtype, device=device) for t, layout in zip(matrices, layouts)]
     out = list(out)
@@ -236,13 +239,42 @@ def orthogonalize(matrices: Sequence[torch.Tensor], *, steps: int = 5, coefficie
         row.src, row.dst, row.batch = t.data_ptr(), o.data_ptr(), t.numel() // (m * n)
         row.rows, row.cols = (n, m) if turned else (m, n)
         row.src_ld, row.src_stride, row.dst_ld, row.dst_stride = ld, stride, into[1], into[2]
-    refuse_shared(out, "out")
+    if given:
+        _refuse_overlap(rows, matrices[0].element_size())
     lib = _cabi.lib()
     with torch.cuda.device(device):
         workspace, size = workspace_for(lib.fsadam_orth_workspace, device, rows, len(matrices), ctypes.byref(options))
         _cabi.check(lib.fsadam_orthogonalize(rows, len(matrices), TYPE_CODE[dtype], ctypes.byref(options), workspace.data_ptr(), size,
                                              int(torch.cuda.current_stream(device).cuda_stream)))
     return out
+
+
+def _refuse_overlap(rows, size: int) -> None:
+    """Raises when a result may lie over another matrix or result of the call.  Tensors of interleaved rows (slices of columns of one
+    tensor) are told apart by their columns where their rows are equally far apart; other interleavings are refused."""
+    spans = []
+    for k, r in enumerate(rows):
+        if not r.batch:
+            continue
+        in_place = (r.src, r.src_ld) == (r.dst, r.dst_ld) and (r.batch == 1 or r.src_stride == r.dst_stride)
+        for start, ld, stride, writes in ((r.dst, r.dst_ld, r.dst_stride, True),) + (() if in_place else ((r.src, r.src_ld, r.src_stride, False),)):
+            step = ld if r.rows > 1 else stride if r.batch > 1 else 0  # from row to row; 0: a single one, -1: not even
+            if r.rows > 1 and r.batch > 1 and stride % ld:
+                step = -1
+            spans.append((start, start + ((r.batch - 1) * stride + (r.rows - 1) * ld + r.cols) * size, writes, step, r.cols))
+    spans.sort()
+    live = []
+    for span in spans:
+        start, _, writes, step, cols = span
+        live = [s for s in live if s[1] > start]
+        for _start, _, _writes, _step, _cols in live:
+            if not (writes or _writes):
+                continue
+            shift, rest = divmod(start - _start, size)
+            apart = not rest and _step > 0 and step in (0, _step) and _cols <= shift % _step <= _step - cols
+            if not apart:
+                raise RuntimeError("out shares memory with another matrix of the call (only a matrix's own result may lie over it)")
+        live.append(span)
 
 
 def _layout_as(t: torch.Tensor, turned: bool) -> Optional[Tuple[bool, int, int]]:

@@ -97,11 +97,12 @@ class Muon(torch.optim.Optimizer):
 
     # ------------------------------------------------------------------ groups and state
 
-    def _check_group(self, group: Dict[str, Any], step: bool = False) -> None:
-        """Raises ValueError for settings the step cannot take; before a step only when they changed since they were looked at."""
+    def _check_group(self, group: Dict[str, Any], gi: int = -1) -> None:
+        """Raises ValueError for settings the step cannot take; before a step (of group ``gi``) only when they changed since the last."""
         settings = tuple(group[name] for name in _SETTINGS) + (self.products,)
         checked = self.__dict__.setdefault("_checked", {})
-        if step and checked.get(id(group)) == settings:
+        step = gi >= 0
+        if step and checked.get(gi) == settings:
             return
         if not 0.0 <= group["lr"] < math.inf:
             raise ValueError(f"Invalid learning rate: {group['lr']}")
@@ -123,11 +124,16 @@ class Muon(torch.optim.Optimizer):
         for p in group["params"]:
             if p.dtype != self._dtype:
                 raise ValueError(f"all parameters must share one dtype, got {self._dtype} and {p.dtype}")
-            if p.dim() < 2:
-                raise ValueError(f"Muon optimizes matrices, got a parameter of shape {tuple(p.shape)} (Adam takes it)")
-            if p.shape[-2] % blocks:
-                raise ValueError(f"{p.shape[-2]} rows cannot be split into {blocks} blocks")
-        checked[id(group)] = settings
+            self._check_shape(p, blocks)
+        if step:
+            checked[gi] = settings
+
+    @staticmethod
+    def _check_shape(p: torch.Tensor, blocks: int) -> None:
+        if p.dim() < 2:
+            raise ValueError(f"Muon optimizes matrices, got a parameter of shape {tuple(p.shape)} (Adam takes it)")
+        if p.shape[-2] % blocks:
+            raise ValueError(f"{p.shape[-2]} rows cannot be split into {blocks} blocks")
 
     def _add_masters(self, group: Dict[str, Any]) -> None:
         masters = []
@@ -181,6 +187,7 @@ class Muon(torch.optim.Optimizer):
             buf = state.get("momentum_buffer")
             if buf is None:
                 self._check_row(p, p, grad, None)
+                self._check_shape(p, int(group["row_blocks"]))
                 if torch.cuda.is_current_stream_capturing():
                     raise RuntimeError("a graph that makes the momentum would clear it at every replay: step once before the capture")
                 buf = state["momentum_buffer"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
@@ -207,33 +214,33 @@ class Muon(torch.optim.Optimizer):
             if t is not None and (t.dtype != torch.float32 or t.device != like.device or t.shape != like.shape or not t.is_contiguous()):
                 raise RuntimeError("momentum and master copies must be contiguous float32 tensors with their parameter's shape and device")
 
-    def _rows(self, group: Dict[str, Any], device: torch.device, lists: Tuple[List[torch.Tensor], ...]) -> np.ndarray:
+    def _rows(self, gi: int, group: Dict[str, Any], device: torch.device, lists: Tuple[List[torch.Tensor], ...]) -> np.ndarray:
         """FsMuonTensor rows of one call."""
         params, grads, bufs, likes = lists
         blocks, how = int(group["row_blocks"]), group["adjust_lr_fn"]
         rows = np.empty((len(params), 8), dtype=np.int64)
         copies = likes if self.mixed_precision else None
         stored = torch.float32 if self.mixed_precision else self._dtype
-        if device.type != "cuda" or not fill_rows((params, grads, bufs, copies), (stored, self._dtype, torch.float32, self._dtype), (0, 2), device, rows):
+        if device.type != "cuda" or not fill_rows((params, grads, bufs, copies), (stored, self._dtype, torch.float32, self._dtype), (0, 2, 3), device, rows):
             for p, like, grad, buf in zip(params, likes, grads, bufs):
                 self._check_row(p, like, grad, buf)
-            refuse_shared(params, "parameters")
-            refuse_shared(bufs, "momenta")
+            refuse_shared([*params, *bufs, *(copies or ())], grads)
             rows[:, :4] = [(p.data_ptr(), g.data_ptr(), m.data_ptr(), c.data_ptr() if copies else 0) for p, g, m, c in zip(params, grads, bufs, likes)]
         # batch, rows, cols and ratio go by the shapes alone
         shapes = (blocks, how, tuple(p.shape for p in params))
-        cached = self.__dict__.setdefault("_geometry", {}).get(id(group))
+        cached = self.__dict__.setdefault("_geometry", {}).get((gi, device))
         if cached is None or cached[0] != shapes:
             cells = np.empty((len(params), 4), dtype=np.int64)
             ratios = cells.view(np.float64)
             for k, p in enumerate(params):
+                self._check_shape(p, blocks)
                 height, cols = p.shape[-2] // blocks, p.shape[-1]
                 cells[k, :3] = p.numel() // (height * cols) if p.numel() else 0, height, cols
                 if how == "match_rms_adamw":
                     ratios[k, 3] = 0.2 * math.sqrt(max(height, cols))
                 else:
                     ratios[k, 3] = math.sqrt(max(1.0, height / cols)) if cols else 1.0
-            cached = self._geometry[id(group)] = (shapes, cells)
+            cached = self._geometry[gi, device] = (shapes, cells)
         rows[:, 4:] = cached[1]
         return rows
 
@@ -250,9 +257,9 @@ class Muon(torch.optim.Optimizer):
         loss = closure() if closure is not None else None
         calls = []
         for gi, group in enumerate(self.param_groups):
-            self._check_group(group, step=True)
+            self._check_group(group, gi)
             for device, lists in self._gather(gi, group).items():
-                calls.append((group, device, self._rows(group, device, lists), *scale_arguments(scale, device)))
+                calls.append((group, device, self._rows(gi, group, device, lists), *scale_arguments(scale, device)))
         if torch.autograd._profiler_enabled():
             with torch.autograd.profiler.record_function("fairscale_amd::muon::fused_step"):
                 for call in calls:

@@ -288,3 +288,62 @@ def test_workspace_of_matrices_that_fit_a_compute_unit():
     assert rc == 0 and 0 < got < 8192
     assert workspace(matrices((1, 129, 129)), options())[1] > 0
     assert workspace(matrices((1, 64, 4096)), options())[1] > 0
+
+
+def orth_row(src, dst, src_ld, dst_ld, shape=(3, 4), batch=1, src_stride=0, dst_stride=0):
+    row = _cabi.FsMatrix()
+    row.src, row.dst, row.batch = src, dst, batch
+    row.rows, row.cols = shape
+    row.src_ld, row.dst_ld, row.src_stride, row.dst_stride = src_ld, dst_ld, src_stride, dst_stride
+    return row
+
+
+@pytest.mark.parametrize("rows, apart", [
+    ([orth_row(1000, 2000, 4, 4), orth_row(3000, 4000, 4, 4)], True),
+    ([orth_row(1000, 1000, 4, 4), orth_row(2000, 2000, 4, 4)], True),                  # in place
+    ([orth_row(1000, 2000, 4, 4), orth_row(1000, 3000, 4, 4)], True),                  # one matrix read twice
+    ([orth_row(1000, 2000, 4, 4), orth_row(2000, 1000, 4, 4)], False),                 # exchanged
+    ([orth_row(1000, 3000, 4, 4), orth_row(2000, 3000, 4, 4)], False),                 # the same result twice
+    ([orth_row(1000, 1004, 4, 4)], False),                                             # shifted by an element
+    ([orth_row(1000, 1000, 4, 8)], False),                                             # other strides
+    ([orth_row(1000, 1000, 8, 8), orth_row(1016, 1016, 8, 8)], True),                  # halves of the columns
+    ([orth_row(1000, 1000, 8, 8), orth_row(1012, 1012, 8, 8)], False),                 # they share a column
+    ([orth_row(1000, 1000, 8, 8), orth_row(1020, 1020, 8, 8)], False),                 # the second runs into the next row
+    ([orth_row(1000, 1000, 8, 8), orth_row(1016, 1016, 9, 9)], False),                 # not told apart
+    ([orth_row(1000, 1000, 8, 8), orth_row(1018, 1018, 8, 8)], False),                 # not by whole elements
+    ([orth_row(1000, 1000, 8, 8), orth_row(1048, 1048, 4, 4, (1, 4))], True),          # a single row in a gap
+    ([orth_row(1000, 1000, 8, 8), orth_row(1044, 1044, 4, 4, (1, 4))], False),
+    ([orth_row(1000, 1000, 8, 8, (3, 4), 2, 24, 24), orth_row(1016, 1016, 8, 8, (3, 4), 2, 24, 24)], True),
+    ([orth_row(1000, 1000, 8, 8, (3, 4), 2, 28, 28), orth_row(1016, 1016, 8, 8, (3, 4), 2, 24, 24)], False),
+    ([orth_row(1000, 1000, 4, 4, (1, 4), 5, 8, 8), orth_row(1016, 1016, 4, 4, (1, 4), 5, 8, 8)], True),
+])
+def test_results_that_share_memory_are_refused(rows, apart):
+    if apart:
+        matrix_ops._refuse_overlap(rows, 4)
+    else:
+        with pytest.raises(RuntimeError, match="shares memory"):
+            matrix_ops._refuse_overlap(rows, 4)
+
+
+def test_tensors_that_are_written_share_memory_with_nothing():
+    base = torch.zeros(64)
+    a, b, c = base[:16], base[16:32], base[8:24]
+    matrix_ops.refuse_shared([a, b], [base[32:], base[40:]])
+    matrix_ops.refuse_shared([a], [b, c[8:], torch.empty(0)])
+    for written, read in (([a, a], []), ([a, c], []), ([a], [c]), ([c], [a]), ([b], [base]), ([base], [b])):
+        with pytest.raises(RuntimeError, match="shares memory"):
+            matrix_ops.refuse_shared(written, read)
+
+
+def test_optimizer_looks_at_parameters_that_come_later():
+    w = torch.nn.Parameter(torch.zeros(6, 4))
+    opt = Muon([w], row_blocks=2)
+    group = opt.param_groups[0]
+    for bad in (torch.zeros(5), torch.zeros(5, 4)):
+        p = torch.nn.Parameter(bad)
+        with pytest.raises(ValueError):
+            opt._check_shape(p, int(group["row_blocks"]))
+    opt._check_group(group, 0)
+    group["row_blocks"] = 4
+    with pytest.raises(ValueError, match="cannot be split"):
+        opt._check_group(group, 0)

@@ -559,3 +559,45 @@ def test_what_a_matrix_gives_does_not_depend_on_the_list(products, others):
 def test_momentum_pass_over_empty_tensors_only():
     got = momentum_pass([torch.zeros(0, device="cuda"), torch.zeros(3, 0, device="cuda")], [torch.zeros(0, device="cuda"), torch.zeros(3, 0, device="cuda")])
     assert got.found_inf.item() == 0.0 and (got.norms == 0).all()
+
+
+# ---- memory shared between the tensors of a call -------------------------------------------------------------------
+
+@pytest.mark.parametrize("rows", [90, 300])
+def test_halves_of_the_columns_of_one_tensor_in_place(rows):
+    whole = randn(rows, 400, seed=3)
+    left, right = whole[:, :160], whole[:, 160:]
+    want = [t.clone() for t in orthogonalize([left, right])]
+    orthogonalize([left, right], out=[left, right])
+    assert torch.equal(left, want[0]) and torch.equal(right, want[1])
+
+
+@pytest.mark.parametrize("rows", [20, 300])
+def test_calls_whose_results_share_memory_are_refused_and_change_nothing(rows):
+    a, b, g = randn(rows, 320, seed=1), randn(rows, 320, seed=2), randn(rows, 320, seed=3)
+    flat = torch.zeros(rows * 320 + 8, device="cuda")
+    shifted = [flat[:rows * 320].view(rows, 320), flat[4:4 + rows * 320].view(rows, 320)]
+    keep = [t.clone() for t in (a, b, g, flat)]
+    for call in (lambda: orthogonalize([a, b], out=[b, a]), lambda: orthogonalize([a, b], out=[a, a]), lambda: orthogonalize([a, b], out=shifted),
+                 lambda: orthogonalize([shifted[0]], out=[shifted[1]]), lambda: momentum_pass([g], [a], updates=[a]),
+                 lambda: momentum_pass([g, b], [a, b]), lambda: momentum_pass([g, b], [a, randn(rows, 320)], updates=[b, g]),
+                 lambda: momentum_pass([g, b], shifted), lambda: momentum_pass([shifted[0]], [shifted[1]])):
+        with pytest.raises(RuntimeError, match="share"):
+            call()
+    p = [torch.nn.Parameter(t) for t in shifted]
+    for q in p:
+        q.grad = torch.ones_like(q)
+    with pytest.raises(RuntimeError, match="share"):
+        Muon(p).step()
+    assert all(torch.equal(t, k) for t, k in zip((a, b, g, flat), keep))
+
+
+def test_parameters_in_one_buffer():
+    flat = randn(2 * 300 * 200, seed=5)
+    apart = [torch.nn.Parameter(t.clone()) for t in flat.view(2, 300, 200)]
+    together = [torch.nn.Parameter(t) for t in flat.view(2, 300, 200)]
+    for ps in (apart, together):
+        for k, p in enumerate(ps):
+            p.grad = randn(300, 200, seed=6 + k)
+        Muon(ps, lr=0.1).step()
+    assert torch.equal(flat.view(2, 300, 200), torch.stack([p.detach() for p in apart]))
