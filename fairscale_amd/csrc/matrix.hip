@@ -144,6 +144,15 @@ struct Chunk {
     bool pairs() const { return products == FSADAM_PRODUCTS_SPLIT; }  // steps are taken two at a time (run_chunk)
     int64_t head_bytes() const { return up((int64_t)rows.size() * sizeof(MatrixRow), 256) + up(matrices * 8, 256) + up(tiles[kTilesChunk] * 8, 256); }
     int64_t bytes() const { return head_bytes() + halves * 2; }
+    int64_t mean_depth() const {  // of the updates' products, over their tiles
+        int64_t tiles = 0, deep = 0;
+        for (const MatrixRow& row : rows) {
+            const int64_t n = (int64_t)row.batch * row.n[kTilesFull64];
+            tiles += n;
+            deep += n * row.s64;
+        }
+        return std::max<int64_t>(64, deep / std::max<int64_t>(1, tiles));
+    }
 };
 
 int64_t symmetric_tiles(int64_t s, int64_t t) { const int64_t n = (s + t - 1) / t; return n * (n + 1) / 2; }
@@ -299,15 +308,18 @@ int check_shape(int64_t t, int64_t batch, int64_t rows, int64_t cols) {
 // The tile of a launch: 64, 128 or 256 square, by what the busiest compute unit is given to do.  A unit of 64 x 64 is 13, what
 // takes 0.65 us per 64 of depth with 22-bit products; 128 takes 1.5 us and 256 takes 4.6 us, so that the larger tiles do 1.7 and
 // 2.2 times the work in the same time -- where there are enough of them for 256 compute units.  (11-bit products: about half
-// the times in the same proportion.)  Six matrices of 768 x 2304 and six of 768 x 768: update 101 / 99 / 73 us with
-// 64 / 128 / 256, square products 33 / 33 / 65.
+// the times in the same proportion.)  With 64 / 128 / 256, 22 bits, six matrices of 768 x 2304 and six of 768 x 768: update
+// 101 / 73 / 73 us, square products 34 / 29 / 61.  11 bits, 4096 x 4096: update 268 / 178 / 145 us, square products 155 / 117 / 137.
+// `last`: what a round of 256 takes longer when the parameters are updated in it.  Their traffic comes in one burst behind the
+// products, with nothing on the compute unit to do meanwhile; two workgroups of 128 share one and take turns.  Per 64 of depth it
+// weighs the less the deeper the products are.  With 128 / 256: the matrices above (768 deep) 95 / 112 us, a layer's (4096 deep) 2.18 / 1.88 ms.
 struct Tiles {
     int size;
     int64_t count;
 };
-Tiles choose_tiles(int64_t t64, int64_t t128, int64_t t256) {
+Tiles choose_tiles(int64_t t64, int64_t t128, int64_t t256, int64_t last) {
     const auto cost = [](int64_t tiles, int64_t unit) { return (tiles + 255) / 256 * unit; };
-    const int64_t c64 = cost(t64, 13), c128 = cost(t128, 30), c256 = cost(t256, 92);
+    const int64_t c64 = cost(t64, 13), c128 = cost(t128, 30), c256 = cost(t256, 92 + last);
     if (c256 < c128 && c256 < c64) return {256, t256};
     if (c128 < c64) return {128, t128};
     return {64, t64};
@@ -315,7 +327,11 @@ Tiles choose_tiles(int64_t t64, int64_t t128, int64_t t256) {
 
 template <int STAGE, int TILE, int PLANES>
 void launch_tile(int64_t count, int n_rows, const MatrixRow* table, const StageArgs& k, _Float16* work, hipStream_t stream) {
-    constexpr int WM = 2, WN = TILE == 64 ? 2 : 4, BK = column_block(PLANES), DEPTH = TILE == 64 && PLANES == 2 ? 4 : 2;
+    constexpr int WM = 2, WN = TILE == 64 ? 2 : 4, BK = column_block(PLANES);
+    // Panels on their way.  Tiles of 64 are taken where there are few of them, one workgroup to a compute unit: what hides the loads'
+    // latency is then its own panels alone (11 bits, 2 / 3 / 4 panels: 512 x 2048 184 / 165 / 164 us, four of 512 x 1024 155 / 149 / 150; 22
+    // bits, half as deep, 3 / 4 / 6: 231 / 225 / 226, 214 / 207 / 228).  Larger tiles have no room for a third.
+    constexpr int DEPTH = TILE > 64 ? 2 : PLANES == 2 ? 4 : 3;
     if (count) hipLaunchKernelGGL((fsadam_matrix_stage<STAGE, TILE, TILE, WM, WN, BK, DEPTH, PLANES>), dim3((uint32_t)count), dim3(64 * WM * WN), 0, stream, table, n_rows, k, work);
 }
 
@@ -323,7 +339,8 @@ template <int STAGE, int PLANES>
 int launch_stage(const Chunk& c, const MatrixRow* table, StageArgs k, _Float16* work, hipStream_t stream) {
     constexpr int kind = STAGE == kStageGram ? 2 : STAGE == kStageSquare ? 0 : 1;
     const int n = (int)c.rows.size();
-    const Tiles t = choose_tiles(c.tiles[kTilesSym64 + kind], c.tiles[kTilesSym128 + kind], c.tiles[kTilesSym256 + kind]);
+    const int64_t last = STAGE == kStageStep ? 550 * 64 / c.mean_depth() : 0;
+    const Tiles t = choose_tiles(c.tiles[kTilesSym64 + kind], c.tiles[kTilesSym128 + kind], c.tiles[kTilesSym256 + kind], last);
     if (t.size == 256) launch_tile<STAGE, 256, PLANES>(t.count, n, table, k, work, stream);
     else if (t.size == 128) launch_tile<STAGE, 128, PLANES>(t.count, n, table, k, work, stream);
     else if (STAGE != kStageGram) launch_tile<STAGE, 64, PLANES>(t.count, n, table, k, work, stream);
