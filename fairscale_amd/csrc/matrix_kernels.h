@@ -20,7 +20,7 @@
 //
 // Storage in the workspace, all sizes padded to 64 with zeros (zero rows and columns stay zero through the iteration,
 // so no product needs a mask): X is s64 x l64, A and B are s64 x s64, the planes one behind the other.  A matrix lies in blocks of
-// kBlock columns (what a panel of a product is deep: 64 halves, 32 with two planes), each block's rows one behind the other: a
+// column_block() columns (what a panel of a product is deep: 64 halves, 32 with two planes), each block's rows one behind the other: a
 // panel's rows, wherever it is cut, are then one contiguous span, every load of a wave 1 KiB of it.  Row-major, a wave's load
 // of 64-byte pieces fills half lines only and gets through at half the rate (62 against 115 GB/s for a compute unit).
 #pragma once
@@ -338,7 +338,10 @@ __device__ __forceinline__ void for_eights(int64_t begin, int64_t end, Each&& ea
     }
 }
 
-// Bound by HBM: 2 + 4 bytes read and 2 + 4 written per element with 16-bit gradients and updates.
+// Bound by HBM: 2 + 4 bytes read and 2 + 4 written per element with 16-bit gradients and updates.  The matrices of a layer of 4096
+// with an FFN of 11008 (202 million elements): 376 us, 6.46 TB/s, where a plain copy of a tensor reaches 4.8 and this library's
+// parameter pass 6.7.  Short workgroups of one piece a thread, all loads before the first store, and stores that write through
+// the L2 (store_through) as in the parameter pass; the L2 would hold the lines until they are in the way of the reads.
 template <int GT, int UT, typename Table>
 __global__ __launch_bounds__(kChunkThreads) void fsadam_momentum_chunks(Table tables, MomentumArgs k, double* partials, float* cleared) {
     if (cleared && blockIdx.x == 0 && threadIdx.x == 0) *cleared = 0.0f;
@@ -423,7 +426,9 @@ __global__ __launch_bounds__(kNormThreads) void fsadam_momentum_norms(Table tabl
 
 // ---- norms and normalisation of the matrices ----------------------------------------------------------------------
 
-// STEP: the source is the gradient, the momentum is updated and what is summed is the update.
+// STEP: the source is the gradient, the momentum is updated and what is summed is the update, which is not stored: the next pass
+// makes it again from the gradient and the new momentum, 6 bytes read in place of 4 written and 4 read.  Bound by HBM: 16-bit
+// gradients, 202 million elements: 342 us, 5.9 TB/s.  Where X is read alone (4096 x 4096 bf16, 34 MB): 8.8 us, 3.8 TB/s.
 template <int ST, bool STEP>
 __global__ __launch_bounds__(kChunkThreads) void fsadam_matrix_chunks(const MatrixRow* table, int n_rows, MomentumArgs k, double* partials) {
     int matrix;
@@ -485,7 +490,8 @@ __global__ __launch_bounds__(kChunkThreads) void fsadam_matrix_norms(const Matri
     }
 }
 
-// X0 * 2^k as two halves, 64 x 64 elements a workgroup, turned where the matrix is tall; the padding is written as zeros.
+// X0 * 2^k as two halves, 64 x 64 elements a workgroup, turned (through LDS) where the matrix is tall; the padding is written as
+// zeros.  Bound by HBM: 16-bit gradients and momentum in, 10 bytes an element in all: 8 x 1024 x 2816 and turned 83 us, 5.5 TB/s.
 template <int ST, bool STEP>
 __global__ __launch_bounds__(256) void fsadam_matrix_normalise(const MatrixRow* table, int n_rows, MomentumArgs k, const double* inverse, double power, int log_block,
                                                                 _Float16* work) {
@@ -594,6 +600,14 @@ __device__ __forceinline__ void loads_arrived() {  // all but the last LEFT load
 }
 __device__ __forceinline__ uint32_t lds_address(const void* p) { return (uint32_t)(uintptr_t)(FM_LDS const void*)p; }
 
+// What bounds it.  With two planes every 32 of depth take three matrix instructions for each pair of fragments, and the matrix cores
+// are busy 72 % of the time at the 1.9 GHz that the power limit leaves: update of 5120 x 13824 in 1.73 ms, 419 TFLOP/s, which is
+// 1.26 PFLOP/s of matrix instructions; a plain 16-bit matrix product of the library runs at 1.26 to 1.32 PFLOP/s on this card.
+// With one plane the panels' way from the L2 to LDS is the longer part (64 KiB per 64 of depth of a 256 x 256 tile, at 100 to
+// 135 GB/s a compute unit): update of 4096 x 4096 in 141 us, 975 TFLOP/s.
+// Fragments: lane (g, c) of 16 x 4 holds row c, eight deep from 8 g on; NN operands lie deep-major and are turned by the
+// transposing LDS loads, four deep of 16 columns each.
+//
 // C tile (TM x TN) = P Q^T (NT) or P Q (NN) over K, by WM x WN waves; the caller's epilogue takes acc.  DEPTH panels are in LDS:
 // one is multiplied while the others are on their way.
 template <int TM, int TN, int WM, int WN, int BK, int DEPTH, int PLANES, bool NN>
@@ -817,7 +831,10 @@ struct Product {
     }
 };
 
-// One stage of the iteration over every matrix of the chunk.
+// One stage of the iteration over every matrix of the chunk.  The tile is chosen on the host (choose_tiles), a product's result stays
+// in registers until its epilogue: the polynomial, the mirror image of a symmetric result, the split into halves, or the
+// update of the parameters.  Accumulators pass through LDS, 64 rows at a time, so that every store and every load of what is
+// added is 16 bytes of a line that its neighbours fill.
 template <int STAGE, int TM, int TN, int WM, int WN, int BK, int DEPTH, int PLANES>
 __global__ __launch_bounds__(64 * WM * WN) void fsadam_matrix_stage(const MatrixRow* table, int n_rows, StageArgs k, _Float16* work) {
     constexpr bool kSym = STAGE <= kStageSquare;
@@ -1074,7 +1091,9 @@ __global__ __launch_bounds__(64 * WM * WN) void fsadam_matrix_stage(const Matrix
 // ---- matrices that fit a compute unit's LDS -----------------------------------------------------------------------
 
 // One workgroup takes a matrix from the source to the result: X (two planes) and one square matrix stay in LDS, products
-// go through registers, nothing is written to memory in between.  All the launches and the trips to the L2 and back
+// go through registers, nothing is written to memory in between.  Bound by latency: a compute unit reads its operands from LDS at
+// 128 bytes a clock, and between the products all its waves wait for each other.  Five steps of 16 x 16 16 us, 64 x 256 36 us, 128 x 128 73 us, where the launches of the
+// stages take 100 us for any matrix this small.  All the launches and the trips to the L2 and back
 // that the stages above are made of are what such a matrix would wait for.
 struct alignas(16) ResidentRow {
     const void* src;

@@ -293,6 +293,11 @@ int fsadam_grad_pass_noalloc(const FsGradTensor* grads, int64_t n_tensors, int g
 #define FSADAM_TYPE_F16 1
 #define FSADAM_TYPE_BF16 2
 
+/* The calls below keep nothing: rows are read before the call returns, scratch memory is the caller's (`workspace`, as many bytes as the
+ * *_workspace call says for the same rows and options, aligned to 256; it belongs to the call until the stream has passed it).  They
+ * enqueue on the given stream of the current device, never wait, and may be recorded into a graph.  What a call writes (and its
+ * workspace) may share memory with nothing else of the call but where said so. */
+
 /* Momentum pass, for every element of every tensor, in fp32 as written:
  *     r = g / scale;   m <- m + (r - m) * (1 - momentum);   u = nesterov ? r + (m - r) * momentum : m
  * m is updated in place; u is stored in update_type (u may be g itself where the types are the same: updates over the
@@ -318,7 +323,7 @@ int fsadam_momentum_pass(const FsMomentumTensor* tensors, int64_t n_tensors, int
  * the result about 2e-3 of its norm), FSADAM_PRODUCTS_SPLIT 22 (like fp32 products, about three times the work; always
  * taken for matrices of a short side up to 128).
  * Refused with FSADAM_EINVAL: coefficients that let singular values in [0, 1] grow past 1024 within the steps, steps
- * outside 1..32, eps that is not positive, sides over 2^20. */
+ * outside 1..32, eps that is not positive, sides or batches over 2^20, matrices of more than 2^34 elements. */
 #define FSADAM_PRODUCTS_HALF 1
 #define FSADAM_PRODUCTS_SPLIT 2
 typedef struct FsOrthOptions {
