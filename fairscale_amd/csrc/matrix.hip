@@ -325,14 +325,22 @@ Tiles choose_tiles(int64_t t64, int64_t t128, int64_t t256, int64_t last) {
     return {64, t64};
 }
 
-template <int STAGE, int TILE, int PLANES>
+template <int STAGE, int TILE, int PLANES, int DEPTH>
 void launch_tile(int64_t count, int n_rows, const MatrixRow* table, const StageArgs& k, _Float16* work, hipStream_t stream) {
     constexpr int WM = 2, WN = TILE == 64 ? 2 : 4, BK = column_block(PLANES);
-    // Panels on their way.  Tiles of 64 are taken where there are few of them, one workgroup to a compute unit: what hides the loads'
-    // latency is then its own panels alone (11 bits, 2 / 3 / 4 panels: 512 x 2048 184 / 165 / 164 us, four of 512 x 1024 155 / 149 / 150; 22
-    // bits, half as deep, 3 / 4 / 6: 231 / 225 / 226, 214 / 207 / 228).  Larger tiles have no room for a third.
-    constexpr int DEPTH = TILE > 64 ? 2 : PLANES == 2 ? 4 : 3;
     if (count) hipLaunchKernelGGL((fsadam_matrix_stage<STAGE, TILE, TILE, WM, WN, BK, DEPTH, PLANES>), dim3((uint32_t)count), dim3(64 * WM * WN), 0, stream, table, n_rows, k, work);
+}
+
+// Panels in LDS.  Tiles of 64 are taken where there are few of them, one workgroup to a compute unit: what hides the loads' latency is
+// then its own panels alone (11 bits, 2 / 3 / 4 panels: 512 x 2048 184 / 165 / 164 us, four of 512 x 1024 155 / 149 / 150; 22 bits, half as
+// deep, 3 / 4 / 6: 231 / 225 / 226, 214 / 207 / 228).  Tiles of 128 take four panels while no compute unit has two of them (11 bits, 2 / 4
+// panels: 1600 x 1600 287 / 262 us, 2048 x 2048 417 / 377; with 22 bits, where the two groups of waves wait for something else, 816 /
+// 801 and no difference elsewhere: left at two).  256 has no room for a third.
+template <int STAGE, int TILE, int PLANES>
+void launch_tiles(int64_t count, int n_rows, const MatrixRow* table, const StageArgs& k, _Float16* work, hipStream_t stream) {
+    if constexpr (TILE == 128)
+        PLANES == 1 && count <= 256 ? launch_tile<STAGE, TILE, PLANES, PLANES == 1 ? 4 : 2>(count, n_rows, table, k, work, stream) : launch_tile<STAGE, TILE, PLANES, 2>(count, n_rows, table, k, work, stream);
+    else launch_tile<STAGE, TILE, PLANES, TILE == 256 ? 2 : PLANES == 2 ? 4 : 3>(count, n_rows, table, k, work, stream);
 }
 
 template <int STAGE, int PLANES>
@@ -341,13 +349,13 @@ int launch_stage(const Chunk& c, const MatrixRow* table, StageArgs k, _Float16* 
     const int n = (int)c.rows.size();
     const int64_t last = STAGE == kStageStep ? 550 * 64 / c.mean_depth() : 0;
     const Tiles t = choose_tiles(c.tiles[kTilesSym64 + kind], c.tiles[kTilesSym128 + kind], c.tiles[kTilesSym256 + kind], last);
-    if (t.size == 256) launch_tile<STAGE, 256, PLANES>(t.count, n, table, k, work, stream);
-    else if (t.size == 128) launch_tile<STAGE, 128, PLANES>(t.count, n, table, k, work, stream);
-    else if (STAGE != kStageGram) launch_tile<STAGE, 64, PLANES>(t.count, n, table, k, work, stream);
+    if (t.size == 256) launch_tiles<STAGE, 256, PLANES>(t.count, n, table, k, work, stream);
+    else if (t.size == 128) launch_tiles<STAGE, 128, PLANES>(t.count, n, table, k, work, stream);
+    else if (STAGE != kStageGram) launch_tiles<STAGE, 64, PLANES>(t.count, n, table, k, work, stream);
     if constexpr (STAGE == kStageGram) {  // split products are in tiles of 64; the others join their launch where they are too
         k.kind = t.size == 64 ? kTilesAllParts : kTilesPart;
-        launch_tile<kStageGram, 64, PLANES>(c.tiles[k.kind], n, table, k, work, stream);
-        launch_tile<kStageJoin, 64, PLANES>(c.tiles[kTilesJoin], n, table, k, work, stream);
+        launch_tiles<kStageGram, 64, PLANES>(c.tiles[k.kind], n, table, k, work, stream);
+        launch_tiles<kStageJoin, 64, PLANES>(c.tiles[kTilesJoin], n, table, k, work, stream);
     }
     return launched();
 }

@@ -601,3 +601,38 @@ def test_parameters_in_one_buffer():
             p.grad = randn(300, 200, seed=6 + k)
         Muon(ps, lr=0.1).step()
     assert torch.equal(flat.view(2, 300, 200), torch.stack([p.detach() for p in apart]))
+
+
+# ---- sizes -----------------------------------------------------------------------------------------------------------
+
+def test_lists_of_several_thousand_rows():
+    """Every matrix of a long list is found: more rows than a wave looks at once, and more than 64 times as many."""
+    shapes = [(3, 5), (150, 140), (1, 1), (0, 4)]
+    us = [randn(*shapes[k % 4], seed=k % 12) for k in range(4500)]
+    alone = {k: orthogonalize([us[k]])[0] for k in range(12)}
+    got = orthogonalize(us)
+    assert all(torch.equal(o, alone[k % 12]) for k, o in enumerate(got))
+    stats = momentum_pass(us, [torch.zeros_like(u) for u in us], 0.5, nesterov=False)
+    want = [momentum_pass([us[k]], [torch.zeros_like(us[k])], 0.5, nesterov=False) for k in range(12)]
+    assert all(torch.equal(u, want[k % 12].updates[0]) for k, u in enumerate(stats.updates))
+    assert torch.equal(stats.norms, torch.cat([w.norms for w in want]).repeat(375))
+
+
+@pytest.mark.parametrize("tall", [False, True])
+def test_matrix_of_more_than_2_31_elements(tall):
+    """Entries only at (i, 2 i): the singular values are their sizes, so the result has the polynomial's values there and zeros elsewhere."""
+    s, l = 32800, 65600
+    d = torch.full((s,), 0.25, device="cuda")
+    d[:3], d[-3:], d[s // 2] = 300.0, -200.0, 250.0
+    u = torch.zeros((l, s) if tall else (s, l), dtype=torch.bfloat16, device="cuda")
+    at = lambda t: t.as_strided((s,), (2 * s + 1,) if tall else (l + 2,))
+    at(u).copy_(d)
+    out = orthogonalize([u], steps=1)[0]
+    x = d.double() / d.double().norm()
+    want = 3.4445 * x - 4.7750 * x**3 + 2.0315 * x**5
+    got = at(out).double()
+    # 11 bits of A, B and X in the products and 8 in the result: (|b| x^3 * 3 + |c| x^5 * 5) 2^-11 + |result| 2^-8, and an fp32 sum's 2^-20
+    bound = (3 * 4.7750 * x.abs()**3 + 5 * 2.0315 * x.abs()**5) * 2.0**-11 + want.abs() * (2.0**-8 + 2.0**-20) + 1e-9
+    assert ((got - want).abs() <= bound).all()
+    at(out).zero_()
+    assert int(torch.count_nonzero(out)) == 0
