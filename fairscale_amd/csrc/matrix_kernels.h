@@ -359,8 +359,15 @@ __global__ __launch_bounds__(kChunkThreads) void fsadam_momentum_chunks(Table ta
     if (cleared && blockIdx.x == 0 && threadIdx.x == 0) *cleared = 0.0f;
     const MomentumRow* table = rows_of(tables);
     const int n_rows = tables.n;
+    // by halving: workgroups this short find the table in the scalar cache (a layer's list 382 us; with find_row 404)
+    int low = 0, high = n_rows - 1;
     const int64_t t = blockIdx.x;
-    const MomentumRow& row = table[find_row(n_rows, t, [&](int r) { return table[r].first; })];
+    while (low < high) {
+        const int mid = (low + high + 1) >> 1;
+        if (table[mid].first <= t) low = mid;
+        else high = mid - 1;
+    }
+    const MomentumRow& row = table[low];
     const int64_t begin = (t - row.first) * kMomentumElems;
     const int64_t end = begin + kMomentumElems < row.numel ? begin + kMomentumElems : row.numel;
     const Divisor by(k);
