@@ -95,6 +95,10 @@ class Muon(torch.optim.Optimizer):
     def supports_memory_efficient_fp16(self) -> bool:
         return True
 
+    def __getstate__(self) -> Dict[str, Any]:  # of copies and pickles
+        return {**super().__getstate__(), "precision": self.precision, "products": self.products, "_dtype": self._dtype,
+                "fp32_param_groups": self.fp32_param_groups}
+
     # ------------------------------------------------------------------ groups and state
 
     def _check_group(self, group: Dict[str, Any], gi: int = -1) -> None:

@@ -2,8 +2,10 @@
 sizes are those of the documented storage, and the Python layer names what it will not take."""
 from __future__ import annotations
 
+import copy
 import ctypes
 import math
+import pickle
 
 import pytest
 import torch
@@ -347,3 +349,16 @@ def test_optimizer_looks_at_parameters_that_come_later():
     group["row_blocks"] = 4
     with pytest.raises(ValueError, match="cannot be split"):
         opt._check_group(group, 0)
+
+
+def test_optimizer_is_copied_whole():
+    w = torch.nn.Parameter(torch.randn(6, 4).half())
+    opt = Muon([w], lr=0.5, products="half")
+    for twin in (copy.deepcopy(opt), pickle.loads(pickle.dumps(opt))):
+        p = twin.param_groups[0]["params"][0]
+        assert p is not w and torch.equal(p, w)
+        assert (twin.precision, twin.products, twin.param_groups[0]["lr"]) == (Precision.MIXED_PRECISION, "half", 0.5)
+        assert twin.fp32_param_groups[0]["params"][0] is twin.state[p]["master"] and torch.equal(twin.state[p]["master"], w.float())
+        with pytest.raises(RuntimeError):
+            p.grad = torch.zeros_like(p)
+            twin.step()  # not on a GPU; gets as far as the check
