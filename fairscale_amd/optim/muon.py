@@ -82,10 +82,15 @@ class Muon(torch.optim.Optimizer):
         self._dtype = first_dtype
         for group in self.param_groups:
             self._check_group(group)
-        self.fp32_param_groups: List[Dict[str, Any]] = []
-        if self.mixed_precision:
-            for group in self.param_groups:
-                self._add_masters(group)
+        self._make_masters(self.param_groups)
+
+    @property
+    def fp32_param_groups(self) -> List[Dict[str, Any]]:
+        """The groups with their fp32 master copies in place of the parameters; empty without masters.  A view: the masters live in
+        ``state[p]["master"]`` alone, which is what the step updates, ``state_dict`` saves and a resuming program assigns."""
+        if not self.mixed_precision:
+            return []
+        return [{**group, "params": [self._master(p) for p in group["params"]]} for group in self.param_groups]
 
     @property
     def mixed_precision(self) -> bool:
@@ -96,8 +101,7 @@ class Muon(torch.optim.Optimizer):
         return True
 
     def __getstate__(self) -> Dict[str, Any]:  # of copies and pickles
-        return {**super().__getstate__(), "precision": self.precision, "products": self.products, "_dtype": self._dtype,
-                "fp32_param_groups": self.fp32_param_groups}
+        return {**super().__getstate__(), "precision": self.precision, "products": self.products, "_dtype": self._dtype}
 
     # ------------------------------------------------------------------ groups and state
 
@@ -139,12 +143,21 @@ class Muon(torch.optim.Optimizer):
         if p.shape[-2] % blocks:
             raise ValueError(f"{p.shape[-2]} rows cannot be split into {blocks} blocks")
 
-    def _add_masters(self, group: Dict[str, Any]) -> None:
-        masters = []
-        for p in group["params"]:
-            self.state[p]["master"] = p.detach().to(torch.float32, memory_format=torch.contiguous_format, copy=True)
-            masters.append(self.state[p]["master"])
-        self.fp32_param_groups.append({**{k: v for k, v in group.items() if k != "params"}, "params": masters})
+    def _master(self, p: torch.Tensor) -> torch.Tensor:
+        """The fp32 master copy of a parameter; made from the parameter where its state has none (a state of another precision)."""
+        state = self.state[p]
+        master = state.get("master")
+        if master is None:
+            if p.is_cuda and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("a graph that makes a master copy would make it again at every replay: step once before the capture")
+            master = state["master"] = p.detach().to(torch.float32, memory_format=torch.contiguous_format, copy=True)
+        return master
+
+    def _make_masters(self, groups: Sequence[Dict[str, Any]]) -> None:
+        if self.mixed_precision:
+            for group in groups:
+                for p in group["params"]:
+                    self._master(p)
 
     def add_param_group(self, param_group: Dict[str, Any]) -> None:
         super().add_param_group(param_group)
@@ -155,35 +168,29 @@ class Muon(torch.optim.Optimizer):
             except ValueError:
                 self.param_groups.pop()
                 raise
-            if self.mixed_precision:
-                self._add_masters(group)
+            self._make_masters([group])
 
     def load_state_dict(self, state_dict: Dict[str, Any]) -> None:
         """Restores momentum and master copies bit for bit (torch alone casts them to the parameters' dtype)."""
         super().load_state_dict(state_dict)
         saved = state_dict["state"]
-        self.fp32_param_groups = []
         for group, saved_group in zip(self.param_groups, state_dict["param_groups"]):
             self._check_group(group)
             for p, pid in zip(group["params"], saved_group["params"]):
                 for key in ("momentum_buffer", "master"):
                     if key in saved.get(pid, {}):
                         self.state[p][key] = saved[pid][key].detach().to(device=p.device, dtype=torch.float32, copy=True).contiguous()
-            if self.mixed_precision:
-                masters = []
-                for p in group["params"]:
-                    if "master" not in self.state[p]:
-                        self.state[p]["master"] = p.detach().to(torch.float32, memory_format=torch.contiguous_format, copy=True)
-                    masters.append(self.state[p]["master"])
-                self.fp32_param_groups.append({**{k: v for k, v in group.items() if k != "params"}, "params": masters})
+                if not self.mixed_precision and p in self.state:
+                    self.state[p].pop("master", None)  # no step would keep it up to date
+        self._make_masters(self.param_groups)
 
     # ------------------------------------------------------------------ the step
 
-    def _gather(self, gi: int, group: Dict[str, Any]) -> Dict[torch.device, Tuple[List[torch.Tensor], ...]]:
-        """(parameters or masters, gradients, momenta, copies) of what takes part, by device.  Changes nothing but for momenta that are made."""
+    def _gather(self, group: Dict[str, Any]) -> Dict[torch.device, Tuple[List[torch.Tensor], ...]]:
+        """(parameters or masters, gradients, momenta, copies) of what takes part, by device.  Changes nothing but for momenta and masters that are made."""
         batches: Dict[torch.device, Tuple[List[torch.Tensor], ...]] = {}
-        masters = self.fp32_param_groups[gi]["params"] if self.mixed_precision else None
-        for k, p in enumerate(group["params"]):
+        mixed = self.mixed_precision
+        for p in group["params"]:
             grad = p.grad
             if grad is None:
                 continue
@@ -195,10 +202,12 @@ class Muon(torch.optim.Optimizer):
                 if torch.cuda.is_current_stream_capturing():
                     raise RuntimeError("a graph that makes the momentum would clear it at every replay: step once before the capture")
                 buf = state["momentum_buffer"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
+            if not mixed:
+                state.pop("master", None)  # assigned with a state of another precision: no step keeps it up to date
             lists = batches.get(p.device)
             if lists is None:
                 lists = batches[p.device] = ([], [], [], [])
-            lists[0].append(p if masters is None else masters[k])
+            lists[0].append(self._master(p) if mixed else p)
             lists[1].append(grad)
             lists[2].append(buf)
             lists[3].append(p)
@@ -262,7 +271,7 @@ class Muon(torch.optim.Optimizer):
         calls = []
         for gi, group in enumerate(self.param_groups):
             self._check_group(group, gi)
-            for device, lists in self._gather(gi, group).items():
+            for device, lists in self._gather(group).items():
                 calls.append((group, device, self._rows(gi, group, device, lists), *scale_arguments(scale, device)))
         if torch.autograd._profiler_enabled():
             with torch.autograd.profiler.record_function("fairscale_amd::muon::fused_step"):

@@ -362,3 +362,74 @@ def test_optimizer_is_copied_whole():
         with pytest.raises(RuntimeError):
             p.grad = torch.zeros_like(p)
             twin.step()  # not on a GPU; gets as far as the check
+
+
+# ---- master copies: what is saved is what is stepped ----------------------------------------------------------------
+
+def mixed_optimizer(grad=True):
+    p = torch.nn.Parameter(torch.randn(6, 4).to(torch.bfloat16))
+    if grad:
+        p.grad = torch.ones_like(p)
+    return p, Muon([p])
+
+
+def stepped(opt, p):
+    """What the step of a parameter's group takes as parameter, momentum and copy."""
+    parameters, _, momenta, copies = opt._gather(opt.param_groups[0])[p.device]
+    return parameters[0], momenta[0], copies[0]
+
+
+def test_a_state_assigned_to_a_parameter_is_the_one_that_is_stepped():
+    """As OSS resumes: ``optimizer.state[p] = {...}``."""
+    p, opt = mixed_optimizer()
+    state = {"master": torch.full((6, 4), 7.0), "momentum_buffer": torch.full((6, 4), 3.0)}
+    opt.state[p] = state
+    assert all(a is b for a, b in zip(stepped(opt, p), (state["master"], state["momentum_buffer"], p)))
+    assert opt.fp32_param_groups[0]["params"][0] is state["master"] is opt.state[p]["master"]
+    assert opt.state_dict()["state"][0]["master"] is state["master"], "and the one that is saved"
+    opt.state[p]["master"] = other = torch.full((6, 4), 8.0)
+    assert stepped(opt, p)[0] is other and opt.fp32_param_groups[0]["params"][0] is other
+
+
+@pytest.mark.parametrize("grad", [True, False])
+def test_a_state_assigned_without_a_master_gets_one_from_the_parameter(grad):
+    """As a checkpoint of another precision is restored; with or without a gradient by then."""
+    p, opt = mixed_optimizer(grad)
+    with torch.no_grad():
+        p.fill_(5.0)
+    opt.state[p] = {"momentum_buffer": torch.zeros(6, 4)}
+    master = opt.fp32_param_groups[0]["params"][0]
+    assert torch.equal(master, torch.full((6, 4), 5.0)) and master is opt.state[p]["master"] is opt.fp32_param_groups[0]["params"][0]
+    if grad:
+        assert stepped(opt, p)[0] is master
+
+
+@pytest.mark.parametrize("bad", [torch.zeros(6, 4, dtype=torch.float16), torch.zeros(4, 6), torch.zeros(4, 6).t(), torch.zeros(6, 4, device="meta")], ids=["dtype", "shape", "strides", "device"])
+def test_a_master_that_the_step_cannot_take_is_refused(bad):
+    p, opt = mixed_optimizer()
+    opt.state[p]["momentum_buffer"] = torch.zeros(6, 4)
+    opt.state[p]["master"] = bad
+    parameters, grads, momenta, copies = opt._gather(opt.param_groups[0])[p.device]
+    assert parameters[0] is bad
+    with pytest.raises(RuntimeError):
+        opt.step()
+
+
+def test_groups_of_masters_show_the_settings_in_use():
+    p, opt = mixed_optimizer()
+    opt.param_groups[0]["lr"] = 0.25
+    assert opt.fp32_param_groups[0]["lr"] == 0.25
+
+
+def test_a_master_that_nothing_steps_is_not_carried_on():
+    """A checkpoint with masters restored without them, stepped, saved and restored with them again must not bring the old ones back."""
+    p, opt = mixed_optimizer()
+    saved = opt.state_dict()
+    q = torch.nn.Parameter(p.detach().clone())
+    other = Muon([q], precision=Precision.MEMORY_EFFICIENT_MIXED_PRECISION)
+    other.load_state_dict(saved)
+    assert "master" not in other.state_dict()["state"].get(0, {})
+    other.state[q] = {"master": torch.zeros(6, 4), "momentum_buffer": torch.zeros(6, 4)}
+    q.grad = torch.ones_like(q)
+    stepped(other, q)
+    assert "master" not in other.state_dict()["state"][0]

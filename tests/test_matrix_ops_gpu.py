@@ -636,3 +636,58 @@ def test_matrix_of_more_than_2_31_elements(tall):
     assert ((got - want).abs() <= bound).all()
     at(out).zero_()
     assert int(torch.count_nonzero(out)) == 0
+
+
+# ---- states that are assigned, as a sharded optimizer's resume does --------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=str)
+def test_muon_resumes_from_an_assigned_state(dtype):
+    """``optimizer.state[p] = {...}`` in a new program, then steps, a checkpoint and another resume: each bit as in the program that went on."""
+    p = torch.nn.Parameter(randn(40, 60, dtype=dtype))
+    opt = Muon([p])
+    grads = [randn(40, 60, seed=k + 1, dtype=dtype) for k in range(4)]
+    for k in range(2):
+        p.grad = grads[k].clone()
+        opt.step()
+    for resume in range(2):
+        q = torch.nn.Parameter(torch.zeros_like(p))  # the masters alone carry the values
+        other = Muon([q])
+        other.state[q] = {key: value.clone() for key, value in opt.state_dict()["state"][0].items()}
+        for o, w in ((opt, p), (other, q)):
+            w.grad = grads[2 + resume].clone()
+            o.step()
+        assert torch.equal(p.detach(), q.detach())
+        saved, kept = other.state_dict()["state"][0], opt.state_dict()["state"][0]
+        assert torch.equal(saved["master"], kept["master"]) and torch.equal(saved["momentum_buffer"], kept["momentum_buffer"])
+        assert torch.equal(saved["master"].to(dtype), q.detach())
+        p, opt = q, other
+
+
+def test_muon_refuses_masters_it_cannot_step_and_changes_nothing():
+    p = torch.nn.Parameter(randn(20, 30, dtype=torch.bfloat16))
+    opt = Muon([p])
+    p.grad = randn(20, 30, seed=1, dtype=torch.bfloat16)
+    opt.step()
+    keep, momentum, good = p.detach().clone(), opt.state[p]["momentum_buffer"].clone(), opt.state[p]["master"]
+    for bad in (good.half(), good[:4], good.cpu(), torch.zeros(30, 20, device="cuda").t(), opt.state[p]["momentum_buffer"]):
+        opt.state[p]["master"] = bad
+        with pytest.raises(RuntimeError):
+            opt.step()
+        assert torch.equal(p.detach(), keep) and torch.equal(opt.state[p]["momentum_buffer"], momentum)
+
+
+def test_muon_refuses_to_make_a_master_inside_a_capture():
+    p = torch.nn.Parameter(randn(8, 8, dtype=torch.float16))
+    p.grad = randn(8, 8, seed=1, dtype=torch.float16)
+    opt = Muon([p])
+    opt.step()
+    keep = p.detach().clone()
+    opt.state[p] = {"momentum_buffer": opt.state[p]["momentum_buffer"]}
+    spare = torch.zeros(1, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        spare.add_(1.0)
+        with pytest.raises(RuntimeError, match="capture"):
+            opt.step()
+    torch.cuda.synchronize()
+    assert torch.equal(p.detach(), keep)
