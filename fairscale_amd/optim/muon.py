@@ -171,17 +171,29 @@ class Muon(torch.optim.Optimizer):
             self._make_masters([group])
 
     def load_state_dict(self, state_dict: Dict[str, Any]) -> None:
-        """Restores momentum and master copies bit for bit (torch alone casts them to the parameters' dtype)."""
-        super().load_state_dict(state_dict)
-        saved = state_dict["state"]
-        for group, saved_group in zip(self.param_groups, state_dict["param_groups"]):
-            self._check_group(group)
-            for p, pid in zip(group["params"], saved_group["params"]):
-                for key in ("momentum_buffer", "master"):
-                    if key in saved.get(pid, {}):
-                        self.state[p][key] = saved[pid][key].detach().to(device=p.device, dtype=torch.float32, copy=True).contiguous()
-                if not self.mixed_precision and p in self.state:
-                    self.state[p].pop("master", None)  # no step would keep it up to date
+        """Restores momentum and master copies bit for bit (torch alone casts them to the parameters' dtype).
+
+        Settings that a checkpoint does not hold (``row_blocks`` in one of ``torch.optim.Muon``) stay as they are.  All of it is
+        checked before anything is replaced: a checkpoint that is refused leaves the optimizer as it was.
+        """
+        saved_groups = state_dict["param_groups"]
+        if [len(g["params"]) for g in saved_groups] != [len(g["params"]) for g in self.param_groups]:
+            raise ValueError("the checkpoint's parameter groups are not those of the optimizer")
+        saved_groups = [{**{name: group[name] for name in _SETTINGS}, **saved} for group, saved in zip(self.param_groups, saved_groups)]
+        restored = []  # (parameter, key, tensor)
+        for group, saved in zip(self.param_groups, saved_groups):
+            self._check_group({**saved, "params": group["params"]})
+            for p, pid in zip(group["params"], saved["params"]):
+                state = state_dict["state"].get(pid, {})
+                for key in ("momentum_buffer", "master") if self.mixed_precision else ("momentum_buffer",):
+                    if key in state:
+                        restored.append((p, key, state[key].detach().to(device=p.device, dtype=torch.float32, copy=True).contiguous()))
+        super().load_state_dict({**state_dict, "param_groups": saved_groups})
+        for p, key, tensor in restored:
+            self.state[p][key] = tensor
+        if not self.mixed_precision:
+            for state in self.state.values():
+                state.pop("master", None)  # no step would keep it up to date
         self._make_masters(self.param_groups)
 
     # ------------------------------------------------------------------ the step

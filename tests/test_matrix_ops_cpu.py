@@ -433,3 +433,55 @@ def test_a_master_that_nothing_steps_is_not_carried_on():
     q.grad = torch.ones_like(q)
     stepped(other, q)
     assert "master" not in other.state_dict()["state"][0]
+
+
+# ---- checkpoints ------------------------------------------------------------------------------------------------------
+
+def test_a_checkpoint_of_torchs_optimizer_is_taken():
+    """Its groups have no ``row_blocks``: what a checkpoint does not hold stays as this program has it."""
+    p, q = torch.nn.Parameter(torch.randn(6, 4)), torch.nn.Parameter(torch.randn(5, 4))
+    theirs = torch.optim.Muon([{"params": [p]}, {"params": [q], "lr": 0.5}], lr=0.25, momentum=0.75)
+    p.grad, q.grad = torch.randn(6, 4), torch.randn(5, 4)
+    theirs.step()
+    saved = theirs.state_dict()
+    assert "row_blocks" not in saved["param_groups"][0]
+    ours = Muon([{"params": [torch.nn.Parameter(p.detach().clone())], "row_blocks": 3}, {"params": [torch.nn.Parameter(q.detach().clone())]}])
+    ours.load_state_dict(saved)
+    assert [(g["lr"], g["momentum"], g["row_blocks"]) for g in ours.param_groups] == [(0.25, 0.75, 3), (0.5, 0.75, 1)]
+    for group, w in zip(ours.param_groups, (p, q)):
+        assert torch.equal(ours.state[group["params"][0]]["momentum_buffer"], theirs.state[w]["momentum_buffer"])
+        ours._check_group(group, 0)
+
+
+@pytest.mark.parametrize("precision", [Precision.MIXED_PRECISION, Precision.MEMORY_EFFICIENT_MIXED_PRECISION], ids=["mixed", "memory_efficient"])
+@pytest.mark.parametrize("change", [dict(lr=-1.0), dict(momentum=1.0), dict(eps=0.0), dict(adjust_lr_fn="other"), dict(row_blocks=4), dict(ns_steps=0),
+                                    dict(ns_coefficients=(50.0, 0.0, 0.0)), dict(lr=None), "group", "parameter", "state"], ids=str)
+def test_a_refused_checkpoint_changes_nothing(precision, change):
+    def make():
+        p, q = torch.nn.Parameter(torch.randn(6, 4).half()), torch.nn.Parameter(torch.randn(6, 4).half())
+        opt = Muon([{"params": [p], "row_blocks": 2}, {"params": [q]}], lr=0.5, precision=precision)
+        for w in (p, q):
+            opt.state[w]["momentum_buffer"] = torch.randn(6, 4)
+        return opt
+
+    opt, other = make(), make()
+    saved = copy.deepcopy(other.state_dict())
+    saved["param_groups"][0]["lr"] = 0.125
+    if change == "group":
+        saved["param_groups"].pop()
+    elif change == "parameter":
+        saved["param_groups"][1]["params"].append(2)
+    elif change == "state":
+        saved["state"][1]["momentum_buffer"] = "missing"
+    else:
+        saved["param_groups"][1].update(change)
+    groups, states = [dict(g) for g in opt.param_groups], {w: dict(st) for w, st in opt.state.items()}
+    masters = [w for g in opt.fp32_param_groups for w in g["params"]]
+    with pytest.raises((ValueError, TypeError, AttributeError)):
+        opt.load_state_dict(saved)
+    assert opt.param_groups == groups
+    assert {w: dict(st) for w, st in opt.state.items()}.keys() == states.keys()
+    assert all(opt.state[w][key] is value for w, st in states.items() for key, value in st.items())
+    assert all(a is b for a, b in zip(masters, [w for g in opt.fp32_param_groups for w in g["params"]]))
+    opt.load_state_dict(other.state_dict())
+    assert opt.param_groups[0]["lr"] == 0.5
