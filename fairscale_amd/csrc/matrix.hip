@@ -93,7 +93,9 @@ int exponent_for(double bound) {  // the largest k with bound * 2^k <= 60000 (ha
 }
 
 // How large the eigenvalues of those matrices can be at every step, when the singular values of X0 are in [0, 1].  2 % a step stands
-// for what rounding adds.
+// for what its rounding adds: with 11-bit products (local_error below) at most 1.76 % of the largest value that an odd polynomial of
+// fifth degree takes on the interval, reached by Chebyshev's 5 x - 20 x^3 + 16 x^5.  Errors of earlier steps need no room: the bound is
+// that of every value in the interval, and so of the one that was moved.
 int step_bounds(const FsOrthOptions& o, std::vector<StepNumbers>& numbers) {
     const double a = o.a, b = o.b, c = o.c;
     const auto q = [&](double t) { return a + t * (b + t * c); };
@@ -121,6 +123,35 @@ int step_bounds(const FsOrthOptions& o, std::vector<StepNumbers>& numbers) {
         numbers.push_back(n);
     }
     return FSADAM_OK;
+}
+
+// What 11-bit products can do to a singular value.  With each of them off by at most u = 2^-11 of itself -- X's first half (d), A (e)
+// and B (f) -- a step is off, to first order, by
+//     x ((b x^2 + 2 c x^4) (2 d + e) + (b x^2 + c x^4) (f + d)),
+// and multiplies what was off before by its slope a + 3 b x^2 + 5 c x^4.  That is what happens to a matrix of one entry in a row and
+// column, or of rank one with entries of one size, where all roundings of a kind are alike; in others they average.  The usual
+// coefficients and five steps: 0.057 (the worst of 2e5 singular values with these roundings made: 0.029; 2e-3 of the norm for Gaussian
+// matrices).  Slopes over 1 multiply it: 0.094 for six steps, 0.62 for five steps of (4.0848, -6.8946, 2.9270).  Above 1/16 the products
+// take 22 bits, whatever was asked for.  256 values tell it to 4 % there.
+constexpr double kMostHalfError = 1.0 / 16;
+int products_of(const FsOrthOptions& o) {
+    if (o.products == FSADAM_PRODUCTS_SPLIT) return FSADAM_PRODUCTS_SPLIT;
+    const double a = o.a, b = o.b, c = o.c, u = 0x1p-11;
+    constexpr int kValues = 256;
+    double x[kValues], error[kValues];
+    for (int k = 0; k < kValues; ++k) x[k] = (k + 1.0) / kValues, error[k] = 0.0;
+    for (int s = 0; s < o.steps; ++s) {
+        int over = 0;
+        for (int k = 0; k < kValues; ++k) {
+            const double t = x[k] * x[k], in_a = t * (b + 2.0 * c * t), in_b = t * (b + c * t);
+            const double local_error = u * std::fabs(x[k]) * (std::fabs(2.0 * in_a + in_b) + std::fabs(in_a) + std::fabs(in_b));
+            error[k] = error[k] * std::fabs(a + t * (3.0 * b + 5.0 * c * t)) + local_error;
+            x[k] *= a + in_b;
+            over |= !(error[k] <= kMostHalfError);
+        }
+        if (over) return FSADAM_PRODUCTS_SPLIT;
+    }
+    return FSADAM_PRODUCTS_HALF;
 }
 
 int check_options(const FsOrthOptions* o) {
@@ -199,10 +230,9 @@ struct Source {  // what a list entry's row starts from
     int src_size, dst_size, copy_size;
 };
 
-// Matrices of a short side up to this are always multiplied to 22 bits.  The error of 11-bit products is about 2e-3 of the
-// result where it averages over many singular values, but a matrix that has few of them can be off by 2 % (rounding A, B
-// and X by 2^-11 each moves b x^3 + c x^5 by up to 32 * 2^-11 at x = 1); and their products are too small to be what a
-// call waits for.
+// Matrices of a short side up to this are always multiplied to 22 bits: their products are too small to be what a call waits for,
+// and few singular values are where the error of 11 bits averages least (products_of; larger matrices can have few as well, so this is
+// no promise about the error).
 constexpr int64_t kAlwaysSplit = 128;
 
 // A Gram matrix of few tiles and long inner products keeps a few compute units busy for long: parts of kPartDepth are summed by
@@ -215,7 +245,9 @@ int gram_parts(int64_t s64, int64_t l64) {
 
 bool resident(const Source& in) { return resident_fits(std::min(in.rows, in.cols), std::max(in.rows, in.cols)); }
 
-void make_chunks(const std::vector<Source>& all, int asked, std::vector<Chunk>& chunks) {
+void make_chunks(const std::vector<Source>& all, const FsOrthOptions& options, std::vector<Chunk>& chunks) {
+  const bool large = std::any_of(all.begin(), all.end(), [](const Source& in) { return std::min(in.rows, in.cols) > kAlwaysSplit; });
+  const int asked = large ? products_of(options) : options.products;
   for (int products : {FSADAM_PRODUCTS_HALF, FSADAM_PRODUCTS_SPLIT}) {
     bool fresh = true;  // a chunk is of one kind
     for (const Source& in : all) {
@@ -272,7 +304,7 @@ struct Residents {
 struct Plan {
     Residents residents;
     std::vector<Chunk> chunks;
-    Plan(const std::vector<Source>& list, int products) {
+    Plan(const std::vector<Source>& list, const FsOrthOptions& options) {
         for (const Source& in : list) {
             if (!resident(in)) continue;
             const int s = (int)std::min(in.rows, in.cols), l = (int)std::max(in.rows, in.cols);
@@ -286,7 +318,7 @@ struct Plan {
             residents.matrices += in.batch;
             residents.lds_bytes = std::max(residents.lds_bytes, (int)up(s, 32) * (resident_pitch(s) + resident_pitch(l)) * 4);
         }
-        make_chunks(list, products, chunks);
+        make_chunks(list, options, chunks);
     }
     int64_t workspace() const {
         int64_t bytes = residents.bytes();  // their table is done with when the chunks begin
@@ -671,7 +703,7 @@ int fsadam_orth_workspace(const FsMatrix* matrices, int64_t n, const FsOrthOptio
         if (rc) return rc;
         std::vector<Source> list;
         if ((rc = sources_of(matrices, n, 1, list))) return rc;
-        *bytes = Plan(list, options->products).workspace();
+        *bytes = Plan(list, *options).workspace();
         return FSADAM_OK;
     });
 }
@@ -684,7 +716,7 @@ int fsadam_orthogonalize(const FsMatrix* matrices, int64_t n, int type, const Fs
         if (rc) return rc;
         std::vector<Source> list;
         if ((rc = sources_of(matrices, n, size_of(type), list))) return rc;
-        const Plan plan(list, options->products);
+        const Plan plan(list, *options);
         Call call{};
         call.src_type = call.dst_type = type;
         call.copy_type = -1;
@@ -700,7 +732,7 @@ int fsadam_muon_workspace(const FsMuonTensor* tensors, int64_t n, const FsOrthOp
         if (rc) return rc;
         std::vector<Source> list;
         if ((rc = sources_of(tensors, n, 1, 1, 0, 0.0, list))) return rc;
-        *bytes = Plan(list, options->products).workspace();
+        *bytes = Plan(list, *options).workspace();
         return FSADAM_OK;
     });
 }
@@ -718,7 +750,7 @@ int fsadam_muon_step(const FsMuonTensor* tensors, int64_t n, int param_type, int
         if ((rc = check_momentum(momentum, scale, scale_dev))) return rc;
         std::vector<Source> list;
         if ((rc = sources_of(tensors, n, size_of(param_type), size_of(grad_type), mixed ? 2 : 0, lr, list))) return rc;
-        const Plan plan(list, options->products);
+        const Plan plan(list, *options);
         Call call{};
         call.step = true;
         call.src_type = grad_type;

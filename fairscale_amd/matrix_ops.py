@@ -192,9 +192,14 @@ def orthogonalize(matrices: Sequence[torch.Tensor], *, steps: int = 5, coefficie
         matrices: tensors of one device and dtype (fp32, fp16 or bf16) with at least two dimensions; leading dimensions
             count matrices (experts, heads: ``w.view(heads, -1, w.shape[-1])``).  Rows or columns must have neighbouring
             elements: slices of rows or columns and transposed matrices are taken as they are, others are refused.
-        products: ``"half"`` multiplies 11 bits of the operands (error about 2e-3 of the result's norm), ``"split"`` 22 bits
-            (errors like fp32 products, at three times the matrix work; always taken where the short side is 128 or less).
-            None: as many as the results can hold, i.e. ``"half"`` for bf16 and ``"split"`` for fp16 and fp32.
+        products: ``"split"`` multiplies 22 bits of the operands: errors like fp32 products, at three times the matrix work.
+            ``"half"`` multiplies 11 bits.  With the default coefficients and steps its error is about 2e-3 of the result's norm, the
+            size of bf16's own rounding, where the roundings average over many singular directions (Gaussian matrices 2e-3, some
+            non-zero rows or equal rows up to 4e-3); it is up to 3e-2 for matrices of a few entries, diagonal ones and those of rank one
+            with entries of one size.  22 bits are taken in its place where the short side is 128 or less and for coefficients and
+            steps that would multiply the error (a first-order bound over 1/16: six of the default steps).
+            None: ``"half"`` for bf16, ``"split"`` for fp16 and fp32.  Ask for ``"split"`` where bf16 matrices of few or aligned
+            directions have to be exact to their rounding.
         out: tensors to write the results to (of the same shapes, dtype and order of strides).  Each may be its own matrix, but share
             memory with no other one of the call; side by side in the columns of one tensor is no sharing.
     """

@@ -44,8 +44,9 @@ class Muon(torch.optim.Optimizer):
             fp32 master copies in ``fp32_param_groups``) or MEMORY_EFFICIENT_MIXED_PRECISION (fp16 or bf16, no master copies).
             The momentum is fp32 in all of them; PURE_FP16 is refused, since an average that takes in 5 % of a
             gradient a step loses most of it in 11 bits.  Inferred from the first parameter when None, as ``Adam`` does.
-        products: ``"half"`` or ``"split"`` (see ``orthogonalize``).  None: ``"split"`` where the parameters are updated in
-            fp32, ``"half"`` where they are stored in 16 bits and round its error away.
+        products: ``"half"`` or ``"split"`` (see ``orthogonalize`` for what each is off by).  None: ``"split"`` where the parameters
+            are updated in fp32, ``"half"`` where they are stored in 16 bits without masters: the update is then off by about 2e-3 of its
+            norm, for gradients of few entries or aligned directions by up to 3e-2.
     """
 
     def __init__(

@@ -319,9 +319,14 @@ int fsadam_momentum_pass(const FsMomentumTensor* tensors, int64_t n_tensors, int
  *     X <- a X + (b X X^T + c (X X^T)^2) X         (X^T X on the other side where rows > cols: the same values)
  * which sends each singular value x to a x + b x^3 + c x^5 and leaves the singular vectors.  A matrix of zeros gives
  * zeros (X is held to 2^-40: what is smaller than that beside max(|U|, eps) counts as 0), one with an entry that is not finite gives NaN in every entry; other matrices of the list are not touched by it.
- * products: how many bits of the operands the matrix products take (fp32 sums either way): FSADAM_PRODUCTS_HALF 11 (error of
- * the result about 2e-3 of its norm), FSADAM_PRODUCTS_SPLIT 22 (like fp32 products, about three times the work; always
- * taken for matrices of a short side up to 128).
+ * products: how many bits of the operands the matrix products take (fp32 sums either way).
+ *   FSADAM_PRODUCTS_SPLIT: 22.  Errors like those of fp32 products, about three times the work.
+ *   FSADAM_PRODUCTS_HALF: 11.  With the usual coefficients (3.4445, -4.7750, 2.0315) and five steps the result is off by about 2e-3 of its
+ *   norm where roundings average over many singular directions (Gaussian matrices 2.0e-3; some non-zero rows or equal rows 1.5e-3 to
+ *   4e-3), by up to 3e-2 where they do not: matrices of a few entries, of rank one with entries of one size (1e-2), diagonal ones.  To
+ *   first order no singular value of those is off by more than 0.057.  Other coefficients and steps are taken with 11 bits where that
+ *   bound is at most 1/16 for them (six steps of the usual ones: 0.094), otherwise, and for matrices of a short side up to 128, 22 bits are
+ *   taken instead.
  * Refused with FSADAM_EINVAL: coefficients that let singular values in [0, 1] grow past 1024 within the steps, steps
  * outside 1..32, eps that is not positive, sides or batches over 2^20, matrices of more than 2^34 elements. */
 #define FSADAM_PRODUCTS_HALF 1

@@ -485,3 +485,34 @@ def test_a_refused_checkpoint_changes_nothing(precision, change):
     assert all(a is b for a, b in zip(masters, [w for g in opt.fp32_param_groups for w in g["params"]]))
     opt.load_state_dict(other.state_dict())
     assert opt.param_groups[0]["lr"] == 0.5
+
+
+# ---- products of 11 bits ------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("coefficients, steps, halves", [
+    (M.COEFFICIENTS, 1, True), (M.COEFFICIENTS, 5, True), (M.COEFFICIENTS, 6, False), (M.COEFFICIENTS, 32, False), ((4.0848, -6.8946, 2.9270), 2, True),
+    ((4.0848, -6.8946, 2.9270), 3, False), ((4.0848, -6.8946, 2.9270), 5, False), ((5.0, -20.0, 16.0), 2, False), ((1.5, -0.5, 0.0), 32, True), ((1.0, 0.0, 0.0), 5, True),
+])
+def test_11_bits_are_taken_where_their_error_stays_small(coefficients, steps, halves):
+    """Otherwise the storage is that of 22 bits."""
+    sizes = {p: workspace(matrices((1, 300, 500)), options(steps, coefficients, products=p))[1] for p in (1, 2)}
+    assert (sizes[1] < sizes[2]) is halves and sizes[1] > 0
+
+
+def test_bound_of_11_bit_products_holds_for_one_singular_value_with_the_roundings_made():
+    x = torch.cat([torch.logspace(-3, 0, 300, dtype=torch.float64), torch.linspace(0.3, 1.0, 300, dtype=torch.float64)]).float().double()
+    a, b, c = M.COEFFICIENTS
+
+    def rounded(v):  # to 11 significant bits
+        m, e = torch.frexp(v)
+        return torch.ldexp(torch.round(m * 2048) / 2048, e)
+
+    exact, held = x.clone(), x.clone()
+    for _ in range(5):
+        first = rounded(held)
+        gram = rounded(first * first)
+        held = a * held + rounded(b * gram + c * gram * gram) * first
+        held = rounded(held) + rounded(held - rounded(held))
+        exact = a * exact + b * exact**3 + c * exact**5
+    error, bound = (held - exact).abs(), torch.tensor([M.half_bound(v, v) for v in x.tolist()])
+    assert (error <= bound).all() and error.max() > 0.01, "and it is not far from what happens"
