@@ -52,7 +52,9 @@ bool aligned(const void* p, uintptr_t bytes) { return reinterpret_cast<uintptr_t
 int64_t up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
 
 constexpr int64_t kMaxSide = 1 << 20;
-constexpr int64_t kMaxTiles = INT32_MAX / 2;  // of one launch
+// A launch takes fewer than 2^32 threads.
+constexpr int64_t most_workgroups(int64_t threads) { return UINT32_MAX / threads; }
+constexpr int64_t kMaxTiles = most_workgroups(512);  // of a chunk, of any kind: no launch over them has larger workgroups
 // Intermediate matrices of one chunk.  Enough for eight 4096 x 11008 matrices, whose products then have thousands of
 // tiles for the 256 compute units; a matrix that needs more gets what it needs.
 constexpr int64_t kChunkBytes = int64_t(4) << 30;
@@ -298,6 +300,9 @@ struct Residents {
     std::vector<ResidentRow> rows;
     int64_t matrices = 0;
     int lds_bytes = 0;  // of the largest
+    int check() const {
+        return matrices <= most_workgroups(kResidentThreads) ? FSADAM_OK : fail(FSADAM_EINVAL, "the list has too many matrices of a short side up to 128 for one call (2^22 or more)");
+    }
     int64_t bytes() const { return rows.size() > kResidentRowsPerLaunch ? up((int64_t)(rows.size() * sizeof(ResidentRow)), 256) : 0; }
 };
 
@@ -497,7 +502,6 @@ int run_chunk(const Chunk& c, const Call& call, void* workspace, hipStream_t str
 
 int run_residents(const Residents& r, const Call& call, void* workspace, hipStream_t stream) {
     if (r.rows.empty()) return FSADAM_OK;
-    if (r.matrices > kMaxTiles) return fail(FSADAM_EINVAL, "the list has too many matrices for one call");
     const FsOrthOptions& o = call.options;
     ResidentArgs k{};
     k.steps = o.steps;
@@ -539,7 +543,7 @@ int run_residents(const Residents& r, const Call& call, void* workspace, hipStre
 
 int run_call(const Plan& plan, Call& call, void* workspace, int64_t workspace_bytes, void* hip_stream) {
     int rc = step_bounds(call.options, call.numbers);
-    if (rc) return rc;
+    if (rc || (rc = plan.residents.check())) return rc;
     const std::vector<Chunk>& chunks = plan.chunks;
     const int64_t need = plan.workspace();
     if (need && (!workspace || !aligned(workspace, 256))) return fail(FSADAM_EINVAL, "the workspace must be a device pointer aligned to 256 bytes");
@@ -613,7 +617,8 @@ int momentum_rows(const FsMomentumTensor* t, int64_t n, std::vector<MomentumRow>
         rows.push_back({t[k].g, t[k].m, t[k].u, t[k].numel, chunks});
         chunks += up(t[k].numel, kMomentumElems) / kMomentumElems;
     }
-    if (chunks > kMaxTiles || n > kMaxTiles) return fail(FSADAM_EINVAL, "the list has too many elements for one call");
+    if (chunks > most_workgroups(kChunkThreads)) return fail(FSADAM_EINVAL, "the list has too many elements for one call (about 2^34 or more)");
+    if (n > most_workgroups(kNormThreads)) return fail(FSADAM_EINVAL, "the list has too many tensors for one call (2^22 or more)");
     return FSADAM_OK;
 }
 // The arguments of a launch are slow to read (they are not in the GPU's memory): worth it for a few workgroups only.
@@ -703,7 +708,9 @@ int fsadam_orth_workspace(const FsMatrix* matrices, int64_t n, const FsOrthOptio
         if (rc) return rc;
         std::vector<Source> list;
         if ((rc = sources_of(matrices, n, 1, list))) return rc;
-        *bytes = Plan(list, *options).workspace();
+        const Plan plan(list, *options);
+        if ((rc = plan.residents.check())) return rc;
+        *bytes = plan.workspace();
         return FSADAM_OK;
     });
 }
@@ -732,7 +739,9 @@ int fsadam_muon_workspace(const FsMuonTensor* tensors, int64_t n, const FsOrthOp
         if (rc) return rc;
         std::vector<Source> list;
         if ((rc = sources_of(tensors, n, 1, 1, 0, 0.0, list))) return rc;
-        *bytes = Plan(list, *options).workspace();
+        const Plan plan(list, *options);
+        if ((rc = plan.residents.check())) return rc;
+        *bytes = plan.workspace();
         return FSADAM_OK;
     });
 }

@@ -303,7 +303,9 @@ int fsadam_grad_pass_noalloc(const FsGradTensor* grads, int64_t n_tensors, int g
  * m is updated in place; u is stored in update_type (u may be g itself where the types are the same: updates over the
  * gradients).  norms_dev[t] (may be NULL) is the L2 norm of tensor t's update as stored, summed in fp64 in a fixed order;
  * found_inf_dev[0] (may be NULL) is set to 1.0f where a stored update is not finite; clear_found_inf != 0: and to 0.0f before.
- * scale_dev, when not NULL, is a device float[1] read in place of scale. */
+ * scale_dev, when not NULL, is a device float[1] read in place of scale.
+ * A call takes fewer than 2^22 tensors and 2^24 pieces of 1024 elements (of a tensor, its last one counted whole), i.e. about 2^34
+ * elements; longer lists are refused with FSADAM_EINVAL, by the workspace call too. */
 typedef struct FsMomentumTensor {
     const void* g;
     float* m;
@@ -328,7 +330,8 @@ int fsadam_momentum_pass(const FsMomentumTensor* tensors, int64_t n_tensors, int
  *   bound is at most 1/16 for them (six steps of the usual ones: 0.094), otherwise, and for matrices of a short side up to 128, 22 bits are
  *   taken instead.
  * Refused with FSADAM_EINVAL: coefficients that let singular values in [0, 1] grow past 1024 within the steps, steps
- * outside 1..32, eps that is not positive, sides or batches over 2^20, matrices of more than 2^34 elements. */
+ * outside 1..32, eps that is not positive, sides or batches over 2^20, matrices of more than 2^34 elements, and lists of 2^22 or more
+ * matrices that fit a compute unit's LDS (short side up to 128).  Longer lists of larger ones go through the workspace in parts. */
 #define FSADAM_PRODUCTS_HALF 1
 #define FSADAM_PRODUCTS_SPLIT 2
 typedef struct FsOrthOptions {

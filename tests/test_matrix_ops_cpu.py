@@ -516,3 +516,41 @@ def test_bound_of_11_bit_products_holds_for_one_singular_value_with_the_rounding
         exact = a * exact + b * exact**3 + c * exact**5
     error, bound = (held - exact).abs(), torch.tensor([M.half_bound(v, v) for v in x.tolist()])
     assert (error <= bound).all() and error.max() > 0.01, "and it is not far from what happens"
+
+
+# ---- what a launch can hold -----------------------------------------------------------------------------------------------
+
+def test_lists_longer_than_a_launch_are_refused_by_name():
+    """A launch takes fewer than 2^32 threads; nothing of a call may be enqueued before that is known."""
+    size = ctypes.c_int64()
+    most = ((1 << 32) - 1) // 256 * 1024  # elements of the momentum pass: four to a thread
+    for numel, rc in ((most, 0), (most + 1, -1), (1 << 40, -1)):
+        rows = momentum_rows(numel=numel)
+        assert L.fsadam_momentum_workspace(rows, 1, ctypes.byref(size)) == rc
+        if rc:
+            assert b"too many" in L.fsadam_last_error()
+            assert L.fsadam_momentum_pass(rows, 1, 0, 0, 0.9, 1, 1.0, None, None, None, 0, FAKE, 1 << 40, None) == -1 and b"too many" in L.fsadam_last_error()
+    halves = (_cabi.FsMomentumTensor * 2)()
+    for row in halves:
+        row.g, row.m, row.u, row.numel = FAKE, FAKE * 2, FAKE * 3, most // 2 + 1024
+    assert L.fsadam_momentum_workspace(halves, 2, ctypes.byref(size)) == -1 and b"too many" in L.fsadam_last_error()
+    many = (_cabi.FsMomentumTensor * (1 << 22))()  # one workgroup of 1024 threads to each norm
+    assert L.fsadam_momentum_workspace(many, (1 << 22) - 1, ctypes.byref(size)) == 0
+    assert L.fsadam_momentum_workspace(many, 1 << 22, ctypes.byref(size)) == -1 and b"too many" in L.fsadam_last_error()
+
+
+def test_more_small_matrices_than_a_launch_holds_are_refused_by_name():
+    opt = options()
+    for shapes, rc in (([(1 << 20, 4, 4)] * 3 + [((1 << 20) - 1, 4, 4)], 0), ([(1 << 20, 4, 4)] * 4, -1)):
+        rows = matrices(*shapes)
+        assert workspace(rows, opt)[0] == rc
+        if rc:
+            assert b"too many" in L.fsadam_last_error()
+            assert L.fsadam_orthogonalize(rows, len(rows), 0, ctypes.byref(opt), FAKE, 1 << 40, None) == -1 and b"too many" in L.fsadam_last_error()
+    steps = (_cabi.FsMuonTensor * 4)()
+    for row in steps:
+        row.p, row.g, row.m, row.batch, row.rows, row.cols, row.ratio = FAKE, FAKE * 2, FAKE * 3, 1 << 20, 4, 4, 1.0
+    size = ctypes.c_int64()
+    assert L.fsadam_muon_workspace(steps, 4, ctypes.byref(opt), ctypes.byref(size)) == -1 and b"too many" in L.fsadam_last_error()
+    assert L.fsadam_muon_step(steps, 4, 0, 0, -1, ctypes.byref(opt), 0.1, 0.9, 1, 0.0, 1.0, None, FAKE, 1 << 40, None) == -1 and b"too many" in L.fsadam_last_error()
+    assert workspace(matrices(*[(1 << 20, 300, 300)] * 8), opt)[0] == 0  # these go through the workspace in chunks
