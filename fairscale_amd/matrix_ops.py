@@ -37,7 +37,7 @@ def orth_options(steps: int, coefficients: Sequence[float], eps: float, products
         raise ValueError(f"coefficients must be three numbers (a, b, c), got {coefficients}")
     if products not in _PRODUCTS:
         raise ValueError(f"products must be 'half' or 'split', got {products!r}")
-    if int(steps) != steps:
+    if not -2**31 <= steps < 2**31 or int(steps) != steps:  # the call's own range is 1 to 32; what does not fit its field would be cut
         raise ValueError(f"steps must be a whole number, got {steps}")
     a, b, c = (float(v) for v in coefficients)
     return _cabi.FsOrthOptions(a, b, c, float(eps), int(steps), _PRODUCTS[products])

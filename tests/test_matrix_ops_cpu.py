@@ -554,3 +554,14 @@ def test_more_small_matrices_than_a_launch_holds_are_refused_by_name():
     assert L.fsadam_muon_workspace(steps, 4, ctypes.byref(opt), ctypes.byref(size)) == -1 and b"too many" in L.fsadam_last_error()
     assert L.fsadam_muon_step(steps, 4, 0, 0, -1, ctypes.byref(opt), 0.1, 0.9, 1, 0.0, 1.0, None, FAKE, 1 << 40, None) == -1 and b"too many" in L.fsadam_last_error()
     assert workspace(matrices(*[(1 << 20, 300, 300)] * 8), opt)[0] == 0  # these go through the workspace in chunks
+
+
+# ---- numbers that do not fit their field ----------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("steps", [2**32 + 5, -(2**32) + 5, 2**31, 2**63, math.inf, math.nan, 5.5])
+def test_steps_that_do_not_fit_are_refused(steps):
+    """Not taken as what is left of them in 32 bits."""
+    with pytest.raises(ValueError, match="steps"):
+        matrix_ops.orth_options(steps, M.COEFFICIENTS, 1e-7, "split")
+    with pytest.raises(ValueError, match="steps"):
+        Muon([torch.nn.Parameter(torch.zeros(4, 4))], ns_steps=steps)
