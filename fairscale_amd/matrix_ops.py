@@ -52,10 +52,19 @@ def scale_arguments(scale: Union[float, torch.Tensor], device: torch.device) -> 
     return 1.0, scale.data_ptr()
 
 
-def workspace_for(size_call, device: torch.device, *arguments) -> Tuple[torch.Tensor, int]:
+def workspace_size(size_call, *arguments) -> int:
     size = ctypes.c_int64(0)
     _cabi.check(size_call(*arguments, ctypes.byref(size)))
-    return torch.empty(max(int(size.value), 256), dtype=torch.uint8, device=device), int(size.value)
+    return int(size.value)
+
+
+def empty_workspace(size: int, device: torch.device) -> torch.Tensor:
+    return torch.empty(max(size, 256), dtype=torch.uint8, device=device)
+
+
+def workspace_for(size_call, device: torch.device, *arguments) -> Tuple[torch.Tensor, int]:
+    size = workspace_size(size_call, *arguments)
+    return empty_workspace(size, device), size
 
 
 def refuse_shared(written: Sequence[torch.Tensor], read: Sequence[torch.Tensor] = ()) -> None:

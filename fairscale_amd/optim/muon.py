@@ -15,7 +15,7 @@ import numpy as np
 import torch
 
 from .. import _cabi
-from ..matrix_ops import NS_COEFFICIENTS, TYPE_CODE, fill_rows, orth_options, refuse_shared, rows_pointer, scale_arguments, workspace_for
+from ..matrix_ops import NS_COEFFICIENTS, TYPE_CODE, empty_workspace, fill_rows, orth_options, refuse_shared, rows_pointer, scale_arguments, workspace_size
 from .adam import Precision
 
 __all__ = ["Muon"]
@@ -288,21 +288,27 @@ class Muon(torch.optim.Optimizer):
                 calls.append((group, device, self._rows(gi, group, device, lists), *scale_arguments(scale, device)))
         if torch.autograd._profiler_enabled():
             with torch.autograd.profiler.record_function("fairscale_amd::muon::fused_step"):
-                for call in calls:
-                    self._launch(*call)
+                self._launch(calls)
         else:
-            for call in calls:
-                self._launch(*call)
+            self._launch(calls)
         return loss
 
-    def _launch(self, group: Dict[str, Any], device: torch.device, rows: np.ndarray, scale: float, scale_pointer: Optional[int]) -> None:
-        options = orth_options(group["ns_steps"], group["ns_coefficients"], group["eps"], self.products)
-        code = TYPE_CODE[self._dtype]
+    def _launch(self, calls: Sequence[Tuple[Dict[str, Any], torch.device, np.ndarray, float, Optional[int]]]) -> None:
         lib = _cabi.lib()
-        pointer = rows_pointer(rows, _cabi.FsMuonTensor)
-        with torch.cuda.device(device):
-            workspace, size = workspace_for(lib.fsadam_muon_workspace, device, pointer, len(rows), ctypes.byref(options))
-            _cabi.check(lib.fsadam_muon_step(
-                pointer, len(rows), _cabi.TYPE_F32 if self.mixed_precision else code, code, code if self.mixed_precision else -1, ctypes.byref(options),
-                float(group["lr"]), float(group["momentum"]), 1 if group["nesterov"] else 0, float(group["weight_decay"]), scale, scale_pointer,
-                workspace.data_ptr(), size, int(torch.cuda.current_stream(device).cuda_stream)))
+        code = TYPE_CODE[self._dtype]
+        # Every call's list is checked, and there is memory for all of them, before the first one runs: a refused step changes nothing.
+        # Calls of one device follow each other on its stream, so the largest workspace serves them all.
+        options, workspaces = [], {}
+        for group, device, rows, _, _ in calls:
+            options.append(orth_options(group["ns_steps"], group["ns_coefficients"], group["eps"], self.products))
+            size = workspace_size(lib.fsadam_muon_workspace, rows_pointer(rows, _cabi.FsMuonTensor), len(rows), ctypes.byref(options[-1]))
+            workspaces[device] = max(size, workspaces.get(device, 0))
+        for device, size in workspaces.items():
+            workspaces[device] = empty_workspace(size, device), size
+        for (group, device, rows, scale, scale_pointer), how in zip(calls, options):
+            with torch.cuda.device(device):
+                workspace, size = workspaces[device]
+                _cabi.check(lib.fsadam_muon_step(
+                    rows_pointer(rows, _cabi.FsMuonTensor), len(rows), _cabi.TYPE_F32 if self.mixed_precision else code, code,
+                    code if self.mixed_precision else -1, ctypes.byref(how), float(group["lr"]), float(group["momentum"]), 1 if group["nesterov"] else 0,
+                    float(group["weight_decay"]), scale, scale_pointer, workspace.data_ptr(), size, int(torch.cuda.current_stream(device).cuda_stream)))

@@ -691,3 +691,38 @@ def test_muon_refuses_to_make_a_master_inside_a_capture():
             opt.step()
     torch.cuda.synchronize()
     assert torch.equal(p.detach(), keep)
+
+
+# ---- groups ------------------------------------------------------------------------------------------------------------
+
+def test_muon_refuses_a_group_before_another_one_is_stepped():
+    """The second group's matrix has more rows than a call takes: the first group stays as it was."""
+    p, q = torch.nn.Parameter(randn(20, 30)), torch.nn.Parameter(torch.zeros((1 << 20) + 1, 1, device="cuda"))
+    p.grad, q.grad = randn(20, 30, seed=1), torch.ones_like(q)
+    keep = p.detach().clone()
+    opt = Muon([{"params": [p]}, {"params": [q]}])
+    for _ in range(2):
+        with pytest.raises(RuntimeError, match="2\\^20"):
+            opt.step()
+        assert torch.equal(p.detach(), keep) and (opt.state[p]["momentum_buffer"] == 0).all() and (q == 0).all()
+    q.grad = None
+    opt.step()
+    alone = torch.nn.Parameter(keep.clone())
+    alone.grad = p.grad
+    Muon([alone]).step()
+    assert torch.equal(p, alone)
+
+
+def test_muon_groups_of_different_sizes_share_a_workspace():
+    """Each bit as from an optimizer of its own: large before small, small before large, one that needs no workspace."""
+    shapes = [(300, 200), (700, 900), (40, 50), (150, 4000)]
+    ps, qs = ([torch.nn.Parameter(randn(*s)) for s in shapes] for _ in range(2))
+    for k, (p, q) in enumerate(zip(ps, qs)):
+        p.grad, q.grad = randn(*shapes[k], seed=k + 1), randn(*shapes[k], seed=k + 1)
+    opt = Muon([{"params": [p], "ns_steps": 5 - k % 2} for k, p in enumerate(ps)])
+    apart = [Muon([q], ns_steps=5 - k % 2) for k, q in enumerate(qs)]
+    for _ in range(3):
+        opt.step()
+        for o in apart:
+            o.step()
+    assert all(torch.equal(p, q) for p, q in zip(ps, qs))
