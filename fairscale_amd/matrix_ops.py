@@ -121,7 +121,8 @@ def momentum_pass(grads: Sequence[torch.Tensor], momenta: Sequence[torch.Tensor]
         scale: the gradients are divided by this: a float, or a one-element float32 tensor the kernel reads when it runs.
         updates: tensors to write the updates to, of one dtype (any of the three); each may be its own gradient, if
             their elements have one size, but share memory with nothing else.  Made in the gradients' dtype when None.
-        found_inf: float32[1] device tensor to raise; a zeroed one is made when None.
+        found_inf: float32[1] device tensor to raise; a zeroed one is made when None.  The momenta have taken the values in by then: gradients
+            that may not be finite go through ``grad_pass`` or a ``GradScaler`` first.
     """
     grads, momenta = list(grads), list(momenta)
     if len(grads) == 0:
