@@ -351,7 +351,7 @@ __device__ __forceinline__ void for_eights(int64_t begin, int64_t end, Each&& ea
 }
 
 // Bound by HBM: 2 + 4 bytes read and 2 + 4 written per element with 16-bit gradients and updates.  The matrices of a layer of 4096
-// with an FFN of 11008 (202 million elements): 376 us, 6.46 TB/s, where a plain copy of a tensor reaches 4.8 and this library's
+// with an FFN of 11008 (202 million elements): 374 us, 6.5 TB/s (382 us the call), where a plain copy of a tensor reaches 4.8 and this library's
 // parameter pass 6.7.  Short workgroups of one piece a thread, all loads before the first store, and stores that write through
 // the L2 (store_through) as in the parameter pass; the L2 would hold the lines until they are in the way of the reads.
 template <int GT, int UT, typename Table>
