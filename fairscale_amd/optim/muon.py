@@ -166,7 +166,7 @@ class Muon(torch.optim.Optimizer):
             group = self.param_groups[-1]
             try:
                 self._check_group(group)
-            except ValueError:
+            except Exception:
                 self.param_groups.pop()
                 raise
             self._make_masters([group])

@@ -565,3 +565,11 @@ def test_steps_that_do_not_fit_are_refused(steps):
         matrix_ops.orth_options(steps, M.COEFFICIENTS, 1e-7, "split")
     with pytest.raises(ValueError, match="steps"):
         Muon([torch.nn.Parameter(torch.zeros(4, 4))], ns_steps=steps)
+
+
+@pytest.mark.parametrize("change", [dict(lr=None), dict(momentum="much"), dict(ns_coefficients=5.0), dict(lr=-1.0), dict(row_blocks=math.inf)], ids=str)
+def test_a_refused_group_is_not_added(change):
+    opt = Muon([torch.nn.Parameter(torch.zeros(4, 4, dtype=torch.float16))])
+    with pytest.raises((ValueError, TypeError, OverflowError)):
+        opt.add_param_group({"params": [torch.nn.Parameter(torch.zeros(4, 4, dtype=torch.float16))], **change})
+    assert len(opt.param_groups) == len(opt.fp32_param_groups) == len(opt.state) == 1
