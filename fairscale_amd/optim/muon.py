@@ -32,8 +32,8 @@ class Muon(torch.optim.Optimizer):
 
     Arguments:
         params: parameters of one dtype with at least two dimensions, or groups of them.  The last two dimensions
-            are the matrix, leading ones count matrices (experts); a convolution's weight is passed as a view
-            of two dimensions.
+            are the matrix, leading ones count matrices (experts).  A convolution's weight is passed as a parameter of two
+            dimensions over its memory, ``Parameter(w.detach().view(len(w), -1))``, that is given ``w.grad.view(len(w), -1)`` before a step.
         lr, weight_decay, momentum, nesterov, ns_coefficients, eps, ns_steps: as in the formulas above and in
             ``fairscale_amd.optim.orthogonalize``.
         adjust_lr_fn: ``ratio`` by the matrix's shape: None or ``"original"`` sqrt(max(1, rows / cols)),

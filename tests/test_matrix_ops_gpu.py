@@ -726,3 +726,18 @@ def test_muon_groups_of_different_sizes_share_a_workspace():
         for o in apart:
             o.step()
     assert all(torch.equal(p, q) for p, q in zip(ps, qs))
+
+
+def test_muon_of_a_convolutions_weight():
+    """As the documentation says: a leaf of two dimensions over the weight's memory, which is given the weight's gradient before a step."""
+    conv = torch.nn.Conv2d(5, 12, 3).cuda()
+    flat = torch.nn.Parameter(conv.weight.detach().view(12, -1))
+    opt = Muon([flat], lr=0.1)
+    conv(randn(2, 5, 8, 8)).square().mean().backward()
+    before = conv.weight.detach().double().cpu().view(12, -1)
+    flat.grad = conv.weight.grad.view(12, -1)
+    opt.step()
+    want, _ = M.step(before, flat.grad, torch.zeros(12, 45), lr=0.1)
+    assert M.relative(conv.weight.view(12, -1), want) < 1e-5
+    with pytest.raises(ValueError, match="non-leaf"):
+        Muon([conv.weight.view(12, -1)])
