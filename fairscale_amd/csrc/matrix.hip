@@ -132,8 +132,8 @@ int step_bounds(const FsOrthOptions& o, std::vector<StepNumbers>& numbers) {
 //     x ((b x^2 + 2 c x^4) (2 d + e) + (b x^2 + c x^4) (f + d)),
 // and multiplies what was off before by its slope a + 3 b x^2 + 5 c x^4.  That is what happens to a matrix of one entry in a row and
 // column, or of rank one with entries of one size, where all roundings of a kind are alike; in others they average.  The usual
-// coefficients and five steps: 0.057 (the worst of 2e5 singular values with these roundings made: 0.029; 2e-3 of the norm for Gaussian
-// matrices).  Slopes over 1 multiply it: 0.094 for six steps, 0.62 for five steps of (4.0848, -6.8946, 2.9270).  Above 1/16 the products
+// coefficients and five steps: 0.057 (the worst of 4e5 singular values with these roundings made: 0.024, and 2.9 % of what a value is sent to;
+// Gaussian matrices 2e-3 of the norm).  Slopes over 1 multiply it: 0.094 for six steps, 0.62 for five steps of (4.0848, -6.8946, 2.9270).  Above 1/16 the products
 // take 22 bits, whatever was asked for.  256 values tell it to 4 % there.
 constexpr double kMostHalfError = 1.0 / 16;
 int products_of(const FsOrthOptions& o) {
